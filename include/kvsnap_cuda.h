@@ -1,7 +1,7 @@
 /*
  * kvsnap_cuda.h: the C ABI of kvsnap_b200/_native/_cuda_native.so.
  *
- * Two groups of entry points, all extern "C", plain pointers and sizes, no
+ * Three groups of entry points, all extern "C", plain pointers and sizes, no
  * torch types. Every int-returning call returns 0 on success and -1 on error,
  * with the message in the calling thread's kvsnap_cuda_error().
  *
@@ -20,6 +20,9 @@
  *    (or mapped pinned memory); packed-block addresses may be device memory or
  *    pinned host memory from cudaHostAlloc, which the kernels read and write in
  *    place over the host link.
+ *
+ * 3. The 8-bit paged KV cache (kvsnap_c8_*): appending to it, attention over
+ *    it, and conversion of blocks between it and a 16-bit cache.
  */
 #ifndef KVSNAP_CUDA_H
 #define KVSNAP_CUDA_H
@@ -332,6 +335,106 @@ int kvsnap_dp_ipc_close(void* ptr);
 int kvsnap_dp_scatter_verify_static(const kvsnap_span* spans, int nspans, uint64_t block_bytes,
                                     const int64_t* sources, const int64_t* blocks, int64_t n,
                                     const uint32_t* expect, uint32_t* status, int vec, int ctas, uintptr_t stream);
+
+/* ---- 3. the 8-bit paged KV cache ------------------------------------------------ */
+
+/*
+ * A layer's paged cache in 8 bits: e4m3 codes [2 sides, blocks, block_size,
+ * kv_heads, head_dim] (side 0 keys, 1 values; last axis contiguous, the other
+ * pitches in bytes and multiples of 16, as the base), and one float scale a
+ * block, side and KV head, scales[block][side][head], contiguous. A code c at
+ * scale s stands for c * s. Scales written here are powers of two: the
+ * smallest s >= 2^-126 with largest finite magnitude <= 448 s, and 0 for a
+ * block of zeros. No counterpart in the reference, which moves caches and
+ * never reads one.
+ */
+typedef struct kvsnap_c8_cache {
+    int64_t codes;            /* device address of block 0's first key code */
+    int64_t scales;           /* device address of scales[0][0][0] */
+    int64_t side_pitch, block_pitch, token_pitch, head_pitch;
+    int32_t blocks, block_size, kv_heads, head_dim;
+    int32_t device, reserved;
+} kvsnap_c8_cache;
+
+/*
+ * The sequences of one call. Sequence s owns the token rows start[s] ..
+ * start[s+1]-1 of the call's tensors; they are its last tokens, lengths[s]
+ * tokens long with them. Its token at position p lies in block
+ * table[s * table_pitch + p / block_size], slot p % block_size. Rows from
+ * start[seqs] on belong to nobody. A row whose position would be negative
+ * (lengths[s] below the row count, 0 for a padded entry) is not in the cache.
+ * All three arrays are device memory, read by the kernels, never by the host.
+ */
+typedef struct kvsnap_c8_batch {
+    int64_t table, start, lengths;      /* device addresses of int32 arrays */
+    int64_t table_pitch;                /* elements between the table's rows */
+    int32_t width;                      /* blocks a row of the table holds */
+    int32_t seqs, rows;                 /* sequences; token rows of the call's tensors */
+    int32_t max_query;                  /* no sequence has more rows than this */
+} kvsnap_c8_batch;
+
+/* 16-bit element types. */
+#define KVSNAP_C8_BF16 0
+#define KVSNAP_C8_FP16 1
+
+/* Status bits beside KVSNAP_DP_BAD_BLOCK (a table entry outside the cache). A
+   kernel that sets one has skipped what the bit is about, not faulted. */
+#define KVSNAP_C8_BAD_LENGTH 16u     /* lengths, start or max_query do not fit the table or the rows */
+#define KVSNAP_C8_BAD_POSITION 32u   /* a position behind the rotary table's end */
+
+/*
+ * Append: key and value rows [rows][kv_heads][head_dim] (token and head
+ * pitches in bytes, multiples of 16) into their pages. With rotary not NULL,
+ * keys are first rotated in 32 bits: rotary[p][i] = (cos, sin) of the angle of
+ * pair i at position p, i < rotary_dim / 2, floats; pair i is elements (i, i +
+ * rotary_dim / 2), or (2i, 2i + 1) with interleaved; elements from rotary_dim
+ * on pass unchanged. One rounding, to the code. With query not NULL its rows
+ * are rotated the same way into query_out, dense [rows][q_heads][head_dim].
+ * A page that already holds tokens of its sequence keeps its scale or grows it
+ * to what the new tokens need, and its older codes are then rounded again at
+ * the new scale; a page whose first slot is written starts anew. Slots behind
+ * the last token keep their codes. Infinities become the largest value the
+ * block's scale holds, NaN stays NaN. Two sequences that append in one call
+ * must not share the page they append to.
+ */
+int kvsnap_c8_append(const kvsnap_c8_cache* cache, const kvsnap_c8_batch* batch, int type, const void* key,
+                     int64_t key_token, int64_t key_head, const void* value, int64_t value_token,
+                     int64_t value_head, const void* query, int64_t query_token, int64_t query_head, int q_heads,
+                     void* query_out, const float* rotary, int64_t positions, int rotary_dim, int interleaved,
+                     uint32_t* status, uintptr_t stream);
+
+/*
+ * Attention of query rows [rows][q_heads][head_dim] over their sequences'
+ * cached tokens: out[i][h] = sum_j softmax_j(scale * q.k_j) v_j over positions j
+ * up to the row's own. Query heads g * q_heads / kv_heads .. share KV head g.
+ * A row that sees no token is zeros; rows that belong to nobody are not
+ * written. out is dense and of the query's type.
+ */
+int kvsnap_c8_attend(const kvsnap_c8_cache* cache, const kvsnap_c8_batch* batch, int type, const void* query,
+                     int64_t query_token, int64_t query_head, int q_heads, float scale, void* out, uint32_t* status,
+                     uintptr_t stream);
+
+/* One layer of a conversion: the 8-bit cache and a 16-bit one of the same
+   block_size, kv_heads and head_dim (pitches as in kvsnap_c8_cache). */
+typedef struct kvsnap_c8_pair {
+    int64_t codes, scales, side_pitch, block_pitch, token_pitch, head_pitch;
+    int64_t wide, wide_side, wide_block, wide_token, wide_head;
+    int32_t blocks, wide_blocks;
+} kvsnap_c8_pair;
+
+/*
+ * Whole blocks between a 16-bit cache and the 8-bit one, every layer in one
+ * launch: pairs is a device array of `layers`, wide_ids and ids device int64
+ * arrays of n block ids. compress writes blocks ids[i] from wide_ids[i]; token
+ * slots from valid_tokens on (counted over the n blocks; negative: none) become
+ * zeros. expand writes blocks wide_ids[i] from ids[i], rounded once.
+ */
+int kvsnap_c8_compress(const kvsnap_c8_pair* pairs, int layers, int block_size, int kv_heads, int head_dim, int type,
+                       const int64_t* wide_ids, const int64_t* ids, int64_t n, int64_t valid_tokens,
+                       uint32_t* status, int device, uintptr_t stream);
+int kvsnap_c8_expand(const kvsnap_c8_pair* pairs, int layers, int block_size, int kv_heads, int head_dim, int type,
+                     const int64_t* ids, const int64_t* wide_ids, int64_t n, uint32_t* status, int device,
+                     uintptr_t stream);
 
 #ifdef __cplusplus
 }

@@ -3,6 +3,8 @@
 Modules:
   dataplane   TorchBlockDataPlane, CudaPool, PinnedAllocation (drop-in for kvsnap.connector.dataplane),
               PendingDigests, DigestCache, CorruptBlockError
+  cache8      PagedCache8, PagedBatch, CacheConverter, rotary_table: an 8-bit paged KV cache, its append,
+              attention and conversion to and from 16-bit caches
   blobs       write_blobs, read_and_restore: KVSBLOB1 files between pinned memory and disk
   native_io   NativeIO, get_io_backend (drop-in for kvsnap.store.native_io's native backend)
   crc32c      crc32c (drop-in for kvsnap.store.crc32c)

@@ -59,6 +59,35 @@ class Span(C.Structure):
 
 assert C.sizeof(Span) == 64
 
+# The 8-bit paged cache (kvsnap_c8_*).
+C8_BAD_LENGTH, C8_BAD_POSITION = 16, 32
+C8_BF16, C8_FP16 = 0, 1
+
+
+class C8Cache(C.Structure):
+    """``kvsnap_c8_cache``: one layer of an 8-bit paged cache."""
+    _fields_ = [("codes", C.c_int64), ("scales", C.c_int64), ("side_pitch", C.c_int64), ("block_pitch", C.c_int64),
+                ("token_pitch", C.c_int64), ("head_pitch", C.c_int64), ("blocks", C.c_int32),
+                ("block_size", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("device", C.c_int32),
+                ("reserved", C.c_int32)]
+
+
+class C8Batch(C.Structure):
+    """``kvsnap_c8_batch``: the sequences of one call."""
+    _fields_ = [("table", C.c_int64), ("start", C.c_int64), ("lengths", C.c_int64), ("table_pitch", C.c_int64),
+                ("width", C.c_int32), ("seqs", C.c_int32), ("rows", C.c_int32), ("max_query", C.c_int32)]
+
+
+class C8Pair(C.Structure):
+    """``kvsnap_c8_pair``: one layer of a conversion."""
+    _fields_ = [("codes", C.c_int64), ("scales", C.c_int64), ("side_pitch", C.c_int64), ("block_pitch", C.c_int64),
+                ("token_pitch", C.c_int64), ("head_pitch", C.c_int64), ("wide", C.c_int64), ("wide_side", C.c_int64),
+                ("wide_block", C.c_int64), ("wide_token", C.c_int64), ("wide_head", C.c_int64), ("blocks", C.c_int32),
+                ("wide_blocks", C.c_int32)]
+
+
+assert (C.sizeof(C8Cache), C.sizeof(C8Batch), C.sizeof(C8Pair)) == (72, 48, 96)
+
 _P = C.c_void_p
 _I64 = C.c_int64
 _U64 = C.c_uint64
@@ -111,6 +140,16 @@ DP_API = {
     "kvsnap_dp_ipc_open": ([_P, C.c_int, C.POINTER(C.c_void_p)], C.c_int),
     "kvsnap_dp_ipc_close": ([_P], C.c_int),
     "kvsnap_dp_scatter_verify_static": ([_P, C.c_int, _U64, _P, _P, _I64, _P, _P, C.c_int, C.c_int, _SZ], C.c_int),
+}
+
+_CACHE, _BATCH = C.POINTER(C8Cache), C.POINTER(C8Batch)
+C8_API = {
+    "kvsnap_c8_append": ([_CACHE, _BATCH, C.c_int, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, C.c_int, _P, _P,
+                          _I64, C.c_int, C.c_int, _P, _SZ], C.c_int),
+    "kvsnap_c8_attend": ([_CACHE, _BATCH, C.c_int, _P, _I64, _I64, C.c_int, C.c_float, _P, _P, _SZ], C.c_int),
+    "kvsnap_c8_compress": ([_P, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _P, _P, _I64, _I64, _P, C.c_int, _SZ],
+                           C.c_int),
+    "kvsnap_c8_expand": ([_P, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _P, _P, _I64, _P, C.c_int, _SZ], C.c_int),
 }
 
 # Blocks the no-allocation verified scatter handles in one call (include/kvsnap_cuda.h).

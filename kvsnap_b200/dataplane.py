@@ -59,6 +59,7 @@ def _load(library=None):
     lib = _abi.load(path, _abi.POOL_API)
     _abi.declare(lib, _abi.POOL_EXTRA, required=False)
     _abi.declare(lib, _abi.DP_API, required=False)
+    _abi.declare(lib, _abi.C8_API, required=False)
     return lib
 
 
