@@ -408,11 +408,16 @@ int kvsnap_c8_append(const kvsnap_c8_cache* cache, const kvsnap_c8_batch* batch,
  * cached tokens: out[i][h] = sum_j softmax_j(scale * q.k_j) v_j over positions j
  * up to the row's own. Query heads g * q_heads / kv_heads .. share KV head g.
  * A row that sees no token is zeros; rows that belong to nobody are not
- * written. out is dense and of the query's type.
+ * written. out is dense and of the query's type. The workspace is device memory,
+ * 16-byte aligned, of at least kvsnap_c8_attend_workspace's bytes for the same
+ * cache, batch and heads; calls that may overlap need one each. What it holds
+ * before does not matter.
  */
 int kvsnap_c8_attend(const kvsnap_c8_cache* cache, const kvsnap_c8_batch* batch, int type, const void* query,
-                     int64_t query_token, int64_t query_head, int q_heads, float scale, void* out, uint32_t* status,
-                     uintptr_t stream);
+                     int64_t query_token, int64_t query_head, int q_heads, float scale, void* out, void* workspace,
+                     size_t workspace_bytes, uint32_t* status, uintptr_t stream);
+int kvsnap_c8_attend_workspace(const kvsnap_c8_cache* cache, const kvsnap_c8_batch* batch, int q_heads,
+                               size_t* bytes);
 
 /* One layer of a conversion: the 8-bit cache and a 16-bit one of the same
    block_size, kv_heads and head_dim (pitches as in kvsnap_c8_cache). */

@@ -146,7 +146,9 @@ _CACHE, _BATCH = C.POINTER(C8Cache), C.POINTER(C8Batch)
 C8_API = {
     "kvsnap_c8_append": ([_CACHE, _BATCH, C.c_int, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, C.c_int, _P, _P,
                           _I64, C.c_int, C.c_int, _P, _SZ], C.c_int),
-    "kvsnap_c8_attend": ([_CACHE, _BATCH, C.c_int, _P, _I64, _I64, C.c_int, C.c_float, _P, _P, _SZ], C.c_int),
+    "kvsnap_c8_attend": ([_CACHE, _BATCH, C.c_int, _P, _I64, _I64, C.c_int, C.c_float, _P, _P, _SZ, _P, _SZ],
+                         C.c_int),
+    "kvsnap_c8_attend_workspace": ([_CACHE, _BATCH, C.c_int, C.POINTER(C.c_size_t)], C.c_int),
     "kvsnap_c8_compress": ([_P, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _P, _P, _I64, _I64, _P, C.c_int, _SZ],
                            C.c_int),
     "kvsnap_c8_expand": ([_P, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _P, _P, _I64, _P, C.c_int, _SZ], C.c_int),

@@ -4,7 +4,7 @@
 
 * ``_cuda_native.so``: the pinned pool (csrc/pool.cpp), the sm_100a
   data-plane kernels (csrc/dataplane.cu) and the 8-bit cache's
-  (csrc/cache8.cu), one C ABI (include/kvsnap_cuda.h).
+  (csrc/cache8.cu, csrc/attend8.cu), one C ABI (include/kvsnap_cuda.h).
   nvcc ``-gencode arch=compute_100a,code=sm_100a``; the CUDA runtime is linked
   statically, so the library needs only the driver at run time.
 * ``_io_native.so``: host CRC32C and the pread/pwrite pool (csrc/io.cpp,
@@ -84,8 +84,8 @@ def _build(target: Path, sources, deps, compiler, flags, force: bool) -> Path:
 def build_cuda(force: bool = False) -> Path:
     flags = [*ARCH, "-O3", "-lineinfo", "-std=c++17", "-shared", "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall",
              "-cudart", "static", "-t", "4", f"-I{INCLUDE}", f"-I{CSRC}"]
-    return _build(CUDA_LIB, [CSRC / "pool.cpp", CSRC / "dataplane.cu", CSRC / "cache8.cu"],
-                  [CSRC / "kvsnap_internal.h", INCLUDE / "kvsnap_cuda.h"], _nvcc(), flags, force)
+    return _build(CUDA_LIB, [CSRC / "pool.cpp", CSRC / "dataplane.cu", CSRC / "cache8.cu", CSRC / "attend8.cu"],
+                  [CSRC / "kvsnap_internal.h", CSRC / "cache8.cuh", INCLUDE / "kvsnap_cuda.h"], _nvcc(), flags, force)
 
 
 def build_io(force: bool = False) -> Path:

@@ -248,8 +248,13 @@ class PagedCache8:
         elif out.data_ptr() % 16:
             raise ValueError("out must be 16-byte aligned")
         scale = self.head_dim ** -0.5 if scale is None else float(scale)
-        self._check(self._lib.kvsnap_c8_attend(cache, self._batch(batch, rows), kind, *q, q_heads, scale,
-                                               out.data_ptr(), self.status.data_ptr(), self._stream()))
+        record, size = self._batch(batch, rows), C.c_size_t()
+        self._check(self._lib.kvsnap_c8_attend_workspace(cache, record, q_heads, size))
+        # A workspace of the call's own, from the stream's (or the capture's) memory: no two calls share one.
+        workspace = torch.empty(size.value, dtype=torch.uint8, device=self.device) if size.value else None
+        self._check(self._lib.kvsnap_c8_attend(cache, record, kind, *q, q_heads, scale, out.data_ptr(),
+                                               workspace.data_ptr() if size.value else None, size.value,
+                                               self.status.data_ptr(), self._stream()))
         return out
 
     def converter(self, caches):

@@ -1,126 +1,11 @@
-// sm_100a kernels of the 8-bit paged KV cache: append with rotation, attention,
-// and conversion of blocks between 16-bit caches and this one.
-//
-// A block (page) of one side (keys or values) and KV head is block_size tokens
-// of head_dim e4m3 codes with one scale s, a power of two: the smallest with
-// amax <= 448 s. e4m3 is a floating format, so a power of two costs no
-// precision, and it buys three things: a page whose scale grows by 2^k re-rounds
-// only codes that fall among e4m3's subnormals; code * s is exact in bf16; and
-// an amax that rounds to either side of a border gives the same values.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_fp8.h>
-#include <cuda_runtime.h>
-
-#include <cstdint>
-
-#include "kvsnap_cuda.h"
-#include "kvsnap_internal.h"
+// sm_100a kernels that fill the 8-bit paged KV cache: append with rotation, and
+// conversion of blocks between 16-bit caches and this one. The format is
+// described in cache8.cuh; attention over it is attend8.cu.
+#include "cache8.cuh"
 
 namespace {
 
-using Cache = kvsnap_c8_cache;
-using Batch = kvsnap_c8_batch;
-
-// ---- elements ---------------------------------------------------------------------
-
-struct Bf16 {
-    static __device__ float2 wide(uint32_t v) {
-        return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
-    }
-    static __device__ uint32_t pack(float a, float b) {
-        const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-        return reinterpret_cast<const uint32_t&>(v);
-    }
-};
-
-struct Fp16 {
-    static __device__ float2 wide(uint32_t v) { return __half22float2(reinterpret_cast<const __half2&>(v)); }
-    static __device__ uint32_t pack(float a, float b) {
-        const __half2 v = __floats2half2_rn(a, b);
-        return reinterpret_cast<const uint32_t&>(v);
-    }
-};
-
-// 8 consecutive 16-bit elements.
-template <typename T>
-__device__ __forceinline__ void load8(const char* at, float (&v)[8]) {
-    const uint4 x = *reinterpret_cast<const uint4*>(at);
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 p = T::wide(w[i]);
-        v[2 * i] = p.x, v[2 * i + 1] = p.y;
-    }
-}
-
-template <typename T>
-__device__ __forceinline__ void store8(char* at, const float (&v)[8]) {
-    *reinterpret_cast<uint4*>(at) =
-        make_uint4(T::pack(v[0], v[1]), T::pack(v[2], v[3]), T::pack(v[4], v[5]), T::pack(v[6], v[7]));
-}
-
-__device__ __forceinline__ float2 from_e4m3x2(uint32_t v) {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(v), __NV_E4M3);
-    return __half22float2(__half2(h));
-}
-
-// 8 consecutive codes, times `by`.
-__device__ __forceinline__ void load_codes(const char* at, float by, float (&v)[8]) {
-    const uint2 x = *reinterpret_cast<const uint2*>(at);
-    const uint32_t w[4] = {x.x & 0xFFFFu, x.x >> 16, x.y & 0xFFFFu, x.y >> 16};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 p = from_e4m3x2(w[i]);
-        v[2 * i] = p.x * by, v[2 * i + 1] = p.y * by;
-    }
-}
-
-// Nearest codes of v * by (ties to even); beyond +-448, infinities included, +-448.
-__device__ __forceinline__ void store_codes(char* at, const float (&v)[8], float by) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        w[i] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * i] * by, v[2 * i + 1] * by), __NV_SATFINITE, __NV_E4M3);
-    *reinterpret_cast<uint2*>(at) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
-}
-
-// ---- scales ------------------------------------------------------------------------
-
-// The smallest 2^e >= 2^-126 with amax <= 448 * 2^e = 1.75 * 2^(e + 8), from amax's bits; 0 for 0.
-__device__ __forceinline__ float needed_scale(float amax) {
-    const uint32_t bits = __float_as_uint(amax);
-    if (!bits) return 0.0f;
-    const int e = int(bits >> 23) - 8 + ((bits & 0x7FFFFFu) > 0x600000u);     // biased
-    return __uint_as_float(uint32_t(e < 1 ? 1 : e) << 23);
-}
-
-// 1 / s of a scale. A block of zeros (s = 0) takes any factor: its codes stand for 0 whatever they are.
-__device__ __forceinline__ float inverse(float s) { return s > 0.0f ? 1.0f / s : 1.0f; }
-
-__device__ __forceinline__ float finite_size(float x) {
-    const float a = fabsf(x);
-    return a <= 3.402823466e38f ? a : 0.0f;      // neither infinities nor NaN set a scale
-}
-
-__device__ __forceinline__ float max8(const float (&v)[8], float m) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_size(v[i]));
-    return m;
-}
-
-__device__ __forceinline__ float warp_max(float m) {
-#pragma unroll
-    for (int k = 16; k; k >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, k));
-    return m;
-}
-
 // ---- append ------------------------------------------------------------------------
-
-struct Rows {                 // 16-bit rows [token][head][dim]
-    const char* at;
-    int64_t token, head;
-};
 
 struct AppendArgs {
     Cache c;
@@ -139,8 +24,6 @@ struct PageRun {
     int first, count;         // slots [first, first + count) are new
     int row;                  // token row of slot `first`
 };
-
-__device__ __forceinline__ const int32_t* ints(int64_t p) { return reinterpret_cast<const int32_t*>(p); }
 
 // Unit u's page. Sequence s's units start at start[s] / N + 2 s, which leaves each
 // sequence room for the pages that its rows can touch ((rows - 2) / N + 2), whatever
@@ -390,142 +273,6 @@ __global__ void __launch_bounds__(256) expand_kernel(const __grid_constant__ Con
     }
 }
 
-// ---- attention -------------------------------------------------------------------------
-
-struct AttendArgs {
-    Cache c;
-    Batch b;
-    Rows query;
-    char* out;
-    int q_heads;
-    float scale;
-    uint32_t* status;
-};
-
-// One warp: one row and query head, a token at a time with the running maximum and sum.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) attend_rows_kernel(const __grid_constant__ AttendArgs a) {
-    constexpr int kEach = D / 32;
-    const int lane = threadIdx.x % 32;
-    const int64_t u = int64_t(blockIdx.x) * 8 + threadIdx.x / 32;
-    const int64_t row = u / a.q_heads;
-    const int head = int(u % a.q_heads), kv = head / (a.q_heads / a.c.kv_heads), n = a.c.block_size;
-    if (row >= a.b.rows) return;
-    const int32_t* start = ints(a.b.start);
-    int lo = 0, hi = a.b.seqs;                       // the first sequence that ends behind the row
-    while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (start[mid + 1] > row) hi = mid; else lo = mid + 1;
-    }
-    if (lo >= a.b.seqs || row < start[lo]) return;
-    const int to = start[lo + 1], length = ints(a.b.lengths)[lo];
-    int64_t seen = length - (to - row) + 1;
-    if (to > a.b.rows || to - start[lo] > a.b.max_query || length > int64_t(a.b.width) * n) {
-        atomicOr(a.status, KVSNAP_C8_BAD_LENGTH);
-        return;
-    }
-    const uint16_t* q16 = reinterpret_cast<const uint16_t*>(a.query.at + row * a.query.token + head * a.query.head);
-    float q[kEach], o[kEach], top = -INFINITY, sum = 0.0f;
-    for (int i = 0; i < kEach; ++i) {
-        q[i] = T::wide(q16[lane * kEach + i]).x * a.scale;
-        o[i] = 0.0f;
-    }
-    const char* codes = reinterpret_cast<const char*>(a.c.codes);
-    const float* scales = reinterpret_cast<const float*>(a.c.scales);
-    for (int64_t j = 0; j < seen; ++j) {
-        const int64_t block = ints(a.b.table)[lo * a.b.table_pitch + j / n];
-        if (block < 0 || block >= a.c.blocks) {
-            atomicOr(a.status, KVSNAP_DP_BAD_BLOCK);
-            continue;
-        }
-        const char* k = codes + block * a.c.block_pitch + (j % n) * a.c.token_pitch + kv * a.c.head_pitch + lane * kEach;
-        const char* v = k + a.c.side_pitch;
-        const float ks = scales[(block * 2) * a.c.kv_heads + kv], vs = scales[(block * 2 + 1) * a.c.kv_heads + kv];
-        float s = 0.0f;
-        for (int i = 0; i < kEach; ++i) s += q[i] * from_e4m3x2(uint8_t(k[i])).x;
-        for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
-        s *= ks;
-        const float now = fmaxf(top, s), keep = __expf(top - now), p = __expf(s - now);
-        sum = sum * keep + p;
-        for (int i = 0; i < kEach; ++i) o[i] = o[i] * keep + p * vs * from_e4m3x2(uint8_t(v[i])).x;
-        top = now;
-    }
-    uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + (row * a.q_heads + head) * D + lane * kEach;
-    for (int i = 0; i < kEach; ++i) out[i] = uint16_t(T::pack(sum > 0.0f ? o[i] / sum : 0.0f, 0.0f));
-}
-
-// ---- host side --------------------------------------------------------------------------
-
-struct Fail {
-    const char* what;
-};
-
-void check(cudaError_t rc) {
-    if (rc != cudaSuccess) throw Fail{cudaGetErrorString(rc)};
-}
-
-void require(bool ok, const char* what) {
-    if (!ok) throw Fail{what};
-}
-
-// Checks the arguments, then runs `body` with `device` current if `checks` says that there is
-// something to do, and puts the caller's device back.
-template <typename C, typename F>
-int on_device(int device, C&& checks, F&& body) {
-    int before = -1;
-    int rc = -1;
-    try {
-        if (!checks()) return 0;
-        check(cudaGetDevice(&before));
-        if (device != before) check(cudaSetDevice(device));
-        body();
-        rc = 0;
-    } catch (const Fail& f) {
-        kvsnap_internal_set_error(f.what);
-    } catch (...) {
-        kvsnap_internal_set_error("the 8-bit cache's host side failed");
-    }
-    if (before >= 0 && device != before) cudaSetDevice(before);
-    return rc;
-}
-
-bool aligned(int64_t v) { return v % 16 == 0; }
-
-void check_cache(const Cache* c) {
-    require(c && c->codes && c->scales, "the 8-bit cache has no storage");
-    require(c->head_dim == 64 || c->head_dim == 128, "head_dim must be 64 or 128");
-    require(c->block_size > 0 && c->block_size % 16 == 0, "block_size must be a multiple of 16");
-    require(c->kv_heads > 0 && c->blocks > 0, "the 8-bit cache is empty");
-    require(aligned(c->codes) && aligned(c->side_pitch) && aligned(c->block_pitch) && aligned(c->token_pitch) &&
-                aligned(c->head_pitch),
-            "the 8-bit cache's codes must be 16-byte aligned");
-}
-
-void check_batch(const Batch* b) {
-    require(b && (!b->seqs || (b->start && b->lengths && (b->table || !b->width))), "the batch has no tables");
-    require(b->seqs >= 0 && b->rows >= 0 && b->width >= 0 && b->max_query >= 0, "invalid batch");
-}
-
-void check_rows(const void* at, int64_t token, int64_t head) {
-    require(at && aligned(reinterpret_cast<intptr_t>(at)) && aligned(token) && aligned(head),
-            "rows must be 16-byte aligned");
-}
-
-void check_type(int type) {
-    require(type == KVSNAP_C8_BF16 || type == KVSNAP_C8_FP16, "the element type must be bf16 or fp16");
-}
-
-template <typename F>
-void by_type(int type, int head_dim, F&& launch) {
-    if (type == KVSNAP_C8_BF16) {
-        if (head_dim == 64) launch(Bf16{}, std::integral_constant<int, 64>{});
-        else launch(Bf16{}, std::integral_constant<int, 128>{});
-    } else {
-        if (head_dim == 64) launch(Fp16{}, std::integral_constant<int, 64>{});
-        else launch(Fp16{}, std::integral_constant<int, 128>{});
-    }
-}
-
 }  // namespace
 
 extern "C" int kvsnap_c8_append(const kvsnap_c8_cache* cache, const kvsnap_c8_batch* batch, int type, const void* key,
@@ -567,31 +314,6 @@ extern "C" int kvsnap_c8_append(const kvsnap_c8_cache* cache, const kvsnap_c8_ba
                 if (interleaved) append_kernel<T, D, false, true><<<grid, 256, 0, s>>>(a);
                 else append_kernel<T, D, false, false><<<grid, 256, 0, s>>>(a);
             }
-        });
-        check(cudaGetLastError());
-    });
-}
-
-extern "C" int kvsnap_c8_attend(const kvsnap_c8_cache* cache, const kvsnap_c8_batch* batch, int type,
-                                const void* query, int64_t query_token, int64_t query_head, int q_heads, float scale,
-                                void* out, uint32_t* status, uintptr_t stream) {
-    return on_device(cache ? cache->device : 0, [&] {
-        check_cache(cache);
-        check_batch(batch);
-        require(status, "the attention needs a status word");
-        if (!batch->rows || !batch->seqs) return false;
-        check_rows(query, query_token, query_head);
-        require(out, "the attention needs an output");
-        require(aligned(reinterpret_cast<intptr_t>(out)), "the output must be 16-byte aligned");
-        check_type(type);
-        require(q_heads > 0 && q_heads % cache->kv_heads == 0, "query heads must be a multiple of the KV heads");
-        return true;
-    }, [&] {
-        const AttendArgs a{*cache, *batch, {static_cast<const char*>(query), query_token, query_head},
-                           static_cast<char*>(out), q_heads, scale, status};
-        by_type(type, cache->head_dim, [&](auto t, auto d) {
-            attend_rows_kernel<decltype(t), decltype(d)::value>
-                <<<unsigned((int64_t(batch->rows) * q_heads + 7) / 8), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a);
         });
         check(cudaGetLastError());
     });

@@ -231,14 +231,14 @@ def test_the_library_refuses_before_it_touches_a_device(cache, batch, more, mess
     assert append(lib, cache, batch, **more) == -1
     assert message in lib.kvsnap_cuda_error().decode()
     if not more and "rows" not in message:
-        assert lib.kvsnap_c8_attend(cache, batch, 0, 4096, 512, 128, 4, 1.0, 4096, 4096, 0) == -1
+        assert lib.kvsnap_c8_attend(cache, batch, 0, 4096, 512, 128, 4, 1.0, 4096, None, 0, 4096, 0) == -1
         assert message in lib.kvsnap_cuda_error().decode()
 
 
 def test_the_library_refuses_attentions_and_conversions():
     lib = library()
     for heads, out, message in ((3, 4096, "multiple"), (0, 4096, "multiple"), (4, None, "output"), (4, 4104, "aligned")):
-        assert lib.kvsnap_c8_attend(c_cache(), c_batch(), 0, 4096, 512, 128, heads, 1.0, out, 4096, 0) == -1
+        assert lib.kvsnap_c8_attend(c_cache(), c_batch(), 0, 4096, 512, 128, heads, 1.0, out, None, 0, 4096, 0) == -1
         assert message in lib.kvsnap_cuda_error().decode()
     for size, heads, dim, n, type, message in ((16, 2, 96, 1, 0, "head_dim"), (8, 2, 64, 1, 0, "block_size"),
                                                (16, 2, 64, -1, 0, "invalid"), (16, 2, 64, 1 << 33, 0, "too many"),
@@ -252,7 +252,7 @@ def test_the_library_refuses_attentions_and_conversions():
 def test_calls_of_nothing_need_no_device():
     lib = library()
     assert append(lib, c_cache(), c_batch(rows=0)) == 0 and append(lib, c_cache(), c_batch(seqs=0)) == 0
-    assert lib.kvsnap_c8_attend(c_cache(), c_batch(rows=0), 0, None, 0, 0, 4, 1.0, None, 4096, 0) == 0
+    assert lib.kvsnap_c8_attend(c_cache(), c_batch(rows=0), 0, None, 0, 0, 4, 1.0, None, None, 0, 4096, 0) == 0
     assert lib.kvsnap_c8_compress(None, 0, 16, 2, 64, 0, None, None, 0, -1, 4096, 0, 0) == 0
 
 
