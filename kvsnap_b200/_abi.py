@@ -60,7 +60,7 @@ class Span(C.Structure):
 assert C.sizeof(Span) == 64
 
 # The 8-bit paged cache (kvsnap_c8_*).
-C8_BAD_LENGTH, C8_BAD_POSITION = 16, 32
+C8_BAD_LENGTH, C8_BAD_POSITION, C8_STALLED = 16, 32, 64
 C8_BF16, C8_FP16 = 0, 1
 
 

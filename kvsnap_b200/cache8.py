@@ -29,6 +29,7 @@ _PROBLEMS = {
     _abi.BAD_BLOCK: "a block id outside the cache",
     _abi.C8_BAD_LENGTH: "a sequence's length or query rows that do not fit the block table, the rows or max_query",
     _abi.C8_BAD_POSITION: "a position behind the rotary table's end",
+    _abi.C8_STALLED: "a wait inside a kernel ran out: its results are not valid",
 }
 
 
@@ -230,7 +231,7 @@ class PagedCache8:
         """Causal attention of ``query`` ``[rows, q_heads, head_dim]`` over the sequences' cached tokens of ``layer``.
 
         Row i of a sequence sees its positions up to its own, the new tokens' own keys (already appended)
-        included. ``scale`` multiplies the scores, 1 / sqrt(head_dim) by default. Query heads g * group to
+        included. ``scale`` (not negative) multiplies the scores, 1 / sqrt(head_dim) by default. Query heads g * group to
         (g + 1) * group - 1 share KV head g. ``out``: a contiguous tensor like ``query`` to write to. A row
         that sees no token is zeros; rows that are no sequence's are left as they are in ``out`` (unspecified
         without it). Sums and the softmax's statistics are 32-bit; weights and cached values meet in 16 bits.
@@ -248,6 +249,8 @@ class PagedCache8:
         elif out.data_ptr() % 16:
             raise ValueError("out must be 16-byte aligned")
         scale = self.head_dim ** -0.5 if scale is None else float(scale)
+        if not 0.0 <= scale < 3.4e38:
+            raise ValueError("scale must be finite and not negative")
         record, size = self._batch(batch, rows), C.c_size_t()
         self._check(self._lib.kvsnap_c8_attend_workspace(cache, record, q_heads, size))
         # A workspace of the call's own, from the stream's (or the capture's) memory: no two calls share one.

@@ -20,6 +20,7 @@ struct AttendArgs {
     Rows query;
     char* out;
     int q_heads, group;       // query heads; query heads a KV head
+    int step_rows;            // sequences of up to so many rows a KV head are the step kernel's
     float scale;              // of the scores, times log2(e)
     uint32_t* status;
 };
@@ -60,6 +61,23 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
     return d;
 }
 
+// A kernel's work is cut evenly over its CTAs, so neighbours share units (a sequence's head, or group of
+// heads, and a tile of its rows). A CTA that holds a part of one leaves the part's sums here: in its
+// second slot where the part begins the unit, in its first where it goes on with one.
+struct SharedUnit {
+    int row;                  // the sequence's first token row
+    int head;                 // first KV head
+    int first, rows;          // rows [first, first + rows) of each head (row r: token r / group, head r % group)
+    int parts;                // CTAs that share it, from this one on; 0: none
+};
+
+struct Parts {
+    float* sums;              // [2 * CTAs][slot rows][D]
+    float2* ml;               // their maxima and weights' sums
+    SharedUnit* units;        // a CTA's unit that it begins and others go on with
+    int heads, head_rows;     // slot rows: heads x rows a head
+};
+
 // ---- few rows: decode -------------------------------------------------------------------
 //
 // Sequences with at most kStepRows rows a KV head (query heads of the group times
@@ -82,9 +100,7 @@ constexpr float kSlack = 8.0f;             // log2 by which a weight may exceed 
 struct StepArgs {
     AttendArgs a;
     int hc, ts, hg;           // heads a CTA, slices of a chunk, groups of heads
-    float* part;              // [2 * CTAs][hc][rows][D] unfinished sums of units that CTAs share
-    float2* part_ml;          // their maxima and weights' sums
-    int4* shared_units;       // a CTA: the unit whose first part it holds: first row, head group, rows, parts
+    Parts parts;
 };
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -115,7 +131,7 @@ __device__ __forceinline__ uint2 load8bytes(const char* at) {
 
 // Chunks of a sequence: TS granules each; a sequence without tokens has one, whose rows become zeros.
 __device__ __forceinline__ int chunks_of(const StepArgs& p, int s, Sequence& q) {
-    if (!read_sequence(p.a.b, p.a.c.block_size, s, q, p.a.status) || q.rows * p.a.group > kStepRows) return 0;
+    if (!read_sequence(p.a.b, p.a.c.block_size, s, q, p.a.status) || q.rows * p.a.group > p.a.step_rows) return 0;
     return max(1, (q.length + p.ts * kGranule - 1) / (p.ts * kGranule));
 }
 
@@ -410,7 +426,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1) step_kernel(const __grid_const
     int s = 0, hg = 0, c0 = 0;
     Sequence q;
     if (SPLIT) {
-        if (threadIdx.x == 0) p.shared_units[blockIdx.x] = make_int4(0, 0, 0, 0);
+        if (threadIdx.x == 0) p.parts.units[blockIdx.x].parts = 0;
         int64_t mine = 0;
         for (int i = threadIdx.x; i < seqs; i += blockDim.x) mine += int64_t(chunks_of(p, i, q)) * p.hg;
         total = block_sum(mine, sh.scratch);
@@ -502,15 +518,15 @@ __global__ void __launch_bounds__(32 * kWarps, 1) step_kernel(const __grid_const
                 store4<T>(p.a.out + (to * D + at) * 2, make_float4(o.x * by, o.y * by, o.z * by, o.w * by));
             } else {
                 const int64_t to = (int64_t(slot) * p.hc + h) * kStepRows + row;
-                *reinterpret_cast<float4*>(p.part + to * D + at) = o;
-                if (at == 0) p.part_ml[to] = make_float2(top, sum);
+                *reinterpret_cast<float4*>(p.parts.sums + to * D + at) = o;
+                if (at == 0) p.parts.ml[to] = make_float2(top, sum);
             }
         }
         if (SPLIT) {
             if (!whole && c0 == 0 && threadIdx.x == 0) {
                 const int64_t past = pos + chunks;                             // the unit's end
                 const int last = int((past * ctas - 1) / total);
-                p.shared_units[blockIdx.x] = make_int4(q.row, hg, rows, last - int(blockIdx.x) + 1);
+                p.parts.units[blockIdx.x] = SharedUnit{q.row, hg * p.hc, 0, rows, last - int(blockIdx.x) + 1};
             }
             __syncthreads();
         }
@@ -520,31 +536,32 @@ __global__ void __launch_bounds__(32 * kWarps, 1) step_kernel(const __grid_const
     }
 }
 
-// Joins the parts of shared units. A unit's parts lie in consecutive CTAs' slots: its first CTA's
-// second slot, then first slots. A warp a row where there are few parts, else a CTA a row.
+// Joins the parts of shared units, which lie in consecutive CTAs' slots. A warp a row where there are
+// few parts, else a CTA a row.
 constexpr int kJoinWarps = 8;
+constexpr int kMostCtas = 512;
 
 template <typename T, int D>
-__global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_constant__ StepArgs p, int ctas) {
+__global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_constant__ AttendArgs a,
+                                                               const __grid_constant__ Parts p, int ctas) {
     constexpr int kEach = D / 32;
-    __shared__ int4 units[512];
-    __shared__ int owner[512];
+    __shared__ SharedUnit units[kMostCtas];
+    __shared__ int owner[kMostCtas];
     __shared__ int count, most;
     __shared__ float sums[kJoinWarps][D];
-    __shared__ float weight[512], stat[kJoinWarps];
+    __shared__ float weight[kMostCtas], stat[kJoinWarps];
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (threadIdx.x == 0) count = most = 0;
-    __syncthreads();
     if (warp == 0) {
         int n = 0, parts = 0;
         for (int i = lane; i < (ctas + 31) / 32 * 32; i += 32) {
-            const int4 u = i < ctas ? p.shared_units[i] : make_int4(0, 0, 0, 0);
-            const uint32_t hit = __ballot_sync(~0u, u.w > 0);
-            if (u.w > 0) {
+            SharedUnit u{};
+            if (i < ctas) u = p.units[i];
+            const uint32_t hit = __ballot_sync(~0u, u.parts > 0);
+            if (u.parts > 0) {
                 const int at = n + __popc(hit & ((1u << lane) - 1));
                 units[at] = u, owner[at] = i;
-                parts = max(parts, u.w);
+                parts = max(parts, u.parts);
             }
             n += __popc(hit);
         }
@@ -555,42 +572,41 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
     const bool alone = most <= 8;                                  // a warp a row
     const int first = alone ? blockIdx.x * kJoinWarps + warp : blockIdx.x;
     const int step = alone ? gridDim.x * kJoinWarps : gridDim.x;
-    for (int task = first; task < count * p.hc * kStepRows; task += step) {
-        const int k = task / (p.hc * kStepRows), h = task / kStepRows % p.hc, row = task % kStepRows;
-        const int4 u = units[k];
-        if (row >= u.z) continue;
-        const auto at = [&](int f) -> int64_t {
-            return (int64_t(2 * (owner[k] + f) + (f == 0)) * p.hc + h) * kStepRows + row;
-        };
+    const int slot_rows = p.heads * p.head_rows;
+    for (int task = first; task < count * slot_rows; task += step) {
+        const int k = task / slot_rows, in = task % slot_rows, h = in / p.head_rows, row = in % p.head_rows;
+        const SharedUnit u = units[k];
+        if (row >= u.rows) continue;
+        const auto at = [&](int f) { return int64_t(2 * (owner[k] + f) + (f == 0)) * slot_rows + in; };
         float o[kEach] = {}, sum = 0.0f;
         const auto add = [&](int f, float by) {
-            const float* from = p.part + at(f) * D + lane * kEach;
+            const float* from = p.sums + at(f) * D + lane * kEach;
 #pragma unroll
             for (int i = 0; i < kEach; ++i) o[i] += by * from[i];
         };
         if (alone) {
-            const float2 ml = lane < u.w ? p.part_ml[at(lane)] : make_float2(kLowest, 0.0f);
+            const float2 ml = lane < u.parts ? p.ml[at(lane)] : make_float2(kLowest, 0.0f);
             float top = ml.x;
 #pragma unroll
             for (int i = 4; i; i >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, i));
             top = __shfl_sync(~0u, top, 0);
             const float f = exp2_fast(ml.x - top);
-            sum = lane < u.w ? f * ml.y : 0.0f;
+            sum = lane < u.parts ? f * ml.y : 0.0f;
 #pragma unroll
             for (int i = 4; i; i >>= 1) sum += __shfl_xor_sync(~0u, sum, i);
             sum = __shfl_sync(~0u, sum, 0);
-            for (int i = 0; i < u.w; ++i) add(i, __shfl_sync(~0u, f, i));
+            for (int i = 0; i < u.parts; ++i) add(i, __shfl_sync(~0u, f, i));
         } else {
             float top = kLowest;
-            for (int i = threadIdx.x; i < u.w; i += blockDim.x) top = fmaxf(top, p.part_ml[at(i)].x);
+            for (int i = threadIdx.x; i < u.parts; i += blockDim.x) top = fmaxf(top, p.ml[at(i)].x);
             top = warp_max(top);
             if (lane == 0) stat[warp] = top;
             __syncthreads();
             top = stat[0];
             for (int w = 1; w < kJoinWarps; ++w) top = fmaxf(top, stat[w]);
             __syncthreads();
-            for (int i = threadIdx.x; i < u.w; i += blockDim.x) {
-                const float2 ml = p.part_ml[at(i)];
+            for (int i = threadIdx.x; i < u.parts; i += blockDim.x) {
+                const float2 ml = p.ml[at(i)];
                 const float f = exp2_fast(ml.x - top);
                 weight[i] = f;
                 sum += f * ml.y;
@@ -602,7 +618,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
             sum = 0.0f;
             for (int w = 0; w < kJoinWarps; ++w) sum += stat[w];
 #pragma unroll 4
-            for (int i = warp; i < u.w; i += kJoinWarps) add(i, weight[i]);
+            for (int i = warp; i < u.parts; i += kJoinWarps) add(i, weight[i]);
 #pragma unroll
             for (int i = 0; i < kEach; ++i) sums[warp][lane * kEach + i] = o[i];
             __syncthreads();
@@ -615,75 +631,759 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
             if (warp) continue;
         }
         const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
-        const int head = u.y * p.hc + h;
-        const int64_t to = int64_t(u.x + row / p.a.group) * p.a.q_heads + head * p.a.group + row % p.a.group;
-        char* out = p.a.out + (to * D + lane * kEach) * 2;
+        const int r = u.first + row;
+        const int64_t to = int64_t(u.row + r / a.group) * a.q_heads + (u.head + h) * a.group + r % a.group;
+        char* out = a.out + (to * D + lane * kEach) * 2;
         if constexpr (kEach == 4) store4<T>(out, make_float4(o[0] * by, o[1] * by, o[2] * by, o[3] * by));
         else *reinterpret_cast<uint32_t*>(out) = T::pack(o[0] * by, o[1] * by);
     }
 }
 
-// One warp: one row and query head, a token at a time with the running maximum and sum.
+// ---- many rows: chunks and prompts --------------------------------------------------------
+//
+// Sequences that the kernel above does not take. Bound by the tensor cores: 4 D operations a
+// query head and visible token, in two products of fp16 operands with 32-bit sums in tensor memory.
+// A CTA takes 256 rows (two tiles of 128) of one KV head over tiles of 128 tokens:
+//   warps 8-15  load a tile's codes, one tile ahead, turn them to fp16 and lay them out for the tensor
+//               cores; both row tiles use them, so a code is converted once per 256 rows;
+//   warp 16     issues S = Q K^T of one row tile while the other's softmax runs, and O += P V;
+//   warps 0-7   a thread a row: maximum, weights, sums; P goes back to tensor memory over S.
+// The running maximum follows a row's true maximum only when that exceeds it by 2^8 (weights stay
+// within fp16), so sums in tensor memory are rarely touched. A page's scale goes into the conversion
+// relative to the largest key scale of the tile (which multiplies S) and the largest value scale so
+// far (which divides O at the end): powers of two, exact in fp16.
+
+constexpr int kTile = 128;                 // tokens a step, rows a tile
+constexpr int kUnitRows = 2 * kTile;
+constexpr int kConvertWarps = 8, kChunkThreads = 32 * (8 + kConvertWarps + 1);
+constexpr uint32_t kSumsAt = 256;          // columns of tensor memory: S and P 0, 128; O 256, 384
+
+struct ChunkArgs {
+    AttendArgs a;
+    Parts parts;
+};
+
+// One tile of a unit: its place in the work, the same for every role of the CTA.
+struct Unit {
+    Sequence q;
+    int s, head, tile;        // sequence, KV head, tile of 256 rows
+    int first, rows;          // its rows of the head
+    int first_seen;           // tokens that its first row sees
+    int steps;                // tiles of tokens that its last row sees
+};
+
+__device__ __forceinline__ bool chunk_sequence(const AttendArgs& a, int s, Sequence& q) {
+    return read_sequence(a.b, a.c.block_size, s, q, a.status) && q.rows * a.group > a.step_rows;
+}
+
+__device__ __forceinline__ int steps_of(const AttendArgs& a, const Sequence& q, int tile) {
+    const int last = min(q.rows * a.group, (tile + 1) * kUnitRows) - 1;
+    const int seen = q.length - q.rows + last / a.group + 1;
+    return max(1, (seen + kTile - 1) / kTile);
+}
+
+__device__ __forceinline__ int row_tiles(const AttendArgs& a, const Sequence& q) {
+    return (q.rows * a.group + kUnitRows - 1) / kUnitRows;
+}
+
+// Steps of one head of sequence s, summed by a warp.
+__device__ __forceinline__ int64_t head_steps(const AttendArgs& a, int s) {
+    Sequence q;
+    if (!chunk_sequence(a, s, q)) return 0;
+    int64_t n = 0;
+    for (int i = threadIdx.x % 32; i < row_tiles(a, q); i += 32) n += steps_of(a, q, i);
+#pragma unroll
+    for (int k = 16; k; k >>= 1) n += __shfl_xor_sync(~0u, n, k);
+    return n;
+}
+
+constexpr int kScanned = 256;              // sequences scanned at a time
+constexpr int kNanUnits = 64;              // more units than the roles can be apart
+
+struct ChunkControl {
+    uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], drained;
+    float k_scale[4], v_scale[4];          // of a step's tile: largest key scale; largest value scale so far
+    uint32_t live[4];                      // of a step's tile: its 16-token granules that are there
+    int nan_unit[kNanUnits];               // a unit (counted from 1) whose last tiles hold a NaN value
+    uint32_t tensor;                       // tensor memory's address
+    volatile int stop;                     // a wait ran out
+    int64_t counts[kScanned], scratch[32];
+    int64_t total, pos;
+    int s, head, tile, step;
+};
+
+template <int D>
+struct ChunkShared {
+    char q[2][kTile * D * 2];
+    char k[2][kTile * D * 2];
+    char v[2][kTile * D * 2];
+    ChunkControl c;
+};
+
+// A role's way through the CTA's steps.
+struct Walk {
+    int64_t left;             // steps to go
+    int step, end;            // of the unit: [step, end) are this CTA's
+    int begin;                // where this CTA's part of the unit begins
+    int unit;                 // counted from 0
+    Unit u;
+
+    __device__ __forceinline__ bool load(const AttendArgs& a) {
+        if (u.s >= a.b.seqs || !chunk_sequence(a, u.s, u.q)) return false;
+        u.first = u.tile * kUnitRows;
+        u.rows = min(u.q.rows * a.group - u.first, kUnitRows);
+        u.first_seen = u.q.length - u.q.rows + u.first / a.group + 1;
+        u.steps = steps_of(a, u.q, u.tile);
+        begin = step;
+        end = int(min(int64_t(u.steps), step + left));
+        return true;
+    }
+    __device__ __forceinline__ bool start(const AttendArgs& a, const ChunkControl& c, int64_t steps) {
+        left = steps, unit = 0;
+        u.s = c.s, u.head = c.head, u.tile = c.tile, step = c.step;
+        return left > 0 && load(a);
+    }
+    // To the next unit, after the steps [begin, end) of this one.
+    __device__ __forceinline__ bool next(const AttendArgs& a) {
+        left -= end - begin;
+        if (left <= 0) return false;
+        step = 0, ++unit;
+        if (++u.tile >= row_tiles(a, u.q)) {
+            u.tile = 0;
+            if (++u.head == a.c.kv_heads) {
+                u.head = 0;
+                for (++u.s; u.s < a.b.seqs && !chunk_sequence(a, u.s, u.q); ++u.s) {}
+            }
+        }
+        return load(a);
+    }
+};
+
+__device__ __forceinline__ uint32_t shared_address(const void* p) {
+    return uint32_t(__cvta_generic_to_shared(p));
+}
+
+__device__ __forceinline__ void barrier_init(uint64_t* b, int count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(shared_address(b)), "r"(count) : "memory");
+}
+
+__device__ __forceinline__ void barrier_arrive(uint64_t* b) {
+    asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(shared_address(b)) : "memory");
+}
+
+// Waits for the barrier's phase of this parity; false after about two seconds, or (unless `last`)
+// once another wait ran out.
+__device__ __forceinline__ bool barrier_wait(uint64_t* b, uint32_t parity, ChunkControl& c, bool last = false) {
+    const uint32_t at = shared_address(b);
+    uint64_t began = 0;
+    for (int i = 0;; ++i) {
+        uint32_t done;
+        asm volatile("{\n.reg .pred p;\n"
+                     "mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n"
+                     "selp.u32 %0, 1, 0, p;\n}"
+                     : "=r"(done) : "r"(at), "r"(parity) : "memory");
+        if (done) return true;
+        if (i % 256 == 255) {
+            uint64_t now;
+            asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
+            if (!began) began = now;
+            if ((c.stop && !last) || now - began > 2000000000ull) {
+                c.stop = 1;
+                return false;
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ bool warp_wait(uint64_t* b, uint32_t parity, ChunkControl& c) {
+    return __all_sync(~0u, barrier_wait(b, parity, c));
+}
+
+__device__ __forceinline__ void commit(uint64_t* b) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
+                 ::"r"(shared_address(b)) : "memory");
+}
+
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// A matrix in shared memory in rows of 128 bytes, 128-byte swizzled in groups of 8 rows (1 KiB).
+// By rows of K (keys, queries): a row is 64 of the contracted elements, `lead` is not used.
+// By rows of N (values): a row is 64 columns of one contracted element; `lead` is the way to the next 64.
+__device__ __forceinline__ uint64_t matrix(uint32_t at, uint32_t lead) {
+    return uint64_t(at >> 4 & 0x3FFF) | uint64_t(lead >> 4) << 16 | uint64_t(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+
+// 128 x n products of fp16 with 32-bit sums; by_n: B lies by rows of N.
+__host__ __device__ constexpr uint32_t instruction(int n, bool by_n) {
+    return 1u << 4 | uint32_t(by_n) << 16 | uint32_t(n >> 3) << 17 | uint32_t(kTile >> 4) << 24;
+}
+
+__device__ __forceinline__ void mma_shared(uint32_t d, uint64_t a, uint64_t b, uint32_t what, bool add) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(what), "r"(uint32_t(add)) : "memory");
+}
+
+__device__ __forceinline__ void mma_tensor(uint32_t d, uint32_t a, uint64_t b, uint32_t what, bool add) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(what), "r"(uint32_t(add)) : "memory");
+}
+
+// 32 columns of the warp's 32 rows of tensor memory, a row a lane.
+__device__ __forceinline__ void tensor_load(uint32_t at, float (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+          "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]),
+          "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+          "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+        : "r"(at));
+}
+
+// The loads so far, and that `v` comes from them.
+__device__ __forceinline__ void tensor_loaded(float (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+        : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+          "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]),
+          "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]),
+          "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31])
+        :: "memory");
+}
+
+__device__ __forceinline__ void tensor_store(uint32_t at, const float (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+        :: "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]),
+          "f"(v[8]), "f"(v[9]), "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]),
+          "f"(v[16]), "f"(v[17]), "f"(v[18]), "f"(v[19]), "f"(v[20]), "f"(v[21]), "f"(v[22]), "f"(v[23]),
+          "f"(v[24]), "f"(v[25]), "f"(v[26]), "f"(v[27]), "f"(v[28]), "f"(v[29]), "f"(v[30]), "f"(v[31]),
+          "r"(at) : "memory");
+}
+
+__device__ __forceinline__ void tensor_store(uint32_t at, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+        :: "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+          "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
+          "r"(at) : "memory");
+}
+
+__device__ __forceinline__ void tensor_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Where 16 bytes (8 fp16) `chunk` of row r lie in a matrix of rows of D fp16.
+template <int D>
+__device__ __forceinline__ uint32_t swizzled(int r, int chunk) {
+    return uint32_t(chunk / 8) * (kTile * 128) + uint32_t(r) * 128 + uint32_t((chunk % 8) ^ (r % 8)) * 16;
+}
+
+__device__ __forceinline__ void store_shared(char* at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    *reinterpret_cast<uint4*>(at) = make_uint4(a, b, c, d);
+}
+
+__device__ __forceinline__ uint32_t times_half2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+
+// The role of warps 8-15.
+template <int D>
+__device__ void convert_role(const ChunkArgs& p, ChunkShared<D>& sh, int64_t steps) {
+    constexpr int kAcross = D / 16, kTokens = 32 * kConvertWarps / kAcross, kEach = kTile / kTokens;
+    const AttendArgs& a = p.a;
+    const Cache& c = a.c;
+    const int tid = threadIdx.x - 256, lane = threadIdx.x % 32;
+    // A thread's 16 codes: token my_token + i * kTokens, dims 16 * piece. Of 8 consecutive lanes
+    // 4 are an even and 4 an odd token, so their swizzled 16-byte stores meet all banks.
+    const int my_token = D == 128 ? tid / 16 * 2 + tid / 4 % 2 : tid / 4;
+    const int piece = D == 128 ? tid % 4 + tid / 8 % 2 * 4 : tid % 4;
+
+    Walk w;
+    if (!w.start(a, sh.c, steps)) return;
+    // Lane p % 8 looks up granule p of a tile: its place, scales.
+    int64_t off = -1;
+    float ks = 0.0f, vs = 0.0f;
+    const auto look_up = [&](int step) {
+        const int64_t token = int64_t(step) * kTile + lane % 8 * kGranule;
+        off = -1, ks = vs = 0.0f;
+        if (token < w.u.q.length) {
+            const int64_t block = ints(a.b.table)[w.u.s * a.b.table_pitch + token / c.block_size];
+            if (block < 0 || block >= c.blocks) {
+                atomicOr(a.status, KVSNAP_DP_BAD_BLOCK);
+            } else {
+                off = block * c.block_pitch + token % c.block_size * c.token_pitch;
+                const float* scales = reinterpret_cast<const float*>(c.scales) + block * 2 * c.kv_heads + w.u.head;
+                ks = scales[0], vs = scales[c.kv_heads];
+            }
+        }
+    };
+    uint4 kr[kEach], vr[kEach];
+    const auto load = [&](uint4 (&r)[kEach], int side, int step) {
+        const char* at = reinterpret_cast<const char*>(c.codes) + side * c.side_pitch + w.u.head * c.head_pitch +
+                         my_token % kGranule * c.token_pitch + 16 * piece;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int token = my_token + i * kTokens;
+            const int64_t o = __shfl_sync(~0u, off, token / kGranule);
+            // Slots behind the last token hold anything, NaN included: they count as zeros.
+            r[i] = o >= 0 && int64_t(step) * kTile + token < w.u.q.length ? load16(at + o) : make_uint4(0, 0, 0, 0);
+        }
+    };
+    const auto tile_max = [&](float x) {
+#pragma unroll
+        for (int k = 4; k; k >>= 1) x = fmaxf(x, __shfl_xor_sync(~0u, x, k));
+        return x;
+    };
+
+    look_up(w.begin);
+    load(kr, 0, w.begin);
+    load(vr, 1, w.begin);
+    float v_top = 0.0f;
+    for (uint32_t it = 0;; ++it) {
+        const int slot = it % 2;
+        const uint32_t free = (it / 2 + 1) % 2;
+        const int step = w.step;
+        // This tile's scales, then the next tile's look-up on its way during the conversion.
+        const float k_top = tile_max(ks);
+        v_top = fmaxf(v_top, tile_max(vs));
+        const __half2 k_half = __float2half2_rn(k_top > 0.0f ? ks / k_top : 0.0f);
+        const __half2 v_half = __float2half2_rn(v_top > 0.0f ? vs / v_top : 0.0f);
+        const uint32_t k_by = reinterpret_cast<const uint32_t&>(k_half);
+        const uint32_t v_by = reinterpret_cast<const uint32_t&>(v_half);
+        if (tid < 32) {
+            const uint32_t live = __ballot_sync(~0u, off >= 0) & 0xFF;
+            if (lane == 0) sh.c.k_scale[it % 4] = k_top, sh.c.v_scale[it % 4] = v_top, sh.c.live[it % 4] = live;
+        }
+        const bool edge = int64_t(step + 1) * kTile > w.u.first_seen;
+        const int unit = w.unit;
+        bool more = true;
+        float next_v_top = v_top;
+        if (++w.step == w.end) {
+            more = w.next(a);
+            next_v_top = 0.0f;
+        }
+        if (more) look_up(w.step);
+
+        const auto convert = [&](char* to, const uint4 (&r)[kEach], uint32_t by) {
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const int token = my_token + i * kTokens;
+                const uint32_t f = __shfl_sync(~0u, by, token / kGranule);
+                const uint32_t x[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+                uint32_t h[8];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    h[2 * j] = times_half2(half2_of_codes(uint16_t(x[j])), f);
+                    h[2 * j + 1] = times_half2(half2_of_codes(uint16_t(x[j] >> 16)), f);
+                }
+                store_shared(to + swizzled<D>(token, 2 * piece), h[0], h[1], h[2], h[3]);
+                store_shared(to + swizzled<D>(token, 2 * piece + 1), h[4], h[5], h[6], h[7]);
+            }
+        };
+        if (!warp_wait(&sh.c.k_empty[slot], free, sh.c)) return;
+        convert(sh.k[slot], kr, k_by);
+        fence_shared();
+        __syncwarp();
+        if (lane == 0) barrier_arrive(&sh.c.k_full[slot]);
+        if (more) load(kr, 0, w.step);
+
+        if (edge) {
+            // Some row does not see some of these tokens, and a weight of 0 times NaN is NaN: NaN
+            // values are left out here, and put back at the end into the rows that see them.
+            bool found = false;
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                uint32_t* x = reinterpret_cast<uint32_t*>(&vr[i]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t bad = ((x[j] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+                    found |= bad != 0;
+                    x[j] &= ~((bad >> 7) * 0xFFu);
+                }
+            }
+            if (found) sh.c.nan_unit[unit % kNanUnits] = unit + 1;
+        }
+        if (!warp_wait(&sh.c.v_empty[slot], free, sh.c)) return;
+        convert(sh.v[slot], vr, v_by);
+        fence_shared();
+        __syncwarp();
+        if (lane == 0) barrier_arrive(&sh.c.v_full[slot]);
+        if (!more) return;
+        load(vr, 1, w.step);
+        v_top = next_v_top;
+    }
+}
+
+// The role of warp 16's first lane.
+template <int D>
+__device__ void issue_role(const ChunkArgs& p, ChunkShared<D>& sh, int64_t steps) {
+    constexpr uint32_t kScores = instruction(kTile, false), kSums = instruction(D, true);
+    const uint32_t tensor = sh.c.tensor;
+    Walk w;
+    if (!w.start(p.a, sh.c, steps)) return;
+    const auto scores = [&](int tile, int slot) {
+        const uint64_t q = matrix(shared_address(sh.q[tile]), 16), k = matrix(shared_address(sh.k[slot]), 16);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+            const uint64_t along = uint64_t((i / 4 * kTile * 128 + i % 4 * 32) >> 4);
+            mma_shared(tensor + tile * kTile, q + along, k + along, kScores, i > 0);
+        }
+        commit(&sh.c.s_full[tile]);
+    };
+    const auto sums = [&](int tile, int slot, bool add) {
+        const uint64_t v = matrix(shared_address(sh.v[slot]), kTile * 128);
+#pragma unroll
+        for (int i = 0; i < kTile / 16; ++i)
+            mma_tensor(tensor + kSumsAt + tile * kTile, tensor + tile * kTile + 8 * i, v + uint64_t(i * 2048 >> 4), kSums,
+                       add || i > 0);
+    };
+    uint32_t it = 0;
+    uint32_t turn[2] = {0, 0}, q_turn[2] = {0, 0};   // steps and units that each row tile has had
+    do {
+        const int tiles = w.u.rows > kTile ? 2 : 1;
+        for (int t = 0; t < tiles; ++t) {
+            if (!barrier_wait(&sh.c.q_full[t], q_turn[t]++ % 2, sh.c)) return;
+        }
+        if (!barrier_wait(&sh.c.k_full[it % 2], it / 2 % 2, sh.c)) return;
+        fence_after();
+        for (int t = 0; t < tiles; ++t) scores(t, it % 2);
+        commit(&sh.c.k_empty[it % 2]);
+        for (int step = w.begin; step < w.end; ++step, ++it) {
+            const bool last = step + 1 == w.end;
+            for (int t = 0; t < tiles; ++t) {
+                if (!barrier_wait(&sh.c.p_full[t], turn[t]++ % 2, sh.c)) return;
+                if (t == 0 && !barrier_wait(&sh.c.v_full[it % 2], it / 2 % 2, sh.c)) return;
+                fence_after();
+                sums(t, it % 2, step > w.begin);
+                if (last) commit(&sh.c.o_full[t]);
+                if (t + 1 == tiles) commit(&sh.c.v_empty[it % 2]);
+                if (!last) {
+                    if (t == 0) {
+                        if (!barrier_wait(&sh.c.k_full[(it + 1) % 2], (it + 1) / 2 % 2, sh.c)) return;
+                        fence_after();
+                    }
+                    scores(t, (it + 1) % 2);
+                    if (t + 1 == tiles) commit(&sh.c.k_empty[(it + 1) % 2]);
+                }
+            }
+        }
+    } while (w.next(p.a));
+}
+
+// The role of warps 0-3 (row tile 0) and 4-7 (row tile 1).
 template <typename T, int D>
-__global__ void __launch_bounds__(256) attend_rows_kernel(const __grid_constant__ AttendArgs a) {
-    constexpr int kEach = D / 32;
-    const int lane = threadIdx.x % 32;
-    const int64_t u = int64_t(blockIdx.x) * 8 + threadIdx.x / 32;
-    const int64_t row = u / a.q_heads;
-    const int head = int(u % a.q_heads), kv = head / (a.q_heads / a.c.kv_heads), n = a.c.block_size;
-    if (row >= a.b.rows) return;
-    const int32_t* start = ints(a.b.start);
-    int lo = 0, hi = a.b.seqs;                       // the first sequence that ends behind the row
-    while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (start[mid + 1] > row) hi = mid; else lo = mid + 1;
-    }
-    if (lo >= a.b.seqs || row < start[lo]) return;
-    if ((start[lo + 1] - start[lo]) * (a.q_heads / a.c.kv_heads) <= kStepRows) return;
-    const int to = start[lo + 1], length = ints(a.b.lengths)[lo];
-    int64_t seen = length - (to - row) + 1;
-    if (to > a.b.rows || to - start[lo] > a.b.max_query || length > int64_t(a.b.width) * n) {
-        atomicOr(a.status, KVSNAP_C8_BAD_LENGTH);
-        return;
-    }
-    const uint16_t* q16 = reinterpret_cast<const uint16_t*>(a.query.at + row * a.query.token + head * a.query.head);
-    float q[kEach], o[kEach], top = -INFINITY, sum = 0.0f;
-    for (int i = 0; i < kEach; ++i) {
-        q[i] = T::wide(q16[lane * kEach + i]).x * a.scale;
-        o[i] = 0.0f;
-    }
-    const char* codes = reinterpret_cast<const char*>(a.c.codes);
-    const float* scales = reinterpret_cast<const float*>(a.c.scales);
-    for (int64_t j = 0; j < seen; ++j) {
-        const int64_t block = ints(a.b.table)[lo * a.b.table_pitch + j / n];
-        if (block < 0 || block >= a.c.blocks) {
-            atomicOr(a.status, KVSNAP_DP_BAD_BLOCK);
+__device__ void softmax_role(const ChunkArgs& p, ChunkShared<D>& sh, int64_t steps, int64_t pos, int64_t total,
+                             int64_t ctas) {
+    const AttendArgs& a = p.a;
+    const int tile = threadIdx.x / 128, r = threadIdx.x % 128, lane = threadIdx.x % 32;
+    const uint32_t lanes = uint32_t(threadIdx.x % 128 / 32 * 32) << 16;
+    const uint32_t scores = sh.c.tensor + lanes + tile * kTile, sums = scores + kSumsAt;
+    Walk w;
+    if (!w.start(a, sh.c, steps)) return;
+    uint32_t it = 0, turn = 0, units = 0;
+    do {
+        const int n_steps = w.end - w.begin;
+        if (tile * kTile >= w.u.rows) {                  // no rows for this tile: its steps pass by
+            it += n_steps, pos += n_steps;
             continue;
         }
-        const char* k = codes + block * a.c.block_pitch + (j % n) * a.c.token_pitch + kv * a.c.head_pitch + lane * kEach;
-        const char* v = k + a.c.side_pitch;
-        const float ks = scales[(block * 2) * a.c.kv_heads + kv], vs = scales[(block * 2 + 1) * a.c.kv_heads + kv];
-        float s = 0.0f;
-        for (int i = 0; i < kEach; ++i) s += q[i] * from_e4m3x2(uint8_t(k[i])).x;
-        for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
-        s *= ks;
-        const float now = fmaxf(top, s), keep = exp2_fast(top - now), p = exp2_fast(s - now);
-        sum = sum * keep + p;
-        for (int i = 0; i < kEach; ++i) o[i] = o[i] * keep + p * vs * from_e4m3x2(uint8_t(v[i])).x;
-        top = now;
+        const Sequence& q = w.u.q;
+        const int row = w.u.first + tile * kTile + r;
+        const bool valid = row < w.u.first + w.u.rows;
+        const int token = row / a.group, head = w.u.head * a.group + row % a.group;
+        const int seen = valid ? q.length - q.rows + token + 1 : 0;
+
+        // The row's query as fp16, times a power of two that brings its largest element to [2^14, 2^15).
+        float factor;
+        {
+            const char* at = a.query.at + int64_t(q.row + token) * a.query.token + int64_t(head) * a.query.head;
+            float top = 0.0f;
+            if (valid) {
+#pragma unroll 4
+                for (int i = 0; i < D / 8; ++i) {
+                    float v[8];
+                    load8<T>(at + 16 * i, v);
+                    top = max8(v, top);
+                }
+            }
+            const int e = max(int(__float_as_uint(top) >> 23), 27);
+            const float up = __uint_as_float(uint32_t(127 + 14 + 127 - e) << 23);
+            factor = __uint_as_float(uint32_t(max(e - 14, 1)) << 23) * a.scale;
+#pragma unroll 4
+            for (int i = 0; i < D / 8; ++i) {
+                float v[8] = {};
+                if (valid) load8<T>(at + 16 * i, v);
+                store_shared(sh.q[tile] + swizzled<D>(r, i), pack_half2(v[0] * up, v[1] * up),
+                             pack_half2(v[2] * up, v[3] * up), pack_half2(v[4] * up, v[5] * up),
+                             pack_half2(v[6] * up, v[7] * up));
+            }
+            fence_shared();
+            __syncwarp();
+            if (lane == 0) barrier_arrive(&sh.c.q_full[tile]);
+        }
+
+        float m = kLowest, l = 0.0f, v_scale = 0.0f;
+        for (int step = w.begin; step < w.end; ++step, ++it) {
+            if (!warp_wait(&sh.c.s_full[tile], turn % 2, sh.c)) return;
+            ++turn;
+            fence_after();
+            const float f = factor * sh.c.k_scale[it % 4], now_v = sh.c.v_scale[it % 4];
+            const uint32_t live = sh.c.live[it % 4];
+            const int see = min(seen - step * kTile, kTile);       // columns up to here are seen
+            const bool masked = __any_sync(~0u, see < kTile) || live != 0xFF;
+            const auto hide = [&](float (&x)[32], int first) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    if (first + i >= see || !(live >> ((first + i) / kGranule) & 1)) x[i] = -INFINITY;
+            };
+            float x[32], top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                tensor_load(scores + 32 * i, x);
+                tensor_loaded(x);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) x[j] *= f;
+                if (masked) hide(x, 32 * i);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) top = fmaxf(top, x[j]);
+            }
+            float keep = 1.0f;
+            if (top > m + kSlack) {
+                keep = exp2_fast(m - top);
+                m = top, l *= keep;
+            }
+            if (now_v != v_scale) {
+                keep *= v_scale / now_v;
+                v_scale = now_v;
+            }
+            // Sums in tensor memory: complete up to the step before, as these scores were issued after them.
+            if (step > w.begin && __any_sync(~0u, keep != 1.0f)) {
+#pragma unroll 1
+                for (int i = 0; i < D / 32; ++i) {
+                    tensor_load(sums + 32 * i, x);
+                    tensor_loaded(x);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) x[j] *= keep;
+                    tensor_store(sums + 32 * i, x);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                tensor_load(scores + 32 * i, x);
+                tensor_loaded(x);
+                if (masked) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) x[j] *= f;
+                    hide(x, 32 * i);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) x[j] = exp2_fast(x[j] - m);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) x[j] = exp2_fast(fmaf(x[j], f, -m));
+                }
+                uint32_t weights[16];
+                float some[4] = {};
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    some[j % 4] += x[2 * j] + x[2 * j + 1];
+                    weights[j] = pack_half2(x[2 * j], x[2 * j + 1]);
+                }
+                l += (some[0] + some[1]) + (some[2] + some[3]);
+                tensor_store(scores + 16 * i, weights);
+            }
+            tensor_stored();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) barrier_arrive(&sh.c.p_full[tile]);
+        }
+
+        if (!warp_wait(&sh.c.o_full[tile], units++ % 2, sh.c)) return;
+        fence_after();
+        const bool whole = w.begin == 0 && w.end == w.u.steps;
+        const int slot = 2 * int(blockIdx.x) + (w.begin == 0);
+        const int64_t part = int64_t(slot) * kUnitRows + tile * kTile + r;
+        const bool nans = sh.c.nan_unit[w.unit % kNanUnits] == w.unit + 1;
+        const float by = whole ? (l == 0.0f ? 0.0f : v_scale / l) : v_scale;
+#pragma unroll 1
+        for (int i = 0; i < D / 32; ++i) {
+            float x[32];
+            tensor_load(sums + 32 * i, x);
+            tensor_loaded(x);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) x[j] *= by;
+            if (!valid) continue;
+            if (l == 0.0f) {                             // no token seen here: the sums are of zero weights
+#pragma unroll
+                for (int j = 0; j < 32; ++j) x[j] = 0.0f;
+            }
+            if (nans) {
+                const int from = max(max(w.u.first_seen, 0) / kTile, w.begin) * kTile, to = min(seen, w.end * kTile);
+                for (int t = from; t < to; ++t) {
+                    const int64_t block = ints(a.b.table)[w.u.s * a.b.table_pitch + t / a.c.block_size];
+                    if (block < 0 || block >= a.c.blocks) continue;
+                    const uint8_t* code = reinterpret_cast<const uint8_t*>(a.c.codes) + a.c.side_pitch +
+                                          block * a.c.block_pitch + t % a.c.block_size * a.c.token_pitch +
+                                          w.u.head * a.c.head_pitch + 32 * i;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if ((code[j] & 0x7F) == 0x7F) x[j] = NAN;
+                }
+            }
+            if (whole) {
+                char* to = a.out + ((int64_t(q.row + token) * a.q_heads + head) * D + 32 * i) * 2;
+#pragma unroll
+                for (int j = 0; j < 32; j += 8) {
+                    const float y[8] = {x[j], x[j + 1], x[j + 2], x[j + 3], x[j + 4], x[j + 5], x[j + 6], x[j + 7]};
+                    store8<T>(to + 2 * j, y);
+                }
+            } else {
+                float* to = p.parts.sums + part * D + 32 * i;
+#pragma unroll
+                for (int j = 0; j < 32; j += 4)
+                    *reinterpret_cast<float4*>(to + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+            }
+        }
+        if (!whole) {
+            if (valid) p.parts.ml[part] = make_float2(m, l);
+            if (w.begin == 0 && threadIdx.x == 0) {
+                const int last = int(((pos + w.u.steps) * ctas - 1) / total);
+                p.parts.units[blockIdx.x] =
+                    SharedUnit{q.row, w.u.head, w.u.first, w.u.rows, last - int(blockIdx.x) + 1};
+            }
+        }
+        pos += n_steps;
+        fence_before();                                  // the sums are read before the next unit's are written
+    } while (w.next(a));
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_constant__ ChunkArgs p) {
+    extern __shared__ char raw[];
+    auto& sh = *reinterpret_cast<ChunkShared<D>*>(raw + (1024 - shared_address(raw) % 1024) % 1024);
+    const AttendArgs& a = p.a;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, seqs = a.b.seqs;
+    constexpr int kAll = kChunkThreads / 32;
+    asm volatile("griddepcontrol.launch_dependents;");
+    if (threadIdx.x == 0) p.parts.units[blockIdx.x].parts = 0;
+
+    // All steps (of every sequence, head and row tile, end to end), and where this CTA's begin.
+    int64_t mine = 0;
+    for (int s = warp; s < seqs; s += kAll) mine += head_steps(a, s);
+    if (lane == 0) sh.c.scratch[warp] = mine;
+    __syncthreads();
+    int64_t total = 0;
+    for (int w = 0; w < kAll; ++w) total += sh.c.scratch[w];
+    total *= a.c.kv_heads;
+    const int64_t ctas = min(int64_t(gridDim.x), total);
+    if (blockIdx.x >= ctas) return;
+    const int64_t pos = total * blockIdx.x / ctas, end = total * (blockIdx.x + 1) / ctas;
+    int64_t before = 0;
+    for (int base = 0; base < seqs; base += kScanned) {
+        for (int s = warp; s < kScanned; s += kAll) {
+            const int64_t n = base + s < seqs ? head_steps(a, base + s) : 0;
+            if (lane == 0) sh.c.counts[s] = n;
+        }
+        __syncthreads();
+        if (warp == 0) {
+            for (int i = 0; i < kScanned; i += 32) {
+                const int64_t n = sh.c.counts[i + lane];
+                int64_t sum = n * a.c.kv_heads;
+#pragma unroll
+                for (int k = 1; k < 32; k <<= 1) {
+                    const int64_t up = __shfl_up_sync(~0u, sum, k);
+                    if (lane >= k) sum += up;
+                }
+                const int64_t first = before + sum - n * a.c.kv_heads;
+                if (n && first <= pos && pos < before + sum) {
+                    sh.c.s = base + i + lane;
+                    sh.c.head = int((pos - first) / n);
+                    sh.c.pos = (pos - first) % n;
+                }
+                before += __shfl_sync(~0u, sum, 31);
+            }
+            if (lane == 0) sh.c.total = before;
+        }
+        __syncthreads();
+        if (sh.c.total > pos) break;
+        __syncthreads();
     }
-    uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + (row * a.q_heads + head) * D + lane * kEach;
-    for (int i = 0; i < kEach; ++i) out[i] = uint16_t(T::pack(sum == 0.0f ? 0.0f : o[i] / sum, 0.0f));
+    if (warp == 0) {
+        Sequence q;
+        chunk_sequence(a, sh.c.s, q);
+        int64_t done = 0;
+        for (int i = 0; i < row_tiles(a, q); i += 32) {
+            const int n = i + lane < row_tiles(a, q) ? steps_of(a, q, i + lane) : 0;
+            int64_t sum = n;
+#pragma unroll
+            for (int k = 1; k < 32; k <<= 1) {
+                const int64_t up = __shfl_up_sync(~0u, sum, k);
+                if (lane >= k) sum += up;
+            }
+            const int64_t first = done + sum - n;
+            if (n && first <= sh.c.pos && sh.c.pos < done + sum) sh.c.tile = i + lane, sh.c.step = int(sh.c.pos - first);
+            done += __shfl_sync(~0u, sum, 31);
+        }
+    }
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            barrier_init(&sh.c.q_full[i], 4);
+            barrier_init(&sh.c.k_full[i], kConvertWarps);
+            barrier_init(&sh.c.v_full[i], kConvertWarps);
+            barrier_init(&sh.c.k_empty[i], 1);
+            barrier_init(&sh.c.v_empty[i], 1);
+            barrier_init(&sh.c.s_full[i], 1);
+            barrier_init(&sh.c.p_full[i], 4);
+            barrier_init(&sh.c.o_full[i], 1);
+        }
+        barrier_init(&sh.c.drained, 1);
+        for (int i = 0; i < kNanUnits; ++i) sh.c.nan_unit[i] = 0;
+        sh.c.stop = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kAll - 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;"
+                     ::"r"(shared_address(&sh.c.tensor)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+
+    const int64_t steps = end - pos;
+    if (warp < 8) {
+        softmax_role<T, D>(p, sh, steps, pos, total, ctas);
+    } else if (warp < 8 + kConvertWarps) {
+        convert_role<D>(p, sh, steps);
+    } else if (lane == 0) {
+        issue_role<D>(p, sh, steps);
+        commit(&sh.c.drained);
+        barrier_wait(&sh.c.drained, 0, sh.c, true);
+    }
+    __syncwarp();
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (warp == kAll - 1)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(sh.c.tensor));
+    if (threadIdx.x == 0 && sh.c.stop) atomicOr(a.status, KVSNAP_C8_STALLED);
 }
 
 // ---- host side ----------------------------------------------------------------------------
 
 // How a call is laid out; the same for its workspace and its launches.
-struct StepPlan {
-    StepArgs args;
-    bool any, split, wide;    // any sequence can be here; units are cut; more than 8 rows a head
-    int64_t ctas;
-    int64_t part_bytes, ml_bytes, unit_bytes;
+struct Plan {
+    StepArgs step;
+    bool stepped, chunked;    // whether each kernel runs
+    bool split, wide;         // the step kernel's units are cut; more than 8 rows a head
+    int step_rows;
+    int64_t ctas, step_ctas;
+    int64_t slots, sum_bytes, bytes;
 };
 
 int sm_count() {
@@ -693,25 +1393,32 @@ int sm_count() {
     return sms;
 }
 
-StepPlan plan_step(const Cache& c, const Batch& b, int q_heads, int sms) {
-    StepPlan plan{};
-    StepArgs& p = plan.args;
+Plan plan_for(const Cache& c, const Batch& b, int q_heads, int sms) {
+    Plan plan{};
+    StepArgs& p = plan.step;
     const int group = q_heads / c.kv_heads;
-    plan.any = group <= kStepRows;
-    plan.wide = int64_t(group) * b.max_query > 8;
+    const int64_t most_rows = int64_t(group) * (b.max_query < b.rows ? b.max_query : b.rows);
+    plan.chunked = most_rows > kStepRows;
+    // With one sequence, the kernel for many rows takes it whatever it holds: one launch, not two.
+    plan.stepped = group <= kStepRows && !(plan.chunked && b.seqs == 1);
+    plan.step_rows = plan.stepped ? kStepRows : 0;
+    plan.wide = most_rows > 8;
     for (p.hc = c.kv_heads < 8 ? c.kv_heads : 8; c.kv_heads % p.hc; --p.hc) {}
     p.ts = kWarps / p.hc, p.hg = c.kv_heads / p.hc;
     const int64_t most = (int64_t(b.width) * c.block_size + p.ts * kGranule - 1) / (p.ts * kGranule);
-    const int64_t units = int64_t(b.seqs) * p.hg;
     // Up to 8 chunks a unit, a CTA each: cutting them would cost more (a scan of the lengths,
     // parts and their join) than a few granules in turn.
     plan.split = most > 8;
-    plan.ctas = plan.split ? sms : units;
-    if (plan.split) {
-        plan.part_bytes = 2 * plan.ctas * p.hc * kStepRows * c.head_dim * int64_t(sizeof(float));
-        plan.ml_bytes = 2 * plan.ctas * p.hc * kStepRows * int64_t(sizeof(float2));
-        plan.unit_bytes = plan.ctas * int64_t(sizeof(int4));
-    }
+    plan.ctas = sms < kMostCtas ? sms : kMostCtas;
+    plan.step_ctas = plan.split ? plan.ctas : int64_t(b.seqs) * p.hg;
+    const int64_t step_slot = plan.stepped && plan.split ? p.hc * kStepRows : 0;
+    const int64_t chunk_slot = plan.chunked ? kUnitRows : 0;
+    // The two kernels and their joins run one after the other: they use the same bytes.
+    plan.slots = 2 * plan.ctas * (step_slot > chunk_slot ? step_slot : chunk_slot);
+    plan.sum_bytes = plan.slots * c.head_dim * int64_t(sizeof(float));
+    plan.bytes = plan.slots ? plan.sum_bytes + plan.slots * int64_t(sizeof(float2)) +
+                                  plan.ctas * int64_t(sizeof(SharedUnit))
+                            : 0;
     return plan;
 }
 
@@ -741,17 +1448,39 @@ void launch(K kernel, int64_t ctas, int threads, size_t shared, cudaStream_t str
 }
 
 template <typename T, int D, int NT>
-void launch_step(const StepPlan& plan, cudaStream_t stream) {
+void launch_step(const Plan& plan, const StepArgs& p, cudaStream_t stream) {
     const size_t shared = sizeof(StepShared<D, NT>);
-    if (plan.split) launch(step_kernel<T, D, NT, true>, plan.ctas, 32 * kWarps, shared, stream, false, plan.args);
-    else launch(step_kernel<T, D, NT, false>, plan.ctas, 32 * kWarps, shared, stream, false, plan.args);
+    if (plan.split) launch(step_kernel<T, D, NT, true>, plan.step_ctas, 32 * kWarps, shared, stream, false, p);
+    else launch(step_kernel<T, D, NT, false>, plan.step_ctas, 32 * kWarps, shared, stream, false, p);
+}
+
+template <typename T, int D>
+void launch_attend(const Plan& plan, const AttendArgs& a, Parts parts, cudaStream_t stream) {
+    const auto join = [&] {
+        launch(join_kernel<T, D>, plan.ctas, 32 * kJoinWarps, 0, stream, true, a, parts, int(plan.ctas));
+    };
+    if (plan.stepped) {
+        StepArgs p = plan.step;
+        parts.heads = p.hc, parts.head_rows = kStepRows;
+        p.a = a, p.parts = parts;
+        if (plan.wide) launch_step<T, D, 2>(plan, p, stream);
+        else launch_step<T, D, 1>(plan, p, stream);
+        if (plan.split) join();
+    }
+    if (plan.chunked) {
+        parts.heads = 1, parts.head_rows = kUnitRows;
+        launch(chunk_kernel<T, D>, plan.ctas, kChunkThreads, sizeof(ChunkShared<D>) + 1024, stream, false,
+               ChunkArgs{a, parts});
+        join();
+    }
 }
 
 void check_attend(const Cache* cache, const Batch* batch, int q_heads) {
     check_cache(cache);
     check_batch(batch);
     require(q_heads > 0 && q_heads % cache->kv_heads == 0, "query heads must be a multiple of the KV heads");
-    require(int64_t(batch->seqs) * cache->kv_heads < (1LL << 31), "too many sequences for one attention");
+    require(int64_t(batch->seqs) * cache->kv_heads < (1LL << 30) && int64_t(batch->rows) * q_heads < (1LL << 30),
+            "too many sequences or rows for one attention");
 }
 
 }  // namespace
@@ -763,8 +1492,7 @@ extern "C" int kvsnap_c8_attend_workspace(const kvsnap_c8_cache* cache, const kv
         *bytes = 0;
         return batch->rows && batch->seqs;
     }, [&] {
-        const StepPlan plan = plan_step(*cache, *batch, q_heads, sm_count());
-        *bytes = size_t(plan.any ? plan.part_bytes + plan.ml_bytes + plan.unit_bytes : 0);
+        *bytes = size_t(plan_for(*cache, *batch, q_heads, sm_count()).bytes);
     });
 }
 
@@ -780,34 +1508,22 @@ extern "C" int kvsnap_c8_attend(const kvsnap_c8_cache* cache, const kvsnap_c8_ba
         require(out, "the attention needs an output");
         require(aligned(reinterpret_cast<intptr_t>(out)), "the output must be 16-byte aligned");
         check_type(type);
+        require(scale >= 0.0f && scale <= 3.402823466e38f, "the scores' scale must be finite and not negative");
         return true;
     }, [&] {
-        const AttendArgs a{*cache, *batch, {static_cast<const char*>(query), query_token, query_head},
-                           static_cast<char*>(out), q_heads, q_heads / cache->kv_heads, scale * 1.4426950408889634f,
-                           status};
-        const auto s = reinterpret_cast<cudaStream_t>(stream);
-        StepPlan plan = plan_step(*cache, *batch, q_heads, sm_count());
-        const int64_t needed = plan.any ? plan.part_bytes + plan.ml_bytes + plan.unit_bytes : 0;
-        require(!needed || (workspace && int64_t(workspace_bytes) >= needed &&
-                            aligned(reinterpret_cast<intptr_t>(workspace))),
+        const Plan plan = plan_for(*cache, *batch, q_heads, sm_count());
+        require(!plan.bytes || (workspace && int64_t(workspace_bytes) >= plan.bytes &&
+                                aligned(reinterpret_cast<intptr_t>(workspace))),
                 "the attention's workspace is too small or not 16-byte aligned");
-        plan.args.a = a;
-        plan.args.part = static_cast<float*>(workspace);
-        plan.args.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + plan.part_bytes);
-        plan.args.shared_units =
-            reinterpret_cast<int4*>(static_cast<char*>(workspace) + plan.part_bytes + plan.ml_bytes);
+        const AttendArgs a{*cache, *batch, {static_cast<const char*>(query), query_token, query_head},
+                           static_cast<char*>(out), q_heads, q_heads / cache->kv_heads, plan.step_rows,
+                           scale * 1.4426950408889634f, status};
+        char* at = static_cast<char*>(workspace);
+        const Parts parts{reinterpret_cast<float*>(at), reinterpret_cast<float2*>(at + plan.sum_bytes),
+                          reinterpret_cast<SharedUnit*>(at + plan.sum_bytes + plan.slots * int64_t(sizeof(float2))),
+                          0, 0};
         by_type(type, cache->head_dim, [&](auto t, auto d) {
-            using T = decltype(t);
-            constexpr int D = decltype(d)::value;
-            if (plan.any) {
-                if (plan.wide) launch_step<T, D, 2>(plan, s);
-                else launch_step<T, D, 1>(plan, s);
-                if (plan.split)
-                    launch(join_kernel<T, D>, plan.ctas, 32 * kJoinWarps, 0, s, true, plan.args, int(plan.ctas));
-            }
-            if (int64_t(a.group) * batch->max_query > kStepRows)
-                attend_rows_kernel<T, D><<<unsigned((int64_t(batch->rows) * q_heads + 7) / 8), 256, 0, s>>>(a);
+            launch_attend<decltype(t), decltype(d)::value>(plan, a, parts, reinterpret_cast<cudaStream_t>(stream));
         });
-        check(cudaGetLastError());
     });
 }
