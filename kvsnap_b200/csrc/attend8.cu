@@ -644,9 +644,10 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
 // Sequences that the kernel above does not take. Bound by the tensor cores: 4 D operations a
 // query head and visible token, in two products of fp16 operands with 32-bit sums in tensor memory.
 // A CTA takes 256 rows (two tiles of 128) of one KV head over tiles of 128 tokens:
-//   warps 8-15  load a tile's codes, one tile ahead, turn them to fp16 and lay them out for the tensor
+//   warp 13     looks up the pages of coming tiles and their scales;
+//   warps 8-11  load a tile's codes, one tile ahead, turn them to fp16 and lay them out for the tensor
 //               cores; both row tiles use them, so a code is converted once per 256 rows;
-//   warp 16     issues S = Q K^T of one row tile while the other's softmax runs, and O += P V;
+//   warp 12     issues S = Q K^T of one row tile while the other's softmax runs, and O += P V;
 //   warps 0-7   a thread a row: maximum, weights, sums; P goes back to tensor memory over S.
 // The running maximum follows a row's true maximum only when that exceeds it by 2^8 (weights stay
 // within fp16), so sums in tensor memory are rarely touched. A page's scale goes into the conversion
@@ -655,7 +656,10 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
 
 constexpr int kTile = 128;                 // tokens a step, rows a tile
 constexpr int kUnitRows = 2 * kTile;
-constexpr int kConvertWarps = 8, kChunkThreads = 32 * (8 + kConvertWarps + 1);
+constexpr int kHalf = kTile / 2;
+constexpr int kConvertWarps = 4, kIssueWarp = 12, kLookWarp = 13, kChunkThreads = 512;
+constexpr int kLooked = 8;                 // tiles looked up ahead
+constexpr int kLookedUnits = 4;            // units
 constexpr uint32_t kSumsAt = 256;          // columns of tensor memory: S and P 0, 128; O 256, 384
 
 struct ChunkArgs {
@@ -700,15 +704,38 @@ __device__ __forceinline__ int64_t head_steps(const AttendArgs& a, int s) {
 constexpr int kScanned = 256;              // sequences scanned at a time
 constexpr int kNanUnits = 64;              // more units than the roles can be apart
 
+// What a step's conversion needs to know.
+struct Looked {
+    int64_t keys[kTile / kGranule];        // addresses of the granules' key codes; 0: not there
+    uint32_t k_by[kTile / kGranule], v_by[kTile / kGranule];   // their scales relative to the two below, as fp16 pairs
+    float k_scale, v_scale;                // largest key scale of the tile; largest value scale so far
+    uint32_t live;                         // granules that are there
+    int tokens;                            // of the tile that the sequence has
+    int edge;                              // some row does not see all of them
+    int unit;
+};
+
+// What the other roles need to know of a unit, and of the steps [begin, end) of it that are this CTA's.
+struct LookedUnit {
+    Sequence q;
+    int s, head, first, rows, first_seen, steps, begin, end;
+    int last;                              // of this CTA
+    int64_t pos;                           // its first step's place in all the work
+};
+
 struct ChunkControl {
     uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], drained;
+    uint64_t looked[kLooked], look_free[kLooked];
+    Looked look[kLooked];
+    uint64_t unit_looked[kLookedUnits], unit_free[kLookedUnits];
+    LookedUnit unit[kLookedUnits];
     float k_scale[4], v_scale[4];          // of a step's tile: largest key scale; largest value scale so far
     uint32_t live[4];                      // of a step's tile: its 16-token granules that are there
     int nan_unit[kNanUnits];               // a unit (counted from 1) whose last tiles hold a NaN value
     uint32_t tensor;                       // tensor memory's address
     volatile int stop;                     // a wait ran out
     int64_t counts[kScanned], scratch[32];
-    int64_t total, pos;
+    int64_t total, ctas, pos, sought, scanned;
     int s, head, tile, step;
 };
 
@@ -720,7 +747,7 @@ struct ChunkShared {
     ChunkControl c;
 };
 
-// A role's way through the CTA's steps.
+// The look-up's way through the CTA's steps.
 struct Walk {
     int64_t left;             // steps to go
     int step, end;            // of the unit: [step, end) are this CTA's
@@ -844,6 +871,87 @@ __device__ __forceinline__ void tensor_load(uint32_t at, float (&v)[32]) {
         : "r"(at));
 }
 
+__device__ __forceinline__ void tensor_load(uint32_t at, float (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+          "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+        : "r"(at));
+}
+
+__device__ __forceinline__ void tensor_loaded(float (&v)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+        : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+          "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
+        :: "memory");
+}
+
+__device__ __forceinline__ void tensor_store(uint32_t at, const float (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+        :: "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]),
+          "f"(v[8]), "f"(v[9]), "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]),
+          "r"(at) : "memory");
+}
+
+__device__ __forceinline__ void tensor_load(uint32_t at, float (&v)[64]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+        "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,"
+        "%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,"
+        "%56,%57,%58,%59,%60,%61,%62,%63"
+        "}, [%64];"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+          "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]),
+          "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]),
+          "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]),
+          "=f"(v[29]), "=f"(v[30]), "=f"(v[31]), "=f"(v[32]), "=f"(v[33]), "=f"(v[34]), "=f"(v[35]),
+          "=f"(v[36]), "=f"(v[37]), "=f"(v[38]), "=f"(v[39]), "=f"(v[40]), "=f"(v[41]), "=f"(v[42]),
+          "=f"(v[43]), "=f"(v[44]), "=f"(v[45]), "=f"(v[46]), "=f"(v[47]), "=f"(v[48]), "=f"(v[49]),
+          "=f"(v[50]), "=f"(v[51]), "=f"(v[52]), "=f"(v[53]), "=f"(v[54]), "=f"(v[55]), "=f"(v[56]),
+          "=f"(v[57]), "=f"(v[58]), "=f"(v[59]), "=f"(v[60]), "=f"(v[61]), "=f"(v[62]), "=f"(v[63])
+        : "r"(at));
+}
+
+// The loads so far, and that `v` comes from them.
+__device__ __forceinline__ void tensor_loaded(float (&v)[64]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+        : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+          "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]),
+          "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]),
+          "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]),
+          "+f"(v[29]), "+f"(v[30]), "+f"(v[31]), "+f"(v[32]), "+f"(v[33]), "+f"(v[34]), "+f"(v[35]),
+          "+f"(v[36]), "+f"(v[37]), "+f"(v[38]), "+f"(v[39]), "+f"(v[40]), "+f"(v[41]), "+f"(v[42]),
+          "+f"(v[43]), "+f"(v[44]), "+f"(v[45]), "+f"(v[46]), "+f"(v[47]), "+f"(v[48]), "+f"(v[49]),
+          "+f"(v[50]), "+f"(v[51]), "+f"(v[52]), "+f"(v[53]), "+f"(v[54]), "+f"(v[55]), "+f"(v[56]),
+          "+f"(v[57]), "+f"(v[58]), "+f"(v[59]), "+f"(v[60]), "+f"(v[61]), "+f"(v[62]), "+f"(v[63])
+        :: "memory");
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// Two products and sums, or sums, in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n.reg .b64 a, b, c;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmov.b64 c, {%6, %7};\n"
+        "fma.rn.f32x2 a, a, b, c;\nmov.b64 {%0, %1}, a;\n}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n.reg .b64 a, b;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\n"
+        "add.rn.f32x2 a, a, b;\nmov.b64 {%0, %1}, a;\n}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
 // The loads so far, and that `v` comes from them.
 __device__ __forceinline__ void tensor_loaded(float (&v)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
@@ -852,17 +960,6 @@ __device__ __forceinline__ void tensor_loaded(float (&v)[32]) {
           "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]),
           "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31])
         :: "memory");
-}
-
-__device__ __forceinline__ void tensor_store(uint32_t at, const float (&v)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
-        :: "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]),
-          "f"(v[8]), "f"(v[9]), "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]),
-          "f"(v[16]), "f"(v[17]), "f"(v[18]), "f"(v[19]), "f"(v[20]), "f"(v[21]), "f"(v[22]), "f"(v[23]),
-          "f"(v[24]), "f"(v[25]), "f"(v[26]), "f"(v[27]), "f"(v[28]), "f"(v[29]), "f"(v[30]), "f"(v[31]),
-          "r"(at) : "memory");
 }
 
 __device__ __forceinline__ void tensor_store(uint32_t at, const uint32_t (&v)[16]) {
@@ -891,90 +988,148 @@ __device__ __forceinline__ uint32_t times_half2(uint32_t a, uint32_t b) {
     return d;
 }
 
-// The role of warps 8-15.
-template <int D>
-__device__ void convert_role(const ChunkArgs& p, ChunkShared<D>& sh, int64_t steps) {
-    constexpr int kAcross = D / 16, kTokens = 32 * kConvertWarps / kAcross, kEach = kTile / kTokens;
+// The role of warp 13: 4 tiles at a time, a lane a granule.
+__device__ __forceinline__ void look_role(const ChunkArgs& p, ChunkControl& c, int64_t steps) {
     const AttendArgs& a = p.a;
-    const Cache& c = a.c;
+    const Cache& cache = a.c;
+    const int lane = threadIdx.x % 32, part = lane / 8, granule = lane % 8;
+    Walk w;
+    if (!w.start(a, c, steps)) return;
+    float v_carry = 0.0f;
+    bool fresh = true;
+    for (int64_t it = 0;;) {
+        if (fresh) {
+            fresh = false;
+            const int k = w.unit % kLookedUnits;
+            if (!warp_wait(&c.unit_free[k], uint32_t(w.unit / kLookedUnits + 1) % 2, c)) return;
+            if (lane == 0) {
+                c.unit[k] = LookedUnit{w.u.q, w.u.s, w.u.head, w.u.first, w.u.rows, w.u.first_seen, w.u.steps, w.begin,
+                                       w.end, w.left == w.end - w.begin, c.pos + steps - w.left};
+                barrier_arrive(&c.unit_looked[k]);
+            }
+        }
+        const int n = min(4, w.end - w.step), step = w.step + part;
+        const int64_t token = int64_t(step) * kTile + granule * kGranule;
+        int64_t at = 0;
+        float ks = 0.0f, vs = 0.0f;
+        if (part < n && token < w.u.q.length) {
+            const int64_t block = ints(a.b.table)[w.u.s * a.b.table_pitch + token / cache.block_size];
+            if (block < 0 || block >= cache.blocks) {
+                atomicOr(a.status, KVSNAP_DP_BAD_BLOCK);
+            } else {
+                at = cache.codes + block * cache.block_pitch + token % cache.block_size * cache.token_pitch +
+                     w.u.head * cache.head_pitch;
+                const float* scales = reinterpret_cast<const float*>(cache.scales) + block * 2 * cache.kv_heads + w.u.head;
+                ks = scales[0], vs = scales[cache.kv_heads];
+            }
+        }
+        const uint32_t live = __ballot_sync(~0u, at != 0) >> (8 * part) & 0xFF;
+        float k_top = ks, v_top = vs;
+#pragma unroll
+        for (int k = 4; k; k >>= 1) {
+            k_top = fmaxf(k_top, __shfl_xor_sync(~0u, k_top, k));
+            v_top = fmaxf(v_top, __shfl_xor_sync(~0u, v_top, k));
+        }
+#pragma unroll
+        for (int k = 8; k < 32; k <<= 1) {
+            const float up = __shfl_up_sync(~0u, v_top, k);
+            if (lane >= k) v_top = fmaxf(v_top, up);
+        }
+        v_top = fmaxf(v_top, v_carry);
+        v_carry = __shfl_sync(~0u, v_top, 8 * (n - 1));
+        const __half2 k_by = __float2half2_rn(k_top > 0.0f ? ks / k_top : 0.0f);
+        const __half2 v_by = __float2half2_rn(v_top > 0.0f ? vs / v_top : 0.0f);
+        for (int i = 0; i < n; ++i)
+            if (!warp_wait(&c.look_free[(it + i) % kLooked], uint32_t((it + i) / kLooked + 1) % 2, c)) return;
+        if (part < n) {
+            Looked& to = c.look[(it + part) % kLooked];
+            to.keys[granule] = at;
+            to.k_by[granule] = reinterpret_cast<const uint32_t&>(k_by);
+            to.v_by[granule] = reinterpret_cast<const uint32_t&>(v_by);
+            if (granule == 0) {
+                to.k_scale = k_top, to.v_scale = v_top, to.live = live;
+                to.tokens = int(min(int64_t(kTile), max(int64_t(0), w.u.q.length - token)));
+                to.edge = int64_t(step + 1) * kTile > w.u.first_seen;
+                to.unit = w.unit;
+            }
+        }
+        __syncwarp();
+        if (lane < n) barrier_arrive(&c.looked[(it + lane) % kLooked]);
+        it += n, w.step += n;
+        if (w.step == w.end) {
+            if (!w.next(a)) return;
+            v_carry = 0.0f, fresh = true;
+        }
+    }
+}
+
+// The role of warps 8-11.
+template <int D>
+__device__ __forceinline__ void convert_role(const ChunkArgs& p, ChunkShared<D>& sh, int64_t steps) {
+    constexpr int kAcross = D / 16, kTokens = 32 * kConvertWarps / kAcross, kEach = kTile / kTokens;
+    const Cache& c = p.a.c;
     const int tid = threadIdx.x - 256, lane = threadIdx.x % 32;
     // A thread's 16 codes: token my_token + i * kTokens, dims 16 * piece. Of 8 consecutive lanes
     // 4 are an even and 4 an odd token, so their swizzled 16-byte stores meet all banks.
     const int my_token = D == 128 ? tid / 16 * 2 + tid / 4 % 2 : tid / 4;
     const int piece = D == 128 ? tid % 4 + tid / 8 % 2 * 4 : tid % 4;
+    const int64_t within = my_token % kGranule * c.token_pitch + 16 * piece;
 
-    Walk w;
-    if (!w.start(a, sh.c, steps)) return;
-    // Lane p % 8 looks up granule p of a tile: its place, scales.
-    int64_t off = -1;
-    float ks = 0.0f, vs = 0.0f;
-    const auto look_up = [&](int step) {
-        const int64_t token = int64_t(step) * kTile + lane % 8 * kGranule;
-        off = -1, ks = vs = 0.0f;
-        if (token < w.u.q.length) {
-            const int64_t block = ints(a.b.table)[w.u.s * a.b.table_pitch + token / c.block_size];
-            if (block < 0 || block >= c.blocks) {
-                atomicOr(a.status, KVSNAP_DP_BAD_BLOCK);
-            } else {
-                off = block * c.block_pitch + token % c.block_size * c.token_pitch;
-                const float* scales = reinterpret_cast<const float*>(c.scales) + block * 2 * c.kv_heads + w.u.head;
-                ks = scales[0], vs = scales[c.kv_heads];
-            }
-        }
-    };
-    uint4 kr[kEach], vr[kEach];
-    const auto load = [&](uint4 (&r)[kEach], int side, int step) {
-        const char* at = reinterpret_cast<const char*>(c.codes) + side * c.side_pitch + w.u.head * c.head_pitch +
-                         my_token % kGranule * c.token_pitch + 16 * piece;
+    // Keys and values of a tile in turn, the next load on its way while one is converted: item i is
+    // side i % 2 of step i / 2.
+    uint4 now[kEach], next[kEach];
+    const auto load = [&](uint4 (&to)[kEach], int64_t item) {
+        const Looked& look = sh.c.look[item / 2 % kLooked];
+        const int64_t side = item % 2 ? c.side_pitch : 0;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
             const int token = my_token + i * kTokens;
-            const int64_t o = __shfl_sync(~0u, off, token / kGranule);
+            const int64_t at = look.keys[token / kGranule];
             // Slots behind the last token hold anything, NaN included: they count as zeros.
-            r[i] = o >= 0 && int64_t(step) * kTile + token < w.u.q.length ? load16(at + o) : make_uint4(0, 0, 0, 0);
+            to[i] = make_uint4(0, 0, 0, 0);
+            if (at && token < look.tokens) to[i] = load16(reinterpret_cast<const char*>(at) + side + within);
         }
     };
-    const auto tile_max = [&](float x) {
+#pragma unroll 1
+    for (int64_t item = -1; item < 2 * steps; ++item) {
+        if (item + 1 < 2 * steps) {
+            const int64_t step = (item + 1) / 2;
+            if (item % 2 && !warp_wait(&sh.c.looked[step % kLooked], uint32_t(step / kLooked) % 2, sh.c)) return;
+            load(next, item + 1);
+        }
+        if (item >= 0) {
+            const int64_t step = item / 2;
+            const int slot = step % 2, side = item % 2;
+            const Looked& look = sh.c.look[step % kLooked];
+            if (side == 0 && tid == 0) {
+                sh.c.k_scale[step % 4] = look.k_scale, sh.c.v_scale[step % 4] = look.v_scale;
+                sh.c.live[step % 4] = look.live;
+            }
+            if (side && look.edge) {
+                // Some row does not see some of these tokens, and a weight of 0 times NaN is NaN: NaN
+                // values are left out here, and put back at the end into the rows that see them.
+                bool found = false;
 #pragma unroll
-        for (int k = 4; k; k >>= 1) x = fmaxf(x, __shfl_xor_sync(~0u, x, k));
-        return x;
-    };
-
-    look_up(w.begin);
-    load(kr, 0, w.begin);
-    load(vr, 1, w.begin);
-    float v_top = 0.0f;
-    for (uint32_t it = 0;; ++it) {
-        const int slot = it % 2;
-        const uint32_t free = (it / 2 + 1) % 2;
-        const int step = w.step;
-        // This tile's scales, then the next tile's look-up on its way during the conversion.
-        const float k_top = tile_max(ks);
-        v_top = fmaxf(v_top, tile_max(vs));
-        const __half2 k_half = __float2half2_rn(k_top > 0.0f ? ks / k_top : 0.0f);
-        const __half2 v_half = __float2half2_rn(v_top > 0.0f ? vs / v_top : 0.0f);
-        const uint32_t k_by = reinterpret_cast<const uint32_t&>(k_half);
-        const uint32_t v_by = reinterpret_cast<const uint32_t&>(v_half);
-        if (tid < 32) {
-            const uint32_t live = __ballot_sync(~0u, off >= 0) & 0xFF;
-            if (lane == 0) sh.c.k_scale[it % 4] = k_top, sh.c.v_scale[it % 4] = v_top, sh.c.live[it % 4] = live;
-        }
-        const bool edge = int64_t(step + 1) * kTile > w.u.first_seen;
-        const int unit = w.unit;
-        bool more = true;
-        float next_v_top = v_top;
-        if (++w.step == w.end) {
-            more = w.next(a);
-            next_v_top = 0.0f;
-        }
-        if (more) look_up(w.step);
-
-        const auto convert = [&](char* to, const uint4 (&r)[kEach], uint32_t by) {
+                for (int i = 0; i < kEach; ++i) {
+                    uint32_t x[4] = {now[i].x, now[i].y, now[i].z, now[i].w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t bad = ((x[j] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+                        found |= bad != 0;
+                        x[j] &= ~((bad >> 7) * 0xFFu);
+                    }
+                    now[i] = make_uint4(x[0], x[1], x[2], x[3]);
+                }
+                if (found) sh.c.nan_unit[look.unit % kNanUnits] = look.unit + 1;
+            }
+            if (!warp_wait(side ? &sh.c.v_empty[slot] : &sh.c.k_empty[slot], uint32_t(step / 2 + 1) % 2, sh.c)) return;
+            char* const to = side ? sh.v[slot] : sh.k[slot];
+            const uint32_t* by = side ? look.v_by : look.k_by;
 #pragma unroll
             for (int i = 0; i < kEach; ++i) {
                 const int token = my_token + i * kTokens;
-                const uint32_t f = __shfl_sync(~0u, by, token / kGranule);
-                const uint32_t x[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+                const uint32_t f = by[token / kGranule];
+                const uint32_t x[4] = {now[i].x, now[i].y, now[i].z, now[i].w};
                 uint32_t h[8];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -984,48 +1139,23 @@ __device__ void convert_role(const ChunkArgs& p, ChunkShared<D>& sh, int64_t ste
                 store_shared(to + swizzled<D>(token, 2 * piece), h[0], h[1], h[2], h[3]);
                 store_shared(to + swizzled<D>(token, 2 * piece + 1), h[4], h[5], h[6], h[7]);
             }
-        };
-        if (!warp_wait(&sh.c.k_empty[slot], free, sh.c)) return;
-        convert(sh.k[slot], kr, k_by);
-        fence_shared();
-        __syncwarp();
-        if (lane == 0) barrier_arrive(&sh.c.k_full[slot]);
-        if (more) load(kr, 0, w.step);
-
-        if (edge) {
-            // Some row does not see some of these tokens, and a weight of 0 times NaN is NaN: NaN
-            // values are left out here, and put back at the end into the rows that see them.
-            bool found = false;
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) {
-                uint32_t* x = reinterpret_cast<uint32_t*>(&vr[i]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t bad = ((x[j] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
-                    found |= bad != 0;
-                    x[j] &= ~((bad >> 7) * 0xFFu);
-                }
+            fence_shared();
+            __syncwarp();
+            if (lane == 0) {
+                barrier_arrive(side ? &sh.c.v_full[slot] : &sh.c.k_full[slot]);
+                if (side) barrier_arrive(&sh.c.look_free[step % kLooked]);
             }
-            if (found) sh.c.nan_unit[unit % kNanUnits] = unit + 1;
         }
-        if (!warp_wait(&sh.c.v_empty[slot], free, sh.c)) return;
-        convert(sh.v[slot], vr, v_by);
-        fence_shared();
-        __syncwarp();
-        if (lane == 0) barrier_arrive(&sh.c.v_full[slot]);
-        if (!more) return;
-        load(vr, 1, w.step);
-        v_top = next_v_top;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) now[i] = next[i];
     }
 }
 
-// The role of warp 16's first lane.
+// The role of warp 12's first lane.
 template <int D>
-__device__ void issue_role(const ChunkArgs& p, ChunkShared<D>& sh, int64_t steps) {
+__device__ __forceinline__ void issue_role(ChunkShared<D>& sh) {
     constexpr uint32_t kScores = instruction(kTile, false), kSums = instruction(D, true);
     const uint32_t tensor = sh.c.tensor;
-    Walk w;
-    if (!w.start(p.a, sh.c, steps)) return;
     const auto scores = [&](int tile, int slot) {
         const uint64_t q = matrix(shared_address(sh.q[tile]), 16), k = matrix(shared_address(sh.k[slot]), 16);
 #pragma unroll
@@ -1044,83 +1174,111 @@ __device__ void issue_role(const ChunkArgs& p, ChunkShared<D>& sh, int64_t steps
     };
     uint32_t it = 0;
     uint32_t turn[2] = {0, 0}, q_turn[2] = {0, 0};   // steps and units that each row tile has had
-    do {
-        const int tiles = w.u.rows > kTile ? 2 : 1;
+    for (uint32_t unit = 0;; ++unit) {
+        if (!barrier_wait(&sh.c.unit_looked[unit % kLookedUnits], unit / kLookedUnits % 2, sh.c)) return;
+        const LookedUnit& u = sh.c.unit[unit % kLookedUnits];
+        const int tiles = u.rows > kTile ? 2 : 1, n = u.end - u.begin;
+        const bool final = u.last;
+        barrier_arrive(&sh.c.unit_free[unit % kLookedUnits]);
+#pragma unroll 1
         for (int t = 0; t < tiles; ++t) {
             if (!barrier_wait(&sh.c.q_full[t], q_turn[t]++ % 2, sh.c)) return;
         }
-        if (!barrier_wait(&sh.c.k_full[it % 2], it / 2 % 2, sh.c)) return;
-        fence_after();
-        for (int t = 0; t < tiles; ++t) scores(t, it % 2);
-        commit(&sh.c.k_empty[it % 2]);
-        for (int step = w.begin; step < w.end; ++step, ++it) {
-            const bool last = step + 1 == w.end;
+        // A step's sums, then the next one's scores; step -1 has no sums, the last no scores.
+#pragma unroll 1
+        for (int step = -1; step < n; ++step) {
+#pragma unroll 1
             for (int t = 0; t < tiles; ++t) {
-                if (!barrier_wait(&sh.c.p_full[t], turn[t]++ % 2, sh.c)) return;
-                if (t == 0 && !barrier_wait(&sh.c.v_full[it % 2], it / 2 % 2, sh.c)) return;
-                fence_after();
-                sums(t, it % 2, step > w.begin);
-                if (last) commit(&sh.c.o_full[t]);
-                if (t + 1 == tiles) commit(&sh.c.v_empty[it % 2]);
-                if (!last) {
+                if (step >= 0) {
+                    if (!barrier_wait(&sh.c.p_full[t], turn[t]++ % 2, sh.c)) return;
+                    if (t == 0 && !barrier_wait(&sh.c.v_full[it % 2], it / 2 % 2, sh.c)) return;
+                    fence_after();
+                    sums(t, it % 2, step > 0);
+                    if (step + 1 == n) commit(&sh.c.o_full[t]);
+                    if (t + 1 == tiles) commit(&sh.c.v_empty[it % 2]);
+                }
+                if (step + 1 < n) {
+                    const uint32_t next = step < 0 ? it : it + 1;
                     if (t == 0) {
-                        if (!barrier_wait(&sh.c.k_full[(it + 1) % 2], (it + 1) / 2 % 2, sh.c)) return;
+                        if (!barrier_wait(&sh.c.k_full[next % 2], next / 2 % 2, sh.c)) return;
                         fence_after();
                     }
-                    scores(t, (it + 1) % 2);
-                    if (t + 1 == tiles) commit(&sh.c.k_empty[(it + 1) % 2]);
+                    scores(t, next % 2);
+                    if (t + 1 == tiles) commit(&sh.c.k_empty[next % 2]);
                 }
             }
+            if (step >= 0) ++it;
         }
-    } while (w.next(p.a));
+        if (final) return;
+    }
+}
+
+// Four lanes of 128 columns of a row to, and from, a warp's 4 KB of shared memory: 32 rows of 128 bytes,
+// in which rows go out (8 lanes a row) that came a lane a row.
+__device__ __forceinline__ char* staged(char* warp_rows, int row, int chunk) {
+    return warp_rows + row * 128 + (chunk ^ row % 8) * 16;
 }
 
 // The role of warps 0-3 (row tile 0) and 4-7 (row tile 1).
 template <typename T, int D>
-__device__ void softmax_role(const ChunkArgs& p, ChunkShared<D>& sh, int64_t steps, int64_t pos, int64_t total,
-                             int64_t ctas) {
+__device__ __forceinline__ void softmax_role(const ChunkArgs& p, ChunkShared<D>& sh) {
+    constexpr int kLanes = D / 8;                        // lanes of 8 elements that a row takes
     const AttendArgs& a = p.a;
-    const int tile = threadIdx.x / 128, r = threadIdx.x % 128, lane = threadIdx.x % 32;
-    const uint32_t lanes = uint32_t(threadIdx.x % 128 / 32 * 32) << 16;
-    const uint32_t scores = sh.c.tensor + lanes + tile * kTile, sums = scores + kSumsAt;
-    Walk w;
-    if (!w.start(a, sh.c, steps)) return;
+    const int tile = threadIdx.x / 128, r = threadIdx.x % 128, lane = threadIdx.x % 32, warp_row = r - lane;
+    const uint32_t scores = sh.c.tensor + (uint32_t(warp_row) << 16) + tile * kTile, sums = scores + kSumsAt;
     uint32_t it = 0, turn = 0, units = 0;
-    do {
-        const int n_steps = w.end - w.begin;
-        if (tile * kTile >= w.u.rows) {                  // no rows for this tile: its steps pass by
-            it += n_steps, pos += n_steps;
+    for (uint32_t unit = 0;; ++unit) {
+        const int ring = unit % kLookedUnits;
+        if (!warp_wait(&sh.c.unit_looked[ring], unit / kLookedUnits % 2, sh.c)) return;
+        const LookedUnit& u = sh.c.unit[ring];
+        const bool final = u.last;
+        const int begin = u.begin, end = u.end;
+        if (tile * kTile >= u.rows) {                    // no rows for this tile: its steps pass by
+            it += end - begin;
+            __syncwarp();
+            if (lane == 0) barrier_arrive(&sh.c.unit_free[ring]);
+            if (final) return;
             continue;
         }
-        const Sequence& q = w.u.q;
-        const int row = w.u.first + tile * kTile + r;
-        const bool valid = row < w.u.first + w.u.rows;
-        const int token = row / a.group, head = w.u.head * a.group + row % a.group;
-        const int seen = valid ? q.length - q.rows + token + 1 : 0;
+        const int rows = min(u.rows - tile * kTile - warp_row, 32);        // of this warp (may be none)
+        const int row = u.first + tile * kTile + r, token = row / a.group;
+        const int seen = lane < rows ? u.q.length - u.q.rows + token + 1 : 0;
 
-        // The row's query as fp16, times a power of two that brings its largest element to [2^14, 2^15).
+        // The queries as fp16, a row times a power of two that brings its largest element to [2^14, 2^15).
+        // They come in D / 8 lanes a row, so that whole lines are read; then a lane takes a row.
+        const int out_row = (u.q.row + token) * a.q_heads + u.head * a.group + row % a.group;
         float factor;
         {
-            const char* at = a.query.at + int64_t(q.row + token) * a.query.token + int64_t(head) * a.query.head;
-            float top = 0.0f;
-            if (valid) {
-#pragma unroll 4
-                for (int i = 0; i < D / 8; ++i) {
-                    float v[8];
-                    load8<T>(at + 16 * i, v);
-                    top = max8(v, top);
-                }
+            const int64_t mine = int64_t(u.q.row + token) * a.query.token +
+                                 int64_t(u.head * a.group + row % a.group) * a.query.head;
+            char* const to = sh.q[tile];
+            uint4 raw[kLanes];
+#pragma unroll
+            for (int i = 0; i < kLanes; ++i) {
+                const int x = i * (32 / kLanes) + lane / kLanes;
+                const int64_t at = __shfl_sync(~0u, mine, x);
+                raw[i] = make_uint4(0, 0, 0, 0);
+                if (x < rows) raw[i] = *reinterpret_cast<const uint4*>(a.query.at + at + lane % kLanes * 16);
+            }
+#pragma unroll
+            for (int i = 0; i < kLanes; ++i)
+                *reinterpret_cast<uint4*>(to + swizzled<D>(warp_row + i * (32 / kLanes) + lane / kLanes, lane % kLanes)) = raw[i];
+            __syncwarp();
+            float top = 0.0f, v[8];
+#pragma unroll 1
+            for (int i = 0; i < kLanes; ++i) {
+                load8<T>(to + swizzled<D>(r, i), v);
+                top = max8(v, top);
             }
             const int e = max(int(__float_as_uint(top) >> 23), 27);
             const float up = __uint_as_float(uint32_t(127 + 14 + 127 - e) << 23);
             factor = __uint_as_float(uint32_t(max(e - 14, 1)) << 23) * a.scale;
-#pragma unroll 4
-            for (int i = 0; i < D / 8; ++i) {
-                float v[8] = {};
-                if (valid) load8<T>(at + 16 * i, v);
-                store_shared(sh.q[tile] + swizzled<D>(r, i), pack_half2(v[0] * up, v[1] * up),
-                             pack_half2(v[2] * up, v[3] * up), pack_half2(v[4] * up, v[5] * up),
-                             pack_half2(v[6] * up, v[7] * up));
+#pragma unroll 1
+            for (int i = 0; i < kLanes; ++i) {
+                char* const at = to + swizzled<D>(r, i);
+                load8<T>(at, v);
+                store_shared(at, pack_half2(v[0] * up, v[1] * up), pack_half2(v[2] * up, v[3] * up),
+                             pack_half2(v[4] * up, v[5] * up), pack_half2(v[6] * up, v[7] * up));
             }
             fence_shared();
             __syncwarp();
@@ -1128,74 +1286,88 @@ __device__ void softmax_role(const ChunkArgs& p, ChunkShared<D>& sh, int64_t ste
         }
 
         float m = kLowest, l = 0.0f, v_scale = 0.0f;
-        for (int step = w.begin; step < w.end; ++step, ++it) {
+        for (int step = begin; step < end; ++step, ++it) {
             if (!warp_wait(&sh.c.s_full[tile], turn % 2, sh.c)) return;
             ++turn;
             fence_after();
-            const float f = factor * sh.c.k_scale[it % 4], now_v = sh.c.v_scale[it % 4];
+            // Never 0, so that a hidden score stays -infinity.
+            const float f = fmaxf(factor * sh.c.k_scale[it % 4], 1.17549435e-38f), now_v = sh.c.v_scale[it % 4];
             const uint32_t live = sh.c.live[it % 4];
             const int see = min(seen - step * kTile, kTile);       // columns up to here are seen
             const bool masked = __any_sync(~0u, see < kTile) || live != 0xFF;
-            const auto hide = [&](float (&x)[32], int first) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (first + i >= see || !(live >> ((first + i) / kGranule) & 1)) x[i] = -INFINITY;
-            };
-            float x[32], top = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                tensor_load(scores + 32 * i, x);
-                tensor_loaded(x);
-#pragma unroll
-                for (int j = 0; j < 32; ++j) x[j] *= f;
-                if (masked) hide(x, 32 * i);
-#pragma unroll
-                for (int j = 0; j < 32; ++j) top = fmaxf(top, x[j]);
-            }
-            float keep = 1.0f;
-            if (top > m + kSlack) {
-                keep = exp2_fast(m - top);
-                m = top, l *= keep;
-            }
-            if (now_v != v_scale) {
-                keep *= v_scale / now_v;
-                v_scale = now_v;
-            }
-            // Sums in tensor memory: complete up to the step before, as these scores were issued after them.
-            if (step > w.begin && __any_sync(~0u, keep != 1.0f)) {
+            // Three passes over half a row each: the second half's maximum, the first half's maximum and
+            // weights, the second half's weights. It is read twice as registers hold one half; and
+            // rolled up, as three roles' unrolled code would not stay in the instruction cache.
+            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            float2 some[2] = {};
 #pragma unroll 1
-                for (int i = 0; i < D / 32; ++i) {
-                    tensor_load(sums + 32 * i, x);
-                    tensor_loaded(x);
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) x[j] *= keep;
-                    tensor_store(sums + 32 * i, x);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                tensor_load(scores + 32 * i, x);
+            for (int pass = 0; pass < 3; ++pass) {
+                const int half = pass != 1;
+                float x[kHalf];
+                __syncwarp();                            // lanes meet before each access to tensor memory
+                tensor_load(scores + half * kHalf, x);
                 tensor_loaded(x);
                 if (masked) {
+                    const int shown = min(max(see - half * kHalf, 0), kHalf);
+                    uint64_t bits = shown == kHalf ? ~0ull : (1ull << shown) - 1;
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) x[j] *= f;
-                    hide(x, 32 * i);
+                    for (int i = 0; i < kHalf / kGranule; ++i)
+                        if (!(live >> (half * kHalf / kGranule + i) & 1)) bits &= ~(0xFFFFull << (kGranule * i));
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) x[j] = exp2_fast(x[j] - m);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) x[j] = exp2_fast(fmaf(x[j], f, -m));
+                    for (int i = 0; i < kHalf; ++i)
+                        if (!(bits >> i & 1)) x[i] = -INFINITY;
                 }
-                uint32_t weights[16];
-                float some[4] = {};
+                if (pass < 2) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    some[j % 4] += x[2 * j] + x[2 * j + 1];
-                    weights[j] = pack_half2(x[2 * j], x[2 * j + 1]);
+                    for (int j = 0; j < kHalf; j += 8)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) tops[i] = max3(tops[i], x[j + 2 * i], x[j + 2 * i + 1]);
                 }
-                l += (some[0] + some[1]) + (some[2] + some[3]);
-                tensor_store(scores + 16 * i, weights);
+                if (pass == 1) {
+                    const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * f;
+                    float keep = 1.0f;
+                    if (top > m + kSlack) {
+                        keep = exp2_fast(m - top);
+                        m = top, l *= keep;
+                    }
+                    if (now_v != v_scale) {
+                        keep *= v_scale / now_v;
+                        v_scale = now_v;
+                    }
+                    // Sums in tensor memory: complete up to the step before, as these scores were issued after them.
+                    if (step > begin && __any_sync(~0u, keep != 1.0f)) {
+#pragma unroll 1
+                        for (int i = 0; i < D / 16; ++i) {
+                            float y[16];
+                            __syncwarp();
+                            tensor_load(sums + 16 * i, y);
+                            tensor_loaded(y);
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) y[j] *= keep;
+                            tensor_store(sums + 16 * i, y);
+                        }
+                    }
+                }
+                if (pass > 0) {
+                    const float2 ff = make_float2(f, f), mm = make_float2(-m, -m);
+#pragma unroll
+                    for (int i = 0; i < kHalf; i += 32) {
+                        uint32_t weights[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            float2 y = fma2(make_float2(x[i + 2 * j], x[i + 2 * j + 1]), ff, mm);
+                            y.x = exp2_fast(y.x), y.y = exp2_fast(y.y);
+                            some[j % 2] = add2(some[j % 2], y);
+                            weights[j] = pack_half2(y.x, y.y);
+                        }
+                        __syncwarp();
+                        tensor_store(scores + (half * kHalf + i) / 2, weights);
+                    }
+                }
             }
+            some[0] = add2(some[0], some[1]);
+            l += some[0].x + some[0].y;
+            __syncwarp();
             tensor_stored();
             fence_before();
             __syncwarp();
@@ -1204,61 +1376,75 @@ __device__ void softmax_role(const ChunkArgs& p, ChunkShared<D>& sh, int64_t ste
 
         if (!warp_wait(&sh.c.o_full[tile], units++ % 2, sh.c)) return;
         fence_after();
-        const bool whole = w.begin == 0 && w.end == w.u.steps;
-        const int slot = 2 * int(blockIdx.x) + (w.begin == 0);
-        const int64_t part = int64_t(slot) * kUnitRows + tile * kTile + r;
-        const bool nans = sh.c.nan_unit[w.unit % kNanUnits] == w.unit + 1;
-        const float by = whole ? (l == 0.0f ? 0.0f : v_scale / l) : v_scale;
+        const bool whole = begin == 0 && end == u.steps;
+        const int64_t slot = (2 * int64_t(blockIdx.x) + (begin == 0)) * kUnitRows + tile * kTile + warp_row;
+        const bool nans = sh.c.nan_unit[unit % kNanUnits] == int(unit) + 1;
+        // A row that sees no token has l = 0, and sums of zero weights that count as zeros.
+        const float by = l == 0.0f ? 0.0f : whole ? v_scale / l : v_scale;
+        // The queries are done with: their place takes the rows on their way out, 128 bytes of each at a time.
+        char* const warp_rows = sh.q[tile] + warp_row * 128;
 #pragma unroll 1
-        for (int i = 0; i < D / 32; ++i) {
-            float x[32];
-            tensor_load(sums + 32 * i, x);
-            tensor_loaded(x);
+        for (int i = 0; i < D; i += 32) {
+            float y[32];
+            __syncwarp();
+            tensor_load(sums + i, y);
+            tensor_loaded(y);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) x[j] *= by;
-            if (!valid) continue;
-            if (l == 0.0f) {                             // no token seen here: the sums are of zero weights
-#pragma unroll
-                for (int j = 0; j < 32; ++j) x[j] = 0.0f;
-            }
+            for (int j = 0; j < 32; ++j) y[j] *= by;
             if (nans) {
-                const int from = max(max(w.u.first_seen, 0) / kTile, w.begin) * kTile, to = min(seen, w.end * kTile);
+                uint32_t found = 0;
+                const int from = max(max(u.first_seen, 0) / kTile, begin) * kTile, to = min(seen, end * kTile);
                 for (int t = from; t < to; ++t) {
-                    const int64_t block = ints(a.b.table)[w.u.s * a.b.table_pitch + t / a.c.block_size];
+                    const int64_t block = ints(a.b.table)[u.s * a.b.table_pitch + t / a.c.block_size];
                     if (block < 0 || block >= a.c.blocks) continue;
                     const uint8_t* code = reinterpret_cast<const uint8_t*>(a.c.codes) + a.c.side_pitch +
                                           block * a.c.block_pitch + t % a.c.block_size * a.c.token_pitch +
-                                          w.u.head * a.c.head_pitch + 32 * i;
-#pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        if ((code[j] & 0x7F) == 0x7F) x[j] = NAN;
+                                          u.head * a.c.head_pitch + i;
+#pragma unroll 1
+                    for (int j = 0; j < 32; ++j) found |= uint32_t((code[j] & 0x7F) == 0x7F) << j;
                 }
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    if (found >> j & 1) y[j] = NAN;
             }
             if (whole) {
-                char* to = a.out + ((int64_t(q.row + token) * a.q_heads + head) * D + 32 * i) * 2;
 #pragma unroll
-                for (int j = 0; j < 32; j += 8) {
-                    const float y[8] = {x[j], x[j + 1], x[j + 2], x[j + 3], x[j + 4], x[j + 5], x[j + 6], x[j + 7]};
-                    store8<T>(to + 2 * j, y);
-                }
+                for (int j = 0; j < 32; j += 8)
+                    store_shared(staged(warp_rows, lane, (i % 64 + j) / 8), T::pack(y[j], y[j + 1]),
+                                 T::pack(y[j + 2], y[j + 3]), T::pack(y[j + 4], y[j + 5]), T::pack(y[j + 6], y[j + 7]));
+                if (i % 64 == 0) continue;
             } else {
-                float* to = p.parts.sums + part * D + 32 * i;
 #pragma unroll
                 for (int j = 0; j < 32; j += 4)
-                    *reinterpret_cast<float4*>(to + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+                    store_shared(staged(warp_rows, lane, j / 4), __float_as_uint(y[j]), __float_as_uint(y[j + 1]),
+                                 __float_as_uint(y[j + 2]), __float_as_uint(y[j + 3]));
             }
+            __syncwarp();
+#pragma unroll 2
+            for (int j = 0; j < 8; ++j) {
+                const int mine = j * 4 + lane / 8;
+                const int64_t to = __shfl_sync(~0u, out_row, mine);
+                const uint4 piece = *reinterpret_cast<const uint4*>(staged(warp_rows, mine, lane % 8));
+                if (mine >= rows) continue;
+                char* at = whole ? a.out + (to * D + i - 32) * 2
+                                 : reinterpret_cast<char*>(p.parts.sums + (slot + mine) * D + i);
+                *reinterpret_cast<uint4*>(at + lane % 8 * 16) = piece;
+            }
+            __syncwarp();
         }
         if (!whole) {
-            if (valid) p.parts.ml[part] = make_float2(m, l);
-            if (w.begin == 0 && threadIdx.x == 0) {
-                const int last = int(((pos + w.u.steps) * ctas - 1) / total);
+            if (lane < rows) p.parts.ml[slot + lane] = make_float2(m, l);
+            if (begin == 0 && threadIdx.x == 0) {
+                const int last = int(((u.pos + u.steps) * sh.c.ctas - 1) / sh.c.total);
                 p.parts.units[blockIdx.x] =
-                    SharedUnit{q.row, w.u.head, w.u.first, w.u.rows, last - int(blockIdx.x) + 1};
+                    SharedUnit{u.q.row, u.head, u.first, u.rows, last - int(blockIdx.x) + 1};
             }
         }
-        pos += n_steps;
         fence_before();                                  // the sums are read before the next unit's are written
-    } while (w.next(a));
+        __syncwarp();
+        if (lane == 0) barrier_arrive(&sh.c.unit_free[ring]);
+        if (final) return;
+    }
 }
 
 template <typename T, int D>
@@ -1302,14 +1488,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
                 if (n && first <= pos && pos < before + sum) {
                     sh.c.s = base + i + lane;
                     sh.c.head = int((pos - first) / n);
-                    sh.c.pos = (pos - first) % n;
+                    sh.c.sought = (pos - first) % n;
                 }
                 before += __shfl_sync(~0u, sum, 31);
             }
-            if (lane == 0) sh.c.total = before;
+            if (lane == 0) sh.c.scanned = before;
         }
         __syncthreads();
-        if (sh.c.total > pos) break;
+        if (sh.c.scanned > pos) break;
         __syncthreads();
     }
     if (warp == 0) {
@@ -1325,7 +1511,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
                 if (lane >= k) sum += up;
             }
             const int64_t first = done + sum - n;
-            if (n && first <= sh.c.pos && sh.c.pos < done + sum) sh.c.tile = i + lane, sh.c.step = int(sh.c.pos - first);
+            if (n && first <= sh.c.sought && sh.c.sought < done + sum)
+                sh.c.tile = i + lane, sh.c.step = int(sh.c.sought - first);
             done += __shfl_sync(~0u, sum, 31);
         }
     }
@@ -1341,12 +1528,21 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
             barrier_init(&sh.c.p_full[i], 4);
             barrier_init(&sh.c.o_full[i], 1);
         }
+        for (int i = 0; i < kLooked; ++i) {
+            barrier_init(&sh.c.looked[i], 1);
+            barrier_init(&sh.c.look_free[i], kConvertWarps);
+        }
+        for (int i = 0; i < kLookedUnits; ++i) {
+            barrier_init(&sh.c.unit_looked[i], 1);
+            barrier_init(&sh.c.unit_free[i], 9);         // 8 warps of rows, and the issue
+        }
         barrier_init(&sh.c.drained, 1);
+        sh.c.total = total, sh.c.ctas = ctas, sh.c.pos = pos;
         for (int i = 0; i < kNanUnits; ++i) sh.c.nan_unit[i] = 0;
         sh.c.stop = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == kAll - 1) {
+    if (warp == kIssueWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;"
                      ::"r"(shared_address(&sh.c.tensor)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -1357,19 +1553,23 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
 
     const int64_t steps = end - pos;
     if (warp < 8) {
-        softmax_role<T, D>(p, sh, steps, pos, total, ctas);
+        softmax_role<T, D>(p, sh);
     } else if (warp < 8 + kConvertWarps) {
         convert_role<D>(p, sh, steps);
-    } else if (lane == 0) {
-        issue_role<D>(p, sh, steps);
-        commit(&sh.c.drained);
-        barrier_wait(&sh.c.drained, 0, sh.c, true);
+    } else {
+        if (warp == kLookWarp) {
+            look_role(p, sh.c, steps);
+        } else if (warp == kIssueWarp && lane == 0) {
+            issue_role<D>(sh);
+            commit(&sh.c.drained);
+            barrier_wait(&sh.c.drained, 0, sh.c, true);
+        }
     }
     __syncwarp();
     fence_before();
     __syncthreads();
     fence_after();
-    if (warp == kAll - 1)
+    if (warp == kIssueWarp)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(sh.c.tensor));
     if (threadIdx.x == 0 && sh.c.stop) atomicOr(a.status, KVSNAP_C8_STALLED);
 }

@@ -46,14 +46,18 @@ struct Fp16 {
 
 // 8 consecutive 16-bit elements.
 template <typename T>
-__device__ __forceinline__ void load8(const char* at, float (&v)[8]) {
-    const uint4 x = *reinterpret_cast<const uint4*>(at);
+__device__ __forceinline__ void widen8(const uint4& x, float (&v)[8]) {
     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float2 p = T::wide(w[i]);
         v[2 * i] = p.x, v[2 * i + 1] = p.y;
     }
+}
+
+template <typename T>
+__device__ __forceinline__ void load8(const char* at, float (&v)[8]) {
+    widen8<T>(*reinterpret_cast<const uint4*>(at), v);
 }
 
 template <typename T>
