@@ -116,16 +116,21 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     return d;
 }
 
-__device__ __forceinline__ uint4 load16(const char* at) {
+// 16 (8) bytes of a cache that are read once, or zeros. Predicated, not branched around: where a branch
+// around a load joins, the load is waited for.
+__device__ __forceinline__ uint4 load16(const char* at, bool there) {
     uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(at));
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %5, 0;\nmov.u32 %0, 0;\nmov.u32 %1, 0;\nmov.u32 %2, 0;\nmov.u32 %3, 0;\n"
+                 "@p ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n}"
+                 : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w) : "l"(at), "r"(uint32_t(there)));
     return v;
 }
 
-__device__ __forceinline__ uint2 load8bytes(const char* at) {
+__device__ __forceinline__ uint2 load8bytes(const char* at, bool there) {
     uint2 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(at));
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %3, 0;\nmov.u32 %0, 0;\nmov.u32 %1, 0;\n"
+                 "@p ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];\n}"
+                 : "=&r"(v.x), "=&r"(v.y) : "l"(at), "r"(uint32_t(there)));
     return v;
 }
 
@@ -229,19 +234,16 @@ struct StepWarp {
             for (int half = 0; half < kHalves; ++half)
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                    kr[half][i] = off >= 0 ? load16(k_lane + off + i * two_tokens + 64 * half) : make_uint4(0, 0, 0, 0);
+                    kr[half][i] = load16(k_lane + off + i * two_tokens + 64 * half, off >= 0);
         };
         const auto load_values = [&](int64_t off) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                vr[j] = make_uint4(0, 0, 0, 0);
-                if (off >= 0) {
-                    if constexpr (D == 128) {
-                        vr[j] = load16(v_lane + off + j * c.token_pitch);
-                    } else {
-                        const uint2 x = load8bytes(v_lane + off + j * c.token_pitch);
-                        vr[j].x = x.x, vr[j].y = x.y;
-                    }
+                if constexpr (D == 128) {
+                    vr[j] = load16(v_lane + off + j * c.token_pitch, off >= 0);
+                } else {
+                    const uint2 x = load8bytes(v_lane + off + j * c.token_pitch, off >= 0);
+                    vr[j] = make_uint4(x.x, x.y, 0, 0);
                 }
             }
         };
@@ -643,24 +645,31 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
 //
 // Sequences that the kernel above does not take. Bound by the tensor cores: 4 D operations a
 // query head and visible token, in two products of fp16 operands with 32-bit sums in tensor memory.
-// A CTA takes 256 rows (two tiles of 128) of one KV head over tiles of 128 tokens:
-//   warp 13     looks up the pages of coming tiles and their scales;
-//   warps 8-11  load a tile's codes, one tile ahead, turn them to fp16 and lay them out for the tensor
+// A CTA takes 256 rows (two tiles of 128) of one KV head in steps of 64 tokens:
+//   warp 13     looks up the pages of coming steps and their scales;
+//   warps 8-11  load a step's codes, one step ahead, turn them to fp16 and lay them out for the tensor
 //               cores; both row tiles use them, so a code is converted once per 256 rows;
-//   warp 12     issues S = Q K^T of one row tile while the other's softmax runs, and O += P V;
+//   warp 12     issues S = Q K^T and O += P V, the scores two steps ahead of the sums, so that a
+//               row tile's next scores are there when its softmax of these ends;
 //   warps 0-7   a thread a row: maximum, weights, sums; P goes back to tensor memory over S.
+// Tensor memory holds exactly this: two tiles' sums (2 x 128 columns) and two steps of scores of each
+// (4 x 64). With one step of 128 tokens instead, scores and softmax took turns: 1.02 ms for an 8k
+// prompt of 32 heads.
 // The running maximum follows a row's true maximum only when that exceeds it by 2^8 (weights stay
 // within fp16), so sums in tensor memory are rarely touched. A page's scale goes into the conversion
 // relative to the largest key scale of the tile (which multiplies S) and the largest value scale so
 // far (which divides O at the end): powers of two, exact in fp16.
 
-constexpr int kTile = 128;                 // tokens a step, rows a tile
+constexpr int kTile = 128;                 // rows a tile
 constexpr int kUnitRows = 2 * kTile;
-constexpr int kHalf = kTile / 2;
+constexpr int kStep = 64;                  // tokens a step
+constexpr int kGranules = kStep / kGranule;
+constexpr int kStages = 4;                 // steps of keys and of values in shared memory
 constexpr int kConvertWarps = 4, kIssueWarp = 12, kLookWarp = 13, kChunkThreads = 512;
-constexpr int kLooked = 8;                 // tiles looked up ahead
+constexpr int kLooked = 16;                // steps looked up ahead
+constexpr int kScales = 8;                 // steps whose scales the softmax may still need
 constexpr int kLookedUnits = 4;            // units
-constexpr uint32_t kSumsAt = 256;          // columns of tensor memory: S and P 0, 128; O 256, 384
+constexpr uint32_t kSumsAt = 256;          // columns of tensor memory: S and P 0 to 255, O from here
 
 struct ChunkArgs {
     AttendArgs a;
@@ -673,7 +682,7 @@ struct Unit {
     int s, head, tile;        // sequence, KV head, tile of 256 rows
     int first, rows;          // its rows of the head
     int first_seen;           // tokens that its first row sees
-    int steps;                // tiles of tokens that its last row sees
+    int steps;                // that its last row sees
 };
 
 __device__ __forceinline__ bool chunk_sequence(const AttendArgs& a, int s, Sequence& q) {
@@ -683,7 +692,7 @@ __device__ __forceinline__ bool chunk_sequence(const AttendArgs& a, int s, Seque
 __device__ __forceinline__ int steps_of(const AttendArgs& a, const Sequence& q, int tile) {
     const int last = min(q.rows * a.group, (tile + 1) * kUnitRows) - 1;
     const int seen = q.length - q.rows + last / a.group + 1;
-    return max(1, (seen + kTile - 1) / kTile);
+    return max(1, (seen + kStep - 1) / kStep);
 }
 
 __device__ __forceinline__ int row_tiles(const AttendArgs& a, const Sequence& q) {
@@ -706,11 +715,11 @@ constexpr int kNanUnits = 64;              // more units than the roles can be a
 
 // What a step's conversion needs to know.
 struct Looked {
-    int64_t keys[kTile / kGranule];        // addresses of the granules' key codes; 0: not there
-    uint32_t k_by[kTile / kGranule], v_by[kTile / kGranule];   // their scales relative to the two below, as fp16 pairs
-    float k_scale, v_scale;                // largest key scale of the tile; largest value scale so far
+    int64_t keys[kGranules];               // addresses of the granules' key codes; 0: not there
+    uint32_t k_by[kGranules], v_by[kGranules];   // their scales relative to the two below, as fp16 pairs
+    float k_scale, v_scale;                // largest key scale of the step; largest value scale so far
     uint32_t live;                         // granules that are there
-    int tokens;                            // of the tile that the sequence has
+    int tokens;                            // of the step that the sequence has
     int edge;                              // some row does not see all of them
     int unit;
 };
@@ -724,14 +733,15 @@ struct LookedUnit {
 };
 
 struct ChunkControl {
-    uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], drained;
+    uint64_t q_full[2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
+    uint64_t s_full[2][2], p_full[2][2], o_full[2][2], drained;    // of a row tile; of a step's turn
     uint64_t looked[kLooked], look_free[kLooked];
     Looked look[kLooked];
     uint64_t unit_looked[kLookedUnits], unit_free[kLookedUnits];
     LookedUnit unit[kLookedUnits];
-    float k_scale[4], v_scale[4];          // of a step's tile: largest key scale; largest value scale so far
-    uint32_t live[4];                      // of a step's tile: its 16-token granules that are there
-    int nan_unit[kNanUnits];               // a unit (counted from 1) whose last tiles hold a NaN value
+    float k_scale[kScales], v_scale[kScales];    // of a step: largest key scale; largest value scale so far
+    uint32_t live[kScales];                // of a step: its 16-token granules that are there
+    int nan_unit[kNanUnits];               // a unit (counted from 1) whose last steps hold a NaN value
     uint32_t tensor;                       // tensor memory's address
     volatile int stop;                     // a wait ran out
     int64_t counts[kScanned], scratch[32];
@@ -742,8 +752,8 @@ struct ChunkControl {
 template <int D>
 struct ChunkShared {
     char q[2][kTile * D * 2];
-    char k[2][kTile * D * 2];
-    char v[2][kTile * D * 2];
+    char k[kStages][kStep * D * 2];
+    char v[kStages][kStep * D * 2];
     ChunkControl c;
 };
 
@@ -826,9 +836,13 @@ __device__ __forceinline__ bool warp_wait(uint64_t* b, uint32_t parity, ChunkCon
     return __all_sync(~0u, barrier_wait(b, parity, c));
 }
 
-__device__ __forceinline__ void commit(uint64_t* b) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
-                 ::"r"(shared_address(b)) : "memory");
+// The tensor cores' instructions are issued by one lane, `chosen`, of a warp that goes through the code
+// as a whole, so that addresses stay in uniform registers: built by a lane alone, each instruction took
+// 70 to 110 clocks to issue, for 32 to 64 of work.
+__device__ __forceinline__ void commit(uint64_t* b, uint32_t chosen) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %1, 0;\n"
+                 "@p tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}"
+                 ::"r"(shared_address(b)), "r"(chosen) : "memory");
 }
 
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -838,25 +852,29 @@ __device__ __forceinline__ void fence_shared() { asm volatile("fence.proxy.async
 // A matrix in shared memory in rows of 128 bytes, 128-byte swizzled in groups of 8 rows (1 KiB).
 // By rows of K (keys, queries): a row is 64 of the contracted elements, `lead` is not used.
 // By rows of N (values): a row is 64 columns of one contracted element; `lead` is the way to the next 64.
-__device__ __forceinline__ uint64_t matrix(uint32_t at, uint32_t lead) {
-    return uint64_t(at >> 4 & 0x3FFF) | uint64_t(lead >> 4) << 16 | uint64_t(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
-}
+// Low word of its description; the high one is the same for all.
+__device__ __forceinline__ uint32_t matrix(uint32_t at, uint32_t lead) { return at >> 4 | lead >> 4 << 16; }
+constexpr uint32_t kMatrixHigh = 1024 >> 4 | 1 << 14 | 2 << 29;
 
 // 128 x n products of fp16 with 32-bit sums; by_n: B lies by rows of N.
 __host__ __device__ constexpr uint32_t instruction(int n, bool by_n) {
     return 1u << 4 | uint32_t(by_n) << 16 | uint32_t(n >> 3) << 17 | uint32_t(kTile >> 4) << 24;
 }
 
-__device__ __forceinline__ void mma_shared(uint32_t d, uint64_t a, uint64_t b, uint32_t what, bool add) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(what), "r"(uint32_t(add)) : "memory");
+__device__ __forceinline__ void mma_shared(uint32_t d, uint32_t a, uint32_t b, uint32_t what, uint32_t add,
+                                           uint32_t chosen) {
+    asm volatile("{\n.reg .pred p, q;\n.reg .b64 a, b;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\n"
+                 "mov.b64 a, {%1, %6};\nmov.b64 b, {%2, %6};\n"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n}"
+                 ::"r"(d), "r"(a), "r"(b), "r"(what), "r"(add), "r"(chosen), "r"(kMatrixHigh) : "memory");
 }
 
-__device__ __forceinline__ void mma_tensor(uint32_t d, uint32_t a, uint64_t b, uint32_t what, bool add) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
-                 ::"r"(d), "r"(a), "l"(b), "r"(what), "r"(uint32_t(add)) : "memory");
+__device__ __forceinline__ void mma_tensor(uint32_t d, uint32_t a, uint32_t b, uint32_t what, uint32_t add,
+                                           uint32_t chosen) {
+    asm volatile("{\n.reg .pred p, q;\n.reg .b64 b;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\n"
+                 "mov.b64 b, {%2, %6};\n"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n}"
+                 ::"r"(d), "r"(a), "r"(b), "r"(what), "r"(add), "r"(chosen), "r"(kMatrixHigh) : "memory");
 }
 
 // 32 columns of the warp's 32 rows of tensor memory, a row a lane.
@@ -972,10 +990,10 @@ __device__ __forceinline__ void tensor_store(uint32_t at, const uint32_t (&v)[16
 
 __device__ __forceinline__ void tensor_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Where 16 bytes (8 fp16) `chunk` of row r lie in a matrix of rows of D fp16.
-template <int D>
+// Where 16 bytes (8 fp16) `chunk` of row r lie in a matrix of R rows of fp16.
+template <int R>
 __device__ __forceinline__ uint32_t swizzled(int r, int chunk) {
-    return uint32_t(chunk / 8) * (kTile * 128) + uint32_t(r) * 128 + uint32_t((chunk % 8) ^ (r % 8)) * 16;
+    return uint32_t(chunk / 8) * (R * 128) + uint32_t(r) * 128 + uint32_t((chunk % 8) ^ (r % 8)) * 16;
 }
 
 __device__ __forceinline__ void store_shared(char* at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -988,11 +1006,12 @@ __device__ __forceinline__ uint32_t times_half2(uint32_t a, uint32_t b) {
     return d;
 }
 
-// The role of warp 13: 4 tiles at a time, a lane a granule.
+// The role of warp 13: 8 steps at a time, a lane a granule.
 __device__ __forceinline__ void look_role(const ChunkArgs& p, ChunkControl& c, int64_t steps) {
     const AttendArgs& a = p.a;
     const Cache& cache = a.c;
-    const int lane = threadIdx.x % 32, part = lane / 8, granule = lane % 8;
+    const int lane = threadIdx.x % 32, part = lane / kGranules, granule = lane % kGranules;
+    constexpr int kParts = 32 / kGranules;
     Walk w;
     if (!w.start(a, c, steps)) return;
     float v_carry = 0.0f;
@@ -1008,8 +1027,8 @@ __device__ __forceinline__ void look_role(const ChunkArgs& p, ChunkControl& c, i
                 barrier_arrive(&c.unit_looked[k]);
             }
         }
-        const int n = min(4, w.end - w.step), step = w.step + part;
-        const int64_t token = int64_t(step) * kTile + granule * kGranule;
+        const int n = min(kParts, w.end - w.step), step = w.step + part;
+        const int64_t token = int64_t(step) * kStep + granule * kGranule;
         int64_t at = 0;
         float ks = 0.0f, vs = 0.0f;
         if (part < n && token < w.u.q.length) {
@@ -1023,20 +1042,20 @@ __device__ __forceinline__ void look_role(const ChunkArgs& p, ChunkControl& c, i
                 ks = scales[0], vs = scales[cache.kv_heads];
             }
         }
-        const uint32_t live = __ballot_sync(~0u, at != 0) >> (8 * part) & 0xFF;
+        const uint32_t live = __ballot_sync(~0u, at != 0) >> (kGranules * part) & ((1u << kGranules) - 1);
         float k_top = ks, v_top = vs;
 #pragma unroll
-        for (int k = 4; k; k >>= 1) {
+        for (int k = kGranules / 2; k; k >>= 1) {
             k_top = fmaxf(k_top, __shfl_xor_sync(~0u, k_top, k));
             v_top = fmaxf(v_top, __shfl_xor_sync(~0u, v_top, k));
         }
 #pragma unroll
-        for (int k = 8; k < 32; k <<= 1) {
+        for (int k = kGranules; k < 32; k <<= 1) {
             const float up = __shfl_up_sync(~0u, v_top, k);
             if (lane >= k) v_top = fmaxf(v_top, up);
         }
         v_top = fmaxf(v_top, v_carry);
-        v_carry = __shfl_sync(~0u, v_top, 8 * (n - 1));
+        v_carry = __shfl_sync(~0u, v_top, kGranules * (n - 1));
         const __half2 k_by = __float2half2_rn(k_top > 0.0f ? ks / k_top : 0.0f);
         const __half2 v_by = __float2half2_rn(v_top > 0.0f ? vs / v_top : 0.0f);
         for (int i = 0; i < n; ++i)
@@ -1048,8 +1067,8 @@ __device__ __forceinline__ void look_role(const ChunkArgs& p, ChunkControl& c, i
             to.v_by[granule] = reinterpret_cast<const uint32_t&>(v_by);
             if (granule == 0) {
                 to.k_scale = k_top, to.v_scale = v_top, to.live = live;
-                to.tokens = int(min(int64_t(kTile), max(int64_t(0), w.u.q.length - token)));
-                to.edge = int64_t(step + 1) * kTile > w.u.first_seen;
+                to.tokens = int(min(int64_t(kStep), max(int64_t(0), w.u.q.length - token)));
+                to.edge = int64_t(step + 1) * kStep > w.u.first_seen;
                 to.unit = w.unit;
             }
         }
@@ -1066,7 +1085,7 @@ __device__ __forceinline__ void look_role(const ChunkArgs& p, ChunkControl& c, i
 // The role of warps 8-11.
 template <int D>
 __device__ __forceinline__ void convert_role(const ChunkArgs& p, ChunkShared<D>& sh, int64_t steps) {
-    constexpr int kAcross = D / 16, kTokens = 32 * kConvertWarps / kAcross, kEach = kTile / kTokens;
+    constexpr int kAcross = D / 16, kTokens = 32 * kConvertWarps / kAcross, kEach = kStep / kTokens;
     const Cache& c = p.a.c;
     const int tid = threadIdx.x - 256, lane = threadIdx.x % 32;
     // A thread's 16 codes: token my_token + i * kTokens, dims 16 * piece. Of 8 consecutive lanes
@@ -1075,146 +1094,157 @@ __device__ __forceinline__ void convert_role(const ChunkArgs& p, ChunkShared<D>&
     const int piece = D == 128 ? tid % 4 + tid / 8 % 2 * 4 : tid % 4;
     const int64_t within = my_token % kGranule * c.token_pitch + 16 * piece;
 
-    // Keys and values of a tile in turn, the next load on its way while one is converted: item i is
-    // side i % 2 of step i / 2.
-    uint4 now[kEach], next[kEach];
-    const auto load = [&](uint4 (&to)[kEach], int64_t item) {
-        const Looked& look = sh.c.look[item / 2 % kLooked];
-        const int64_t side = item % 2 ? c.side_pitch : 0;
+    // Keys and values in turn, the next load on its way while one is converted.
+    const auto load = [&](uint4 (&to)[kEach], int64_t step, int64_t side) {
+        const Looked& look = sh.c.look[step % kLooked];
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
             const int token = my_token + i * kTokens;
             const int64_t at = look.keys[token / kGranule];
             // Slots behind the last token hold anything, NaN included: they count as zeros.
-            to[i] = make_uint4(0, 0, 0, 0);
-            if (at && token < look.tokens) to[i] = load16(reinterpret_cast<const char*>(at) + side + within);
+            to[i] = load16(reinterpret_cast<const char*>(at) + side + within, at && token < look.tokens);
         }
     };
-#pragma unroll 1
-    for (int64_t item = -1; item < 2 * steps; ++item) {
-        if (item + 1 < 2 * steps) {
-            const int64_t step = (item + 1) / 2;
-            if (item % 2 && !warp_wait(&sh.c.looked[step % kLooked], uint32_t(step / kLooked) % 2, sh.c)) return;
-            load(next, item + 1);
+    const auto convert = [&](const uint4 (&from)[kEach], char* to, const uint32_t* by) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int token = my_token + i * kTokens;
+            const uint32_t f = by[token / kGranule];
+            const uint32_t x[4] = {from[i].x, from[i].y, from[i].z, from[i].w};
+            uint32_t h[8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                h[2 * j] = times_half2(half2_of_codes(uint16_t(x[j])), f);
+                h[2 * j + 1] = times_half2(half2_of_codes(uint16_t(x[j] >> 16)), f);
+            }
+            store_shared(to + swizzled<kStep>(token, 2 * piece), h[0], h[1], h[2], h[3]);
+            store_shared(to + swizzled<kStep>(token, 2 * piece + 1), h[4], h[5], h[6], h[7]);
         }
-        if (item >= 0) {
-            const int64_t step = item / 2;
-            const int slot = step % 2, side = item % 2;
-            const Looked& look = sh.c.look[step % kLooked];
-            if (side == 0 && tid == 0) {
-                sh.c.k_scale[step % 4] = look.k_scale, sh.c.v_scale[step % 4] = look.v_scale;
-                sh.c.live[step % 4] = look.live;
-            }
-            if (side && look.edge) {
-                // Some row does not see some of these tokens, and a weight of 0 times NaN is NaN: NaN
-                // values are left out here, and put back at the end into the rows that see them.
-                bool found = false;
-#pragma unroll
-                for (int i = 0; i < kEach; ++i) {
-                    uint32_t x[4] = {now[i].x, now[i].y, now[i].z, now[i].w};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint32_t bad = ((x[j] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
-                        found |= bad != 0;
-                        x[j] &= ~((bad >> 7) * 0xFFu);
-                    }
-                    now[i] = make_uint4(x[0], x[1], x[2], x[3]);
-                }
-                if (found) sh.c.nan_unit[look.unit % kNanUnits] = look.unit + 1;
-            }
-            if (!warp_wait(side ? &sh.c.v_empty[slot] : &sh.c.k_empty[slot], uint32_t(step / 2 + 1) % 2, sh.c)) return;
-            char* const to = side ? sh.v[slot] : sh.k[slot];
-            const uint32_t* by = side ? look.v_by : look.k_by;
+        fence_shared();
+        __syncwarp();
+    };
+    uint4 kr[kEach], vr[kEach];
+    if (!warp_wait(&sh.c.looked[0], 0, sh.c)) return;
+    load(kr, 0, 0);
+#pragma unroll 1
+    for (int64_t step = 0; step < steps; ++step) {
+        const int slot = step % kStages;
+        const uint32_t free = uint32_t(step / kStages + 1) % 2;
+        const Looked& look = sh.c.look[step % kLooked];
+        load(vr, step, c.side_pitch);
+        if (tid == 0) {
+            sh.c.k_scale[step % kScales] = look.k_scale, sh.c.v_scale[step % kScales] = look.v_scale;
+            sh.c.live[step % kScales] = look.live;
+        }
+        if (!warp_wait(&sh.c.k_empty[slot], free, sh.c)) return;
+        convert(kr, sh.k[slot], look.k_by);
+        if (lane == 0) barrier_arrive(&sh.c.k_full[slot]);
+        if (step + 1 < steps) {
+            if (!warp_wait(&sh.c.looked[(step + 1) % kLooked], uint32_t((step + 1) / kLooked) % 2, sh.c)) return;
+            load(kr, step + 1, 0);
+        }
+        if (look.edge) {
+            // Some row does not see some of these tokens, and a weight of 0 times NaN is NaN: NaN
+            // values are left out here, and put back at the end into the rows that see them.
+            bool found = false;
 #pragma unroll
             for (int i = 0; i < kEach; ++i) {
-                const int token = my_token + i * kTokens;
-                const uint32_t f = by[token / kGranule];
-                const uint32_t x[4] = {now[i].x, now[i].y, now[i].z, now[i].w};
-                uint32_t h[8];
+                uint32_t x[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    h[2 * j] = times_half2(half2_of_codes(uint16_t(x[j])), f);
-                    h[2 * j + 1] = times_half2(half2_of_codes(uint16_t(x[j] >> 16)), f);
+                    const uint32_t bad = ((x[j] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+                    found |= bad != 0;
+                    x[j] &= ~((bad >> 7) * 0xFFu);
                 }
-                store_shared(to + swizzled<D>(token, 2 * piece), h[0], h[1], h[2], h[3]);
-                store_shared(to + swizzled<D>(token, 2 * piece + 1), h[4], h[5], h[6], h[7]);
+                vr[i] = make_uint4(x[0], x[1], x[2], x[3]);
             }
-            fence_shared();
-            __syncwarp();
-            if (lane == 0) {
-                barrier_arrive(side ? &sh.c.v_full[slot] : &sh.c.k_full[slot]);
-                if (side) barrier_arrive(&sh.c.look_free[step % kLooked]);
-            }
+            if (found) sh.c.nan_unit[look.unit % kNanUnits] = look.unit + 1;
         }
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) now[i] = next[i];
+        if (!warp_wait(&sh.c.v_empty[slot], free, sh.c)) return;
+        convert(vr, sh.v[slot], look.v_by);
+        if (lane == 0) {
+            barrier_arrive(&sh.c.v_full[slot]);
+            barrier_arrive(&sh.c.look_free[step % kLooked]);
+        }
     }
 }
 
-// The role of warp 12's first lane.
+// The role of warp 12.
 template <int D>
 __device__ __forceinline__ void issue_role(ChunkShared<D>& sh) {
-    constexpr uint32_t kScores = instruction(kTile, false), kSums = instruction(D, true);
-    const uint32_t tensor = sh.c.tensor;
-    const auto scores = [&](int tile, int slot) {
-        const uint64_t q = matrix(shared_address(sh.q[tile]), 16), k = matrix(shared_address(sh.k[slot]), 16);
+    constexpr uint32_t kScores = instruction(kStep, false), kSums = instruction(D, true);
+    const uint32_t tensor = __shfl_sync(~0u, sh.c.tensor, 0);
+    uint32_t chosen;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xFFFFFFFF;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(chosen));
+    const uint32_t q_at = matrix(shared_address(sh.q[0]), 16), k_at = matrix(shared_address(sh.k[0]), 16);
+    const uint32_t v_at = matrix(shared_address(sh.v[0]), kStep * 128);
+    // S of a row tile's step, in the half of its columns that the step's turn gives.
+    const auto scores = [&](uint32_t tile, uint32_t step, uint32_t turn) {
+        const uint32_t d = tensor + tile * kTile + turn % 2 * kStep;
+        const uint32_t q = q_at + tile * (sizeof(sh.q[0]) >> 4), k = k_at + step % kStages * (sizeof(sh.k[0]) >> 4);
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-            const uint64_t along = uint64_t((i / 4 * kTile * 128 + i % 4 * 32) >> 4);
-            mma_shared(tensor + tile * kTile, q + along, k + along, kScores, i > 0);
-        }
-        commit(&sh.c.s_full[tile]);
+        for (int i = 0; i < D / 16; ++i)
+            mma_shared(d, q + ((i / 4 * kTile * 128 + i % 4 * 32) >> 4), k + ((i / 4 * kStep * 128 + i % 4 * 32) >> 4),
+                       kScores, i > 0, chosen);
+        commit(&sh.c.s_full[tile][turn % 2], chosen);
     };
-    const auto sums = [&](int tile, int slot, bool add) {
-        const uint64_t v = matrix(shared_address(sh.v[slot]), kTile * 128);
+    const auto sums = [&](uint32_t tile, uint32_t step, uint32_t turn, bool add) {
+        const uint32_t d = tensor + kSumsAt + tile * kTile, p = tensor + tile * kTile + turn % 2 * kStep;
+        const uint32_t v = v_at + step % kStages * (sizeof(sh.v[0]) >> 4);
 #pragma unroll
-        for (int i = 0; i < kTile / 16; ++i)
-            mma_tensor(tensor + kSumsAt + tile * kTile, tensor + tile * kTile + 8 * i, v + uint64_t(i * 2048 >> 4), kSums,
-                       add || i > 0);
+        for (int i = 0; i < kStep / 16; ++i)
+            mma_tensor(d, p + 8 * i, v + (i * 2048 >> 4), kSums, add || i > 0, chosen);
+        commit(&sh.c.o_full[tile][turn % 2], chosen);
     };
     uint32_t it = 0;
-    uint32_t turn[2] = {0, 0}, q_turn[2] = {0, 0};   // steps and units that each row tile has had
+    uint32_t turn0 = 0, turn1 = 0, q_turn0 = 0, q_turn1 = 0;     // steps and units that each row tile has had
     for (uint32_t unit = 0;; ++unit) {
-        if (!barrier_wait(&sh.c.unit_looked[unit % kLookedUnits], unit / kLookedUnits % 2, sh.c)) return;
+        if (!warp_wait(&sh.c.unit_looked[unit % kLookedUnits], unit / kLookedUnits % 2, sh.c)) return;
         const LookedUnit& u = sh.c.unit[unit % kLookedUnits];
-        const int tiles = u.rows > kTile ? 2 : 1, n = u.end - u.begin;
-        const bool final = u.last;
-        barrier_arrive(&sh.c.unit_free[unit % kLookedUnits]);
+        const bool both = __shfl_sync(~0u, u.rows, 0) > kTile, final = __shfl_sync(~0u, u.last, 0);
+        const int n = __shfl_sync(~0u, u.end - u.begin, 0);
+        if (chosen) barrier_arrive(&sh.c.unit_free[unit % kLookedUnits]);
+        if (!warp_wait(&sh.c.q_full[0], q_turn0++ % 2, sh.c)) return;
+        if (both && !warp_wait(&sh.c.q_full[1], q_turn1++ % 2, sh.c)) return;
+        // A step's sums, then the scores of the step after the next, which take the columns of its weights.
 #pragma unroll 1
-        for (int t = 0; t < tiles; ++t) {
-            if (!barrier_wait(&sh.c.q_full[t], q_turn[t]++ % 2, sh.c)) return;
-        }
-        // A step's sums, then the next one's scores; step -1 has no sums, the last no scores.
-#pragma unroll 1
-        for (int step = -1; step < n; ++step) {
-#pragma unroll 1
-            for (int t = 0; t < tiles; ++t) {
+        for (int step = -2; step < n; ++step) {
+            const uint32_t now = it + step, ahead = it + step + 2;
+            const bool more = step + 2 < n;
+            if (step >= 0) {
+                if (!warp_wait(&sh.c.p_full[0][turn0 % 2], turn0 / 2 % 2, sh.c)) return;
+                if (!warp_wait(&sh.c.v_full[now % kStages], now / kStages % 2, sh.c)) return;
+                fence_after();
+                sums(0, now, turn0, step > 0);
+                if (!both) commit(&sh.c.v_empty[now % kStages], chosen);
+            }
+            if (more) {
+                if (!warp_wait(&sh.c.k_full[ahead % kStages], ahead / kStages % 2, sh.c)) return;
+                fence_after();
+                scores(0, ahead, step >= 0 ? turn0 + 2 : turn0 + step + 2);
+                if (!both) commit(&sh.c.k_empty[ahead % kStages], chosen);
+            }
+            if (both) {
                 if (step >= 0) {
-                    if (!barrier_wait(&sh.c.p_full[t], turn[t]++ % 2, sh.c)) return;
-                    if (t == 0 && !barrier_wait(&sh.c.v_full[it % 2], it / 2 % 2, sh.c)) return;
+                    if (!warp_wait(&sh.c.p_full[1][turn1 % 2], turn1 / 2 % 2, sh.c)) return;
                     fence_after();
-                    sums(t, it % 2, step > 0);
-                    if (step + 1 == n) commit(&sh.c.o_full[t]);
-                    if (t + 1 == tiles) commit(&sh.c.v_empty[it % 2]);
+                    sums(1, now, turn1, step > 0);
+                    commit(&sh.c.v_empty[now % kStages], chosen);
                 }
-                if (step + 1 < n) {
-                    const uint32_t next = step < 0 ? it : it + 1;
-                    if (t == 0) {
-                        if (!barrier_wait(&sh.c.k_full[next % 2], next / 2 % 2, sh.c)) return;
-                        fence_after();
-                    }
-                    scores(t, next % 2);
-                    if (t + 1 == tiles) commit(&sh.c.k_empty[next % 2]);
+                if (more) {
+                    scores(1, ahead, step >= 0 ? turn1 + 2 : turn1 + step + 2);
+                    commit(&sh.c.k_empty[ahead % kStages], chosen);
                 }
             }
-            if (step >= 0) ++it;
+            if (step >= 0) ++turn0, turn1 += both;
         }
+        it += n;
         if (final) return;
     }
 }
 
-// Four lanes of 128 columns of a row to, and from, a warp's 4 KB of shared memory: 32 rows of 128 bytes,
-// in which rows go out (8 lanes a row) that came a lane a row.
+// 16 bytes `chunk` of a row in a warp's 4 KB of shared memory: 32 rows of 128 bytes, in which rows that
+// came a lane a row go out 8 lanes a row.
 __device__ __forceinline__ char* staged(char* warp_rows, int row, int chunk) {
     return warp_rows + row * 128 + (chunk ^ row % 8) * 16;
 }
@@ -1226,7 +1256,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs& p, ChunkShared<D>&
     const AttendArgs& a = p.a;
     const int tile = threadIdx.x / 128, r = threadIdx.x % 128, lane = threadIdx.x % 32, warp_row = r - lane;
     const uint32_t scores = sh.c.tensor + (uint32_t(warp_row) << 16) + tile * kTile, sums = scores + kSumsAt;
-    uint32_t it = 0, turn = 0, units = 0;
+    uint32_t it = 0, turn = 0;
     for (uint32_t unit = 0;; ++unit) {
         const int ring = unit % kLookedUnits;
         if (!warp_wait(&sh.c.unit_looked[ring], unit / kLookedUnits % 2, sh.c)) return;
@@ -1262,20 +1292,22 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs& p, ChunkShared<D>&
             }
 #pragma unroll
             for (int i = 0; i < kLanes; ++i)
-                *reinterpret_cast<uint4*>(to + swizzled<D>(warp_row + i * (32 / kLanes) + lane / kLanes, lane % kLanes)) = raw[i];
+                *reinterpret_cast<uint4*>(to + swizzled<kTile>(warp_row + i * (32 / kLanes) + lane / kLanes, lane % kLanes)) = raw[i];
             __syncwarp();
-            float top = 0.0f, v[8];
-#pragma unroll 1
+            uint32_t tops = 0;
+#pragma unroll 4
             for (int i = 0; i < kLanes; ++i) {
-                load8<T>(to + swizzled<D>(r, i), v);
-                top = max8(v, top);
+                const uint4 x = *reinterpret_cast<const uint4*>(to + swizzled<kTile>(r, i));
+                tops = T::max_size(T::max_size(T::max_size(T::max_size(tops, x.x), x.y), x.z), x.w);
             }
-            const int e = max(int(__float_as_uint(top) >> 23), 27);
+            const float2 pair = T::wide(tops);
+            const int e = max(int(__float_as_uint(fmaxf(pair.x, pair.y)) >> 23), 27);
             const float up = __uint_as_float(uint32_t(127 + 14 + 127 - e) << 23);
             factor = __uint_as_float(uint32_t(max(e - 14, 1)) << 23) * a.scale;
-#pragma unroll 1
+#pragma unroll 4
             for (int i = 0; i < kLanes; ++i) {
-                char* const at = to + swizzled<D>(r, i);
+                char* const at = to + swizzled<kTile>(r, i);
+                float v[8];
                 load8<T>(at, v);
                 store_shared(at, pack_half2(v[0] * up, v[1] * up), pack_half2(v[2] * up, v[3] * up),
                              pack_half2(v[4] * up, v[5] * up), pack_half2(v[6] * up, v[7] * up));
@@ -1287,83 +1319,70 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs& p, ChunkShared<D>&
 
         float m = kLowest, l = 0.0f, v_scale = 0.0f;
         for (int step = begin; step < end; ++step, ++it) {
-            if (!warp_wait(&sh.c.s_full[tile], turn % 2, sh.c)) return;
-            ++turn;
+            if (!warp_wait(&sh.c.s_full[tile][turn % 2], turn / 2 % 2, sh.c)) return;
             fence_after();
+            const uint32_t at = scores + turn % 2 * kStep;
+            float x[kStep];
+            tensor_load(at, x);
             // Never 0, so that a hidden score stays -infinity.
-            const float f = fmaxf(factor * sh.c.k_scale[it % 4], 1.17549435e-38f), now_v = sh.c.v_scale[it % 4];
-            const uint32_t live = sh.c.live[it % 4];
-            const int see = min(seen - step * kTile, kTile);       // columns up to here are seen
-            const bool masked = __any_sync(~0u, see < kTile) || live != 0xFF;
-            // Three passes over half a row each: the second half's maximum, the first half's maximum and
-            // weights, the second half's weights. It is read twice as registers hold one half; and
-            // rolled up, as three roles' unrolled code would not stay in the instruction cache.
+            const float f = fmaxf(factor * sh.c.k_scale[it % kScales], 1.17549435e-38f);
+            const float now_v = sh.c.v_scale[it % kScales];
+            const uint32_t live = sh.c.live[it % kScales];
+            const int see = min(max(seen - step * kStep, 0), kStep);       // columns up to here are seen
+            tensor_loaded(x);
+            if (__any_sync(~0u, see < kStep) || live != (1u << kGranules) - 1) {
+                uint64_t bits = see == kStep ? ~0ull : (1ull << see) - 1;
+#pragma unroll
+                for (int i = 0; i < kGranules; ++i)
+                    if (!(live >> i & 1)) bits &= ~(0xFFFFull << (kGranule * i));
+#pragma unroll
+                for (int i = 0; i < kStep; ++i)
+                    if (!(bits >> i & 1)) x[i] = -INFINITY;
+            }
             float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int j = 0; j < kStep; j += 8)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) tops[i] = max3(tops[i], x[j + 2 * i], x[j + 2 * i + 1]);
+            const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * f;
+            float keep = 1.0f;
+            if (top > m + kSlack) {
+                keep = exp2_fast(m - top);
+                m = top, l *= keep;
+            }
+            if (now_v != v_scale) {
+                keep *= v_scale / now_v;
+                v_scale = now_v;
+            }
+            if (step > begin && __any_sync(~0u, keep != 1.0f)) {
+                // The sums so far, in tensor memory, once the step before is in them.
+                if (!warp_wait(&sh.c.o_full[tile][(turn - 1) % 2], (turn - 1) / 2 % 2, sh.c)) return;
+                fence_after();
+#pragma unroll 1
+                for (int i = 0; i < D / 16; ++i) {
+                    float y[16];
+                    __syncwarp();                        // lanes meet before each access to tensor memory
+                    tensor_load(sums + 16 * i, y);
+                    tensor_loaded(y);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) y[j] *= keep;
+                    tensor_store(sums + 16 * i, y);
+                }
+            }
             float2 some[2] = {};
-#pragma unroll 1
-            for (int pass = 0; pass < 3; ++pass) {
-                const int half = pass != 1;
-                float x[kHalf];
-                __syncwarp();                            // lanes meet before each access to tensor memory
-                tensor_load(scores + half * kHalf, x);
-                tensor_loaded(x);
-                if (masked) {
-                    const int shown = min(max(see - half * kHalf, 0), kHalf);
-                    uint64_t bits = shown == kHalf ? ~0ull : (1ull << shown) - 1;
+            const float2 ff = make_float2(f, f), mm = make_float2(-m, -m);
 #pragma unroll
-                    for (int i = 0; i < kHalf / kGranule; ++i)
-                        if (!(live >> (half * kHalf / kGranule + i) & 1)) bits &= ~(0xFFFFull << (kGranule * i));
+            for (int i = 0; i < kStep; i += 32) {
+                uint32_t weights[16];
 #pragma unroll
-                    for (int i = 0; i < kHalf; ++i)
-                        if (!(bits >> i & 1)) x[i] = -INFINITY;
+                for (int j = 0; j < 16; ++j) {
+                    float2 y = fma2(make_float2(x[i + 2 * j], x[i + 2 * j + 1]), ff, mm);
+                    y.x = exp2_fast(y.x), y.y = exp2_fast(y.y);
+                    some[j % 2] = add2(some[j % 2], y);
+                    weights[j] = pack_half2(y.x, y.y);
                 }
-                if (pass < 2) {
-#pragma unroll
-                    for (int j = 0; j < kHalf; j += 8)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) tops[i] = max3(tops[i], x[j + 2 * i], x[j + 2 * i + 1]);
-                }
-                if (pass == 1) {
-                    const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * f;
-                    float keep = 1.0f;
-                    if (top > m + kSlack) {
-                        keep = exp2_fast(m - top);
-                        m = top, l *= keep;
-                    }
-                    if (now_v != v_scale) {
-                        keep *= v_scale / now_v;
-                        v_scale = now_v;
-                    }
-                    // Sums in tensor memory: complete up to the step before, as these scores were issued after them.
-                    if (step > begin && __any_sync(~0u, keep != 1.0f)) {
-#pragma unroll 1
-                        for (int i = 0; i < D / 16; ++i) {
-                            float y[16];
-                            __syncwarp();
-                            tensor_load(sums + 16 * i, y);
-                            tensor_loaded(y);
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) y[j] *= keep;
-                            tensor_store(sums + 16 * i, y);
-                        }
-                    }
-                }
-                if (pass > 0) {
-                    const float2 ff = make_float2(f, f), mm = make_float2(-m, -m);
-#pragma unroll
-                    for (int i = 0; i < kHalf; i += 32) {
-                        uint32_t weights[16];
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            float2 y = fma2(make_float2(x[i + 2 * j], x[i + 2 * j + 1]), ff, mm);
-                            y.x = exp2_fast(y.x), y.y = exp2_fast(y.y);
-                            some[j % 2] = add2(some[j % 2], y);
-                            weights[j] = pack_half2(y.x, y.y);
-                        }
-                        __syncwarp();
-                        tensor_store(scores + (half * kHalf + i) / 2, weights);
-                    }
-                }
+                __syncwarp();
+                tensor_store(at + i / 2, weights);
             }
             some[0] = add2(some[0], some[1]);
             l += some[0].x + some[0].y;
@@ -1371,10 +1390,11 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs& p, ChunkShared<D>&
             tensor_stored();
             fence_before();
             __syncwarp();
-            if (lane == 0) barrier_arrive(&sh.c.p_full[tile]);
+            if (lane == 0) barrier_arrive(&sh.c.p_full[tile][turn % 2]);
+            ++turn;
         }
 
-        if (!warp_wait(&sh.c.o_full[tile], units++ % 2, sh.c)) return;
+        if (!warp_wait(&sh.c.o_full[tile][(turn - 1) % 2], (turn - 1) / 2 % 2, sh.c)) return;
         fence_after();
         const bool whole = begin == 0 && end == u.steps;
         const int64_t slot = (2 * int64_t(blockIdx.x) + (begin == 0)) * kUnitRows + tile * kTile + warp_row;
@@ -1393,7 +1413,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs& p, ChunkShared<D>&
             for (int j = 0; j < 32; ++j) y[j] *= by;
             if (nans) {
                 uint32_t found = 0;
-                const int from = max(max(u.first_seen, 0) / kTile, begin) * kTile, to = min(seen, end * kTile);
+                const int from = max(max(u.first_seen, 0) / kStep, begin) * kStep, to = min(seen, end * kStep);
                 for (int t = from; t < to; ++t) {
                     const int64_t block = ints(a.b.table)[u.s * a.b.table_pitch + t / a.c.block_size];
                     if (block < 0 || block >= a.c.blocks) continue;
@@ -1452,7 +1472,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
     extern __shared__ char raw[];
     auto& sh = *reinterpret_cast<ChunkShared<D>*>(raw + (1024 - shared_address(raw) % 1024) % 1024);
     const AttendArgs& a = p.a;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, seqs = a.b.seqs;
+    const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32, seqs = a.b.seqs;
     constexpr int kAll = kChunkThreads / 32;
     asm volatile("griddepcontrol.launch_dependents;");
     if (threadIdx.x == 0) p.parts.units[blockIdx.x].parts = 0;
@@ -1520,13 +1540,18 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             barrier_init(&sh.c.q_full[i], 4);
+            barrier_init(&sh.c.s_full[i][0], 1);
+            barrier_init(&sh.c.s_full[i][1], 1);
+            barrier_init(&sh.c.p_full[i][0], 4);
+            barrier_init(&sh.c.p_full[i][1], 4);
+            barrier_init(&sh.c.o_full[i][0], 1);
+            barrier_init(&sh.c.o_full[i][1], 1);
+        }
+        for (int i = 0; i < kStages; ++i) {
             barrier_init(&sh.c.k_full[i], kConvertWarps);
             barrier_init(&sh.c.v_full[i], kConvertWarps);
             barrier_init(&sh.c.k_empty[i], 1);
             barrier_init(&sh.c.v_empty[i], 1);
-            barrier_init(&sh.c.s_full[i], 1);
-            barrier_init(&sh.c.p_full[i], 4);
-            barrier_init(&sh.c.o_full[i], 1);
         }
         for (int i = 0; i < kLooked; ++i) {
             barrier_init(&sh.c.looked[i], 1);
@@ -1559,9 +1584,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
     } else {
         if (warp == kLookWarp) {
             look_role(p, sh.c, steps);
-        } else if (warp == kIssueWarp && lane == 0) {
+        } else if (warp == kIssueWarp) {
             issue_role<D>(sh);
-            commit(&sh.c.drained);
+            __syncwarp();
+            commit(&sh.c.drained, lane == 0);
             barrier_wait(&sh.c.drained, 0, sh.c, true);
         }
     }

@@ -34,6 +34,12 @@ struct Bf16 {
         const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
         return reinterpret_cast<const uint32_t&>(v);
     }
+    // The larger of a (not negative) and |b|, of each half.
+    static __device__ uint32_t max_size(uint32_t a, uint32_t b) {
+        uint32_t d;
+        asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b & 0x7FFF7FFFu));
+        return d;
+    }
 };
 
 struct Fp16 {
@@ -41,6 +47,11 @@ struct Fp16 {
     static __device__ uint32_t pack(float a, float b) {
         const __half2 v = __floats2half2_rn(a, b);
         return reinterpret_cast<const uint32_t&>(v);
+    }
+    static __device__ uint32_t max_size(uint32_t a, uint32_t b) {
+        uint32_t d;
+        asm("max.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b & 0x7FFF7FFFu));
+        return d;
     }
 };
 
