@@ -1026,6 +1026,14 @@ __device__ __forceinline__ void look_role(const ChunkArgs& p, ChunkControl& c, i
                                        w.end, w.left == w.end - w.begin, c.pos + steps - w.left};
                 barrier_arrive(&c.unit_looked[k]);
             }
+            // Its queries come to the L2 meanwhile.
+            for (int i = lane; i < w.u.rows; i += 32) {
+                const int r = w.u.first + i;
+                const char* at = a.query.at + int64_t(w.u.q.row + r / a.group) * a.query.token +
+                                 int64_t(w.u.head * a.group + r % a.group) * a.query.head;
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+                if (cache.head_dim > 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + 128));
+            }
         }
         const int n = min(kParts, w.end - w.step), step = w.step + part;
         const int64_t token = int64_t(step) * kStep + granule * kGranule;
@@ -1123,25 +1131,24 @@ __device__ __forceinline__ void convert_role(const ChunkArgs& p, ChunkShared<D>&
         fence_shared();
         __syncwarp();
     };
-    uint4 kr[kEach], vr[kEach];
-    if (!warp_wait(&sh.c.looked[0], 0, sh.c)) return;
-    load(kr, 0, 0);
-#pragma unroll 1
-    for (int64_t step = 0; step < steps; ++step) {
+    // One step, with the next one's loads on their way: true where there is a next one.
+    const auto turn = [&](uint4 (&kr)[kEach], uint4 (&vr)[kEach], uint4 (&k_next)[kEach], uint4 (&v_next)[kEach],
+                          int64_t step) {
         const int slot = step % kStages;
         const uint32_t free = uint32_t(step / kStages + 1) % 2;
         const Looked& look = sh.c.look[step % kLooked];
-        load(vr, step, c.side_pitch);
+        const bool more = step + 1 < steps;
         if (tid == 0) {
             sh.c.k_scale[step % kScales] = look.k_scale, sh.c.v_scale[step % kScales] = look.v_scale;
             sh.c.live[step % kScales] = look.live;
         }
-        if (!warp_wait(&sh.c.k_empty[slot], free, sh.c)) return;
+        if (!warp_wait(&sh.c.k_empty[slot], free, sh.c)) return false;
         convert(kr, sh.k[slot], look.k_by);
         if (lane == 0) barrier_arrive(&sh.c.k_full[slot]);
-        if (step + 1 < steps) {
-            if (!warp_wait(&sh.c.looked[(step + 1) % kLooked], uint32_t((step + 1) / kLooked) % 2, sh.c)) return;
-            load(kr, step + 1, 0);
+        if (more) {
+            if (!warp_wait(&sh.c.looked[(step + 1) % kLooked], uint32_t((step + 1) / kLooked) % 2, sh.c)) return false;
+            load(k_next, step + 1, 0);
+            load(v_next, step + 1, c.side_pitch);
         }
         if (look.edge) {
             // Some row does not see some of these tokens, and a weight of 0 times NaN is NaN: NaN
@@ -1160,13 +1167,22 @@ __device__ __forceinline__ void convert_role(const ChunkArgs& p, ChunkShared<D>&
             }
             if (found) sh.c.nan_unit[look.unit % kNanUnits] = look.unit + 1;
         }
-        if (!warp_wait(&sh.c.v_empty[slot], free, sh.c)) return;
+        if (!warp_wait(&sh.c.v_empty[slot], free, sh.c)) return false;
         convert(vr, sh.v[slot], look.v_by);
         if (lane == 0) {
             barrier_arrive(&sh.c.v_full[slot]);
             barrier_arrive(&sh.c.look_free[step % kLooked]);
         }
-    }
+        return more;
+    };
+    // Two steps' registers by turns: copies between them would wait for the loads.
+    uint4 ka[kEach], va[kEach], kb[kEach], vb[kEach];
+    if (!warp_wait(&sh.c.looked[0], 0, sh.c)) return;
+    load(ka, 0, 0);
+    load(va, 0, c.side_pitch);
+#pragma unroll 1
+    for (int64_t step = 0;; step += 2)
+        if (!turn(ka, va, kb, vb, step) || !turn(kb, vb, ka, va, step + 1)) return;
 }
 
 // The role of warp 12.
