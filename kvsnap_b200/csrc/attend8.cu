@@ -95,7 +95,7 @@ constexpr int kStepRows = 16;
 constexpr int kWarps = 16;                 // a CTA: HC heads x TS slices of a chunk
 constexpr int kGranule = 16;               // tokens a warp takes at a time
 constexpr float kLowest = -3e38f;          // the running maximum before any token
-constexpr float kSlack = 8.0f;             // log2 by which a weight may exceed 1 before sums are rescaled
+constexpr float kSlack = 14.0f;            // log2 by which a weight may exceed 1 before sums are rescaled (fp16: 2^16)
 
 struct StepArgs {
     AttendArgs a;
@@ -655,7 +655,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
 // Tensor memory holds exactly this: two tiles' sums (2 x 128 columns) and two steps of scores of each
 // (4 x 64). With one step of 128 tokens instead, scores and softmax took turns: 1.02 ms for an 8k
 // prompt of 32 heads.
-// The running maximum follows a row's true maximum only when that exceeds it by 2^8 (weights stay
+// The running maximum follows a row's true maximum only when that exceeds it by 2^14 (weights stay
 // within fp16), so sums in tensor memory are rarely touched. A page's scale goes into the conversion
 // relative to the largest key scale of the tile (which multiplies S) and the largest value scale so
 // far (which divides O at the end): powers of two, exact in fp16.
@@ -665,6 +665,9 @@ constexpr int kUnitRows = 2 * kTile;
 constexpr int kStep = 64;                  // tokens a step
 constexpr int kGranules = kStep / kGranule;
 constexpr int kStages = 4;                 // steps of keys and of values in shared memory
+// What a unit costs besides its steps (queries in, sums out, the pipeline's filling), in steps: work is
+// cut by steps and this, as a CTA with many short units was 1.6 times as long as others without it.
+constexpr int kUnitCost = 8;
 constexpr int kConvertWarps = 4, kIssueWarp = 12, kLookWarp = 13, kChunkThreads = 512;
 constexpr int kLooked = 16;                // steps looked up ahead
 constexpr int kScales = 8;                 // steps whose scales the softmax may still need
@@ -699,12 +702,12 @@ __device__ __forceinline__ int row_tiles(const AttendArgs& a, const Sequence& q)
     return (q.rows * a.group + kUnitRows - 1) / kUnitRows;
 }
 
-// Steps of one head of sequence s, summed by a warp.
-__device__ __forceinline__ int64_t head_steps(const AttendArgs& a, int s) {
+// Cost of one head of sequence s in steps, summed by a warp.
+__device__ __forceinline__ int64_t head_cost(const AttendArgs& a, int s) {
     Sequence q;
     if (!chunk_sequence(a, s, q)) return 0;
     int64_t n = 0;
-    for (int i = threadIdx.x % 32; i < row_tiles(a, q); i += 32) n += steps_of(a, q, i);
+    for (int i = threadIdx.x % 32; i < row_tiles(a, q); i += 32) n += kUnitCost + steps_of(a, q, i);
 #pragma unroll
     for (int k = 16; k; k >>= 1) n += __shfl_xor_sync(~0u, n, k);
     return n;
@@ -721,6 +724,7 @@ struct Looked {
     uint32_t live;                         // granules that are there
     int tokens;                            // of the step that the sequence has
     int edge;                              // some row does not see all of them
+    int last;                              // of the CTA
     int unit;
 };
 
@@ -729,7 +733,7 @@ struct LookedUnit {
     Sequence q;
     int s, head, first, rows, first_seen, steps, begin, end;
     int last;                              // of this CTA
-    int64_t pos;                           // its first step's place in all the work
+    int64_t stop;                          // where it ends in all the work
 };
 
 struct ChunkControl {
@@ -745,8 +749,8 @@ struct ChunkControl {
     uint32_t tensor;                       // tensor memory's address
     volatile int stop;                     // a wait ran out
     int64_t counts[kScanned], scratch[32];
-    int64_t total, ctas, pos, sought, scanned;
-    int s, head, tile, step;
+    int64_t total, ctas, pos, until, base, sought, scanned;      // pos to until: this CTA's part of the total cost
+    int s, head, tile;
 };
 
 template <int D>
@@ -757,42 +761,46 @@ struct ChunkShared {
     ChunkControl c;
 };
 
-// The look-up's way through the CTA's steps.
+// The look-up's way through the units that a CTA has steps of.
 struct Walk {
-    int64_t left;             // steps to go
-    int step, end;            // of the unit: [step, end) are this CTA's
-    int begin;                // where this CTA's part of the unit begins
+    int64_t base, stop;       // where the unit begins in all the work, and where the CTA's work ends, in cost
+    int begin, end;           // steps of the unit that are this CTA's
     int unit;                 // counted from 0
     Unit u;
 
-    __device__ __forceinline__ bool load(const AttendArgs& a) {
-        if (u.s >= a.b.seqs || !chunk_sequence(a, u.s, u.q)) return false;
+    // The unit that u names, from place `from` on; false without a step in it.
+    __device__ __forceinline__ bool load(const AttendArgs& a, int64_t from) {
         u.first = u.tile * kUnitRows;
         u.rows = min(u.q.rows * a.group - u.first, kUnitRows);
         u.first_seen = u.q.length - u.q.rows + u.first / a.group + 1;
         u.steps = steps_of(a, u.q, u.tile);
-        begin = step;
-        end = int(min(int64_t(u.steps), step + left));
+        begin = int(max(int64_t(0), from - base - kUnitCost));
+        end = int(min(int64_t(u.steps), stop - base - kUnitCost));
+        return end > begin;
+    }
+    __device__ __forceinline__ bool next(const AttendArgs& a) {
+        do {
+            base += kUnitCost + u.steps;
+            if (base >= stop) return false;
+            if (++u.tile >= row_tiles(a, u.q)) {
+                u.tile = 0;
+                if (++u.head == a.c.kv_heads) {
+                    u.head = 0;
+                    for (++u.s; u.s < a.b.seqs && !chunk_sequence(a, u.s, u.q); ++u.s) {}
+                    if (u.s >= a.b.seqs) return false;
+                }
+            }
+        } while (!load(a, base));
+        ++unit;
         return true;
     }
-    __device__ __forceinline__ bool start(const AttendArgs& a, const ChunkControl& c, int64_t steps) {
-        left = steps, unit = 0;
-        u.s = c.s, u.head = c.head, u.tile = c.tile, step = c.step;
-        return left > 0 && load(a);
-    }
-    // To the next unit, after the steps [begin, end) of this one.
-    __device__ __forceinline__ bool next(const AttendArgs& a) {
-        left -= end - begin;
-        if (left <= 0) return false;
-        step = 0, ++unit;
-        if (++u.tile >= row_tiles(a, u.q)) {
-            u.tile = 0;
-            if (++u.head == a.c.kv_heads) {
-                u.head = 0;
-                for (++u.s; u.s < a.b.seqs && !chunk_sequence(a, u.s, u.q); ++u.s) {}
-            }
-        }
-        return load(a);
+    __device__ __forceinline__ bool start(const AttendArgs& a, const ChunkControl& c) {
+        base = c.base, stop = c.until, unit = -1;
+        u.s = c.s, u.head = c.head, u.tile = c.tile;
+        if (!chunk_sequence(a, u.s, u.q)) return false;
+        if (!load(a, c.pos)) return next(a);
+        unit = 0;
+        return true;
     }
 };
 
@@ -1007,92 +1015,80 @@ __device__ __forceinline__ uint32_t times_half2(uint32_t a, uint32_t b) {
 }
 
 // The role of warp 13: 8 steps at a time, a lane a granule.
-__device__ __forceinline__ void look_role(const ChunkArgs& p, ChunkControl& c, int64_t steps) {
+__device__ __forceinline__ void look_role(const ChunkArgs& p, ChunkControl& c, Walk w) {
+    constexpr int kParts = 32 / kGranules;
     const AttendArgs& a = p.a;
     const Cache& cache = a.c;
     const int lane = threadIdx.x % 32, part = lane / kGranules, granule = lane % kGranules;
-    constexpr int kParts = 32 / kGranules;
-    Walk w;
-    if (!w.start(a, c, steps)) return;
-    float v_carry = 0.0f;
-    bool fresh = true;
     for (int64_t it = 0;;) {
-        if (fresh) {
-            fresh = false;
-            const int k = w.unit % kLookedUnits;
-            if (!warp_wait(&c.unit_free[k], uint32_t(w.unit / kLookedUnits + 1) % 2, c)) return;
-            if (lane == 0) {
-                c.unit[k] = LookedUnit{w.u.q, w.u.s, w.u.head, w.u.first, w.u.rows, w.u.first_seen, w.u.steps, w.begin,
-                                       w.end, w.left == w.end - w.begin, c.pos + steps - w.left};
-                barrier_arrive(&c.unit_looked[k]);
-            }
-            // Its queries come to the L2 meanwhile.
-            for (int i = lane; i < w.u.rows; i += 32) {
-                const int r = w.u.first + i;
-                const char* at = a.query.at + int64_t(w.u.q.row + r / a.group) * a.query.token +
-                                 int64_t(w.u.head * a.group + r % a.group) * a.query.head;
-                asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
-                if (cache.head_dim > 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + 128));
-            }
+        Walk after = w;
+        const bool more = after.next(a);
+        const int k = w.unit % kLookedUnits;
+        if (!warp_wait(&c.unit_free[k], uint32_t(w.unit / kLookedUnits + 1) % 2, c)) return;
+        if (lane == 0) {
+            c.unit[k] = LookedUnit{w.u.q, w.u.s, w.u.head, w.u.first, w.u.rows, w.u.first_seen, w.u.steps, w.begin,
+                                   w.end, !more, w.base + kUnitCost + w.u.steps};
+            barrier_arrive(&c.unit_looked[k]);
         }
-        const int n = min(kParts, w.end - w.step), step = w.step + part;
-        const int64_t token = int64_t(step) * kStep + granule * kGranule;
-        int64_t at = 0;
-        float ks = 0.0f, vs = 0.0f;
-        if (part < n && token < w.u.q.length) {
-            const int64_t block = ints(a.b.table)[w.u.s * a.b.table_pitch + token / cache.block_size];
-            if (block < 0 || block >= cache.blocks) {
-                atomicOr(a.status, KVSNAP_DP_BAD_BLOCK);
-            } else {
-                at = cache.codes + block * cache.block_pitch + token % cache.block_size * cache.token_pitch +
-                     w.u.head * cache.head_pitch;
-                const float* scales = reinterpret_cast<const float*>(cache.scales) + block * 2 * cache.kv_heads + w.u.head;
-                ks = scales[0], vs = scales[cache.kv_heads];
-            }
+        // Its queries come to the L2 meanwhile.
+        for (int i = lane; i < w.u.rows; i += 32) {
+            const int r = w.u.first + i;
+            const char* at = a.query.at + int64_t(w.u.q.row + r / a.group) * a.query.token +
+                             int64_t(w.u.head * a.group + r % a.group) * a.query.head;
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+            if (cache.head_dim > 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + 128));
         }
-        const uint32_t live = __ballot_sync(~0u, at != 0) >> (kGranules * part) & ((1u << kGranules) - 1);
-        float k_top = ks, v_top = vs;
+        float v_top = 0.0f;
+        for (int first = w.begin; first < w.end; first += kParts) {
+            const int n = min(kParts, w.end - first), step = first + part;
+            const int64_t token = int64_t(step) * kStep + granule * kGranule;
+            int64_t at = 0;
+            float ks = 0.0f, vs = 0.0f;
+            if (part < n && token < w.u.q.length) {
+                const int64_t block = ints(a.b.table)[w.u.s * a.b.table_pitch + token / cache.block_size];
+                if (block < 0 || block >= cache.blocks) {
+                    atomicOr(a.status, KVSNAP_DP_BAD_BLOCK);
+                } else {
+                    at = cache.codes + block * cache.block_pitch + token % cache.block_size * cache.token_pitch +
+                         w.u.head * cache.head_pitch;
+                    const float* scales = reinterpret_cast<const float*>(cache.scales) + block * 2 * cache.kv_heads + w.u.head;
+                    ks = scales[0], vs = scales[cache.kv_heads];
+                }
+            }
+            const uint32_t live = __ballot_sync(~0u, at != 0) >> (kGranules * part) & ((1u << kGranules) - 1);
+            float k_top = ks;
 #pragma unroll
-        for (int k = kGranules / 2; k; k >>= 1) {
-            k_top = fmaxf(k_top, __shfl_xor_sync(~0u, k_top, k));
-            v_top = fmaxf(v_top, __shfl_xor_sync(~0u, v_top, k));
-        }
-#pragma unroll
-        for (int k = kGranules; k < 32; k <<= 1) {
-            const float up = __shfl_up_sync(~0u, v_top, k);
-            if (lane >= k) v_top = fmaxf(v_top, up);
-        }
-        v_top = fmaxf(v_top, v_carry);
-        v_carry = __shfl_sync(~0u, v_top, kGranules * (n - 1));
-        const __half2 k_by = __float2half2_rn(k_top > 0.0f ? ks / k_top : 0.0f);
-        const __half2 v_by = __float2half2_rn(v_top > 0.0f ? vs / v_top : 0.0f);
-        for (int i = 0; i < n; ++i)
-            if (!warp_wait(&c.look_free[(it + i) % kLooked], uint32_t((it + i) / kLooked + 1) % 2, c)) return;
-        if (part < n) {
-            Looked& to = c.look[(it + part) % kLooked];
-            to.keys[granule] = at;
-            to.k_by[granule] = reinterpret_cast<const uint32_t&>(k_by);
-            to.v_by[granule] = reinterpret_cast<const uint32_t&>(v_by);
-            if (granule == 0) {
-                to.k_scale = k_top, to.v_scale = v_top, to.live = live;
-                to.tokens = int(min(int64_t(kStep), max(int64_t(0), w.u.q.length - token)));
-                to.edge = int64_t(step + 1) * kStep > w.u.first_seen;
-                to.unit = w.unit;
+            for (int i = kGranules / 2; i; i >>= 1) k_top = fmaxf(k_top, __shfl_xor_sync(~0u, k_top, i));
+            v_top = fmaxf(v_top, warp_max(vs));        // of all these steps: it changes once in 8 at most
+            const __half2 k_by = __float2half2_rn(k_top > 0.0f ? ks / k_top : 0.0f);
+            const __half2 v_by = __float2half2_rn(v_top > 0.0f ? vs / v_top : 0.0f);
+            for (int i = 0; i < n; ++i)
+                if (!warp_wait(&c.look_free[(it + i) % kLooked], uint32_t((it + i) / kLooked + 1) % 2, c)) return;
+            if (part < n) {
+                Looked& to = c.look[(it + part) % kLooked];
+                to.keys[granule] = at;
+                to.k_by[granule] = reinterpret_cast<const uint32_t&>(k_by);
+                to.v_by[granule] = reinterpret_cast<const uint32_t&>(v_by);
+                if (granule == 0) {
+                    to.k_scale = k_top, to.v_scale = v_top, to.live = live;
+                    to.tokens = int(min(int64_t(kStep), max(int64_t(0), w.u.q.length - token)));
+                    to.edge = int64_t(step + 1) * kStep > w.u.first_seen;
+                    to.last = !more && step + 1 == w.end;
+                    to.unit = w.unit;
+                }
             }
+            __syncwarp();
+            if (lane < n) barrier_arrive(&c.looked[(it + lane) % kLooked]);
+            it += n;
         }
-        __syncwarp();
-        if (lane < n) barrier_arrive(&c.looked[(it + lane) % kLooked]);
-        it += n, w.step += n;
-        if (w.step == w.end) {
-            if (!w.next(a)) return;
-            v_carry = 0.0f, fresh = true;
-        }
+        if (!more) return;
+        w = after;
     }
 }
 
 // The role of warps 8-11.
 template <int D>
-__device__ __forceinline__ void convert_role(const ChunkArgs& p, ChunkShared<D>& sh, int64_t steps) {
+__device__ __forceinline__ void convert_role(const ChunkArgs& p, ChunkShared<D>& sh) {
     constexpr int kAcross = D / 16, kTokens = 32 * kConvertWarps / kAcross, kEach = kStep / kTokens;
     const Cache& c = p.a.c;
     const int tid = threadIdx.x - 256, lane = threadIdx.x % 32;
@@ -1137,7 +1133,7 @@ __device__ __forceinline__ void convert_role(const ChunkArgs& p, ChunkShared<D>&
         const int slot = step % kStages;
         const uint32_t free = uint32_t(step / kStages + 1) % 2;
         const Looked& look = sh.c.look[step % kLooked];
-        const bool more = step + 1 < steps;
+        const bool more = !look.last;
         if (tid == 0) {
             sh.c.k_scale[step % kScales] = look.k_scale, sh.c.v_scale[step % kScales] = look.v_scale;
             sh.c.live[step % kScales] = look.live;
@@ -1471,7 +1467,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs& p, ChunkShared<D>&
         if (!whole) {
             if (lane < rows) p.parts.ml[slot + lane] = make_float2(m, l);
             if (begin == 0 && threadIdx.x == 0) {
-                const int last = int(((u.pos + u.steps) * sh.c.ctas - 1) / sh.c.total);
+                const int last = int((u.stop * sh.c.ctas - 1) / sh.c.total);
                 p.parts.units[blockIdx.x] =
                     SharedUnit{u.q.row, u.head, u.first, u.rows, last - int(blockIdx.x) + 1};
             }
@@ -1493,9 +1489,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
     asm volatile("griddepcontrol.launch_dependents;");
     if (threadIdx.x == 0) p.parts.units[blockIdx.x].parts = 0;
 
-    // All steps (of every sequence, head and row tile, end to end), and where this CTA's begin.
+    // All the work (of every sequence, head and row tile, end to end), and where this CTA's begins.
     int64_t mine = 0;
-    for (int s = warp; s < seqs; s += kAll) mine += head_steps(a, s);
+    for (int s = warp; s < seqs; s += kAll) mine += head_cost(a, s);
     if (lane == 0) sh.c.scratch[warp] = mine;
     __syncthreads();
     int64_t total = 0;
@@ -1507,7 +1503,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
     int64_t before = 0;
     for (int base = 0; base < seqs; base += kScanned) {
         for (int s = warp; s < kScanned; s += kAll) {
-            const int64_t n = base + s < seqs ? head_steps(a, base + s) : 0;
+            const int64_t n = base + s < seqs ? head_cost(a, base + s) : 0;
             if (lane == 0) sh.c.counts[s] = n;
         }
         __syncthreads();
@@ -1539,7 +1535,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
         chunk_sequence(a, sh.c.s, q);
         int64_t done = 0;
         for (int i = 0; i < row_tiles(a, q); i += 32) {
-            const int n = i + lane < row_tiles(a, q) ? steps_of(a, q, i + lane) : 0;
+            const int n = i + lane < row_tiles(a, q) ? kUnitCost + steps_of(a, q, i + lane) : 0;
             int64_t sum = n;
 #pragma unroll
             for (int k = 1; k < 32; k <<= 1) {
@@ -1548,7 +1544,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
             }
             const int64_t first = done + sum - n;
             if (n && first <= sh.c.sought && sh.c.sought < done + sum)
-                sh.c.tile = i + lane, sh.c.step = int(sh.c.sought - first);
+                sh.c.tile = i + lane, sh.c.base = pos - (sh.c.sought - first);
             done += __shfl_sync(~0u, sum, 31);
         }
     }
@@ -1578,7 +1574,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
             barrier_init(&sh.c.unit_free[i], 9);         // 8 warps of rows, and the issue
         }
         barrier_init(&sh.c.drained, 1);
-        sh.c.total = total, sh.c.ctas = ctas, sh.c.pos = pos;
+        sh.c.total = total, sh.c.ctas = ctas, sh.c.pos = pos, sh.c.until = end;
         for (int i = 0; i < kNanUnits; ++i) sh.c.nan_unit[i] = 0;
         sh.c.stop = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -1592,14 +1588,17 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
     __syncthreads();
     fence_after();
 
-    const int64_t steps = end - pos;
-    if (warp < 8) {
+    // A part of the work may hold no step: then no role has anything to do.
+    Walk w;
+    const bool any = w.start(a, sh.c);
+    if (!any) {
+    } else if (warp < 8) {
         softmax_role<T, D>(p, sh);
     } else if (warp < 8 + kConvertWarps) {
-        convert_role<D>(p, sh, steps);
+        convert_role<D>(p, sh);
     } else {
         if (warp == kLookWarp) {
-            look_role(p, sh.c, steps);
+            look_role(p, sh.c, w);
         } else if (warp == kIssueWarp) {
             issue_role<D>(sh);
             __syncwarp();
