@@ -76,24 +76,29 @@ struct Parts {
     float2* ml;               // their maxima and weights' sums
     SharedUnit* units;        // a CTA's unit that it begins and others go on with
     int heads, head_rows;     // slot rows: heads x rows a head
+    int used_rows;            // that a head can have in this call
 };
 
 // ---- few rows: decode -------------------------------------------------------------------
 //
 // Sequences with at most kStepRows rows a KV head (query heads of the group times
 // new tokens). Bound by the cache's bytes, so nothing but a page's codes is read,
-// once, straight into the registers of the lanes whose matrix fragments they are:
-// with the keys as the 16-row operand of m16n8k16, lane (g, t) needs 16 bytes of
-// tokens' rows g, and with the values' transpose, 16 dims of 4 tokens. Which token
+// once, by the lanes whose matrix fragments they are: with the keys as the 16-row
+// operand of m16n8k16, lane (g, t) needs 16 bytes of tokens' rows g, and with the
+// values' transpose, 16 dims of 4 tokens. Which token
 // is row g and which dim is row g of the transpose is free as long as both
 // products agree, so it is chosen to make every load a 16-byte one and every pair
 // of codes that a fragment register holds adjacent after one byte permute. The
 // scores come out transposed, [token][row], and one 8x8 transpose in registers
-// makes them the weights' fragment.
+// makes them the weights' fragment. Each lane copies its own bytes to shared memory
+// asynchronously, kAhead granules ahead, and reads back only those: no warp waits
+// for another, and 128 KB an SM are on their way at a time (loads to registers, a
+// granule ahead, kept 64 KB and reached 4.1 TB/s where this reaches 5.3).
 
 constexpr int kStepRows = 16;
 constexpr int kWarps = 16;                 // a CTA: HC heads x TS slices of a chunk
 constexpr int kGranule = 16;               // tokens a warp takes at a time
+constexpr int kAhead = 3;                  // granules a warp holds: one in use, the others on their way
 constexpr float kLowest = -3e38f;          // the running maximum before any token
 constexpr float kSlack = 14.0f;            // log2 by which a weight may exceed 1 before sums are rescaled (fp16: 2^16)
 
@@ -116,7 +121,7 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     return d;
 }
 
-// 16 (8) bytes of a cache that are read once, or zeros. Predicated, not branched around: where a branch
+// 16 bytes of a cache that are read once, or zeros. Predicated, not branched around: where a branch
 // around a load joins, the load is waited for.
 __device__ __forceinline__ uint4 load16(const char* at, bool there) {
     uint4 v;
@@ -126,11 +131,23 @@ __device__ __forceinline__ uint4 load16(const char* at, bool there) {
     return v;
 }
 
-__device__ __forceinline__ uint2 load8bytes(const char* at, bool there) {
-    uint2 v;
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %3, 0;\nmov.u32 %0, 0;\nmov.u32 %1, 0;\n"
-                 "@p ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];\n}"
-                 : "=&r"(v.x), "=&r"(v.y) : "l"(at), "r"(uint32_t(there)));
+// N bytes to shared memory, or zeros, on their way until copies_done.
+template <int N>
+__device__ __forceinline__ void copy_async(uint32_t to, const char* from, bool there) {
+    if constexpr (N == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(there ? 8 : 0) : "memory");
+}
+
+// All of the thread's copies but its last n groups.
+template <int N>
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void copies_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
+__device__ __forceinline__ uint4 read_shared(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
     return v;
 }
 
@@ -155,12 +172,14 @@ __device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* scratch) {
 template <typename T, int D, int NT>
 struct StepWarp {
     static constexpr int kHalves = D / 64, kTiles = D / 16;
+    static constexpr uint32_t kGranuleBytes = 512 * (2 * kHalves + 4);
     float o[NT][kTiles][4];                // (dim pair, row) sums, relative to m and vref
     float m[NT][2], l[NT][2];              // of rows 8 nt + 2 t, + 1
     float vref;                            // largest value scale so far
 
+    // `ring`: the warp's kAhead granules of shared memory, 16 bytes a lane and piece.
     __device__ __forceinline__ void run(const StepArgs& p, const Sequence& q, int s, int head, int slice, int c0,
-                                        int c1) {
+                                        int c1, uint32_t ring) {
         const int lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
         const Cache& c = p.a.c;
         const int rows = q.rows * p.a.group, first_seen = q.length - q.rows + 1;
@@ -228,54 +247,58 @@ struct StepWarp {
         const char* v_lane = keys + c.side_pitch + 4 * t * c.token_pitch + (D / 8) * g;
         const int64_t two_tokens = 2 * c.token_pitch;
 
-        uint4 kr[kHalves][2], vr[4];
-        const auto load_keys = [&](int64_t off) {
+        ring += lane * 16;
+        // Pages of 32 chunks at a time, one a lane: where the warp's granule lies, and its scales, now and of
+        // the 32 before, as copies run ahead of the products. A page that is not there has a negative scale.
+        int64_t off = -1;
+        float ks = 0.0f, vs = 0.0f, ks_before = 0.0f, vs_before = 0.0f;
+        int window = -1;
+        const auto copy = [&](int chunk) {
+            const int j = chunk - c0;
+            if (j / 32 != window) {
+                window = j / 32;
+                ks_before = ks, vs_before = vs;
+                const int64_t token = (int64_t(chunk + lane) * p.ts + slice) * kGranule;
+                off = -1, ks = 0.0f, vs = -1.0f;
+                if (chunk + lane < c1 && token < q.length) {
+                    const int64_t block = ints(p.a.b.table)[s * p.a.b.table_pitch + token / c.block_size];
+                    if (block < 0 || block >= c.blocks) {
+                        atomicOr(p.a.status, KVSNAP_DP_BAD_BLOCK);
+                    } else {
+                        off = block * c.block_pitch + token % c.block_size * c.token_pitch;
+                        const float* scales = reinterpret_cast<const float*>(c.scales) + block * 2 * c.kv_heads + head;
+                        ks = scales[0], vs = scales[c.kv_heads];
+                    }
+                }
+            }
+            const int64_t found = __shfl_sync(~0u, off, j % 32), at = max(found, int64_t(0));
+            const bool there = found >= 0;
+            const uint32_t to = ring + j % kAhead * kGranuleBytes;
 #pragma unroll
             for (int half = 0; half < kHalves; ++half)
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                    kr[half][i] = load16(k_lane + off + i * two_tokens + 64 * half, off >= 0);
-        };
-        const auto load_values = [&](int64_t off) {
+                    copy_async<16>(to + (half * 2 + i) * 512, k_lane + at + i * two_tokens + 64 * half, there);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if constexpr (D == 128) {
-                    vr[j] = load16(v_lane + off + j * c.token_pitch, off >= 0);
-                } else {
-                    const uint2 x = load8bytes(v_lane + off + j * c.token_pitch, off >= 0);
-                    vr[j] = make_uint4(x.x, x.y, 0, 0);
-                }
-            }
+            for (int i = 0; i < 4; ++i)
+                copy_async<D / 8>(to + (kHalves * 2 + i) * 512, v_lane + at + i * c.token_pitch, there);
         };
 
-        // Pages of 32 chunks at a time, one a lane: where the warp's granule lies, and its scales.
-        int64_t off = -1;
-        float ks = 0.0f, vs = 0.0f;
-        const auto look_up = [&](int chunk) {
-            const int64_t token = (int64_t(chunk + lane) * p.ts + slice) * kGranule;
-            off = -1, ks = vs = 0.0f;
-            if (chunk + lane < c1 && token < q.length) {
-                const int64_t block = ints(p.a.b.table)[s * p.a.b.table_pitch + token / c.block_size];
-                if (block < 0 || block >= c.blocks) {
-                    atomicOr(p.a.status, KVSNAP_DP_BAD_BLOCK);
-                } else {
-                    off = block * c.block_pitch + token % c.block_size * c.token_pitch;
-                    const float* scales = reinterpret_cast<const float*>(c.scales) + block * 2 * c.kv_heads + head;
-                    ks = scales[0], vs = scales[c.kv_heads];
-                }
-            }
-        };
-
-        look_up(c0);
-        int64_t now = __shfl_sync(~0u, off, 0);
-        load_keys(now);
-        load_values(now);
+#pragma unroll
+        for (int i = 0; i < kAhead - 1; ++i) {
+            if (c0 + i < c1) copy(c0 + i);
+            copies_group();
+        }
         for (int chunk = c0; chunk < c1; ++chunk) {
-            const int j = (chunk - c0) % 32;
-            const float k_scale = __shfl_sync(~0u, ks, j), v_scale = __shfl_sync(~0u, vs, j);
-            const bool dead = now < 0;
-            if (j == 31) look_up(chunk + 1);
-            const int64_t next = __shfl_sync(~0u, off, (j + 1) % 32);
+            const int j = chunk - c0;
+            if (chunk + kAhead - 1 < c1) copy(chunk + kAhead - 1);
+            copies_group();
+            copies_done<kAhead - 1>();
+            const uint32_t at = ring + j % kAhead * kGranuleBytes;
+            const bool old = j / 32 != window;
+            const float k_scale = __shfl_sync(~0u, old ? ks_before : ks, j % 32);
+            const float v_scale = __shfl_sync(~0u, old ? vs_before : vs, j % 32);
+            const bool dead = v_scale < 0.0f;
             const int64_t base = (int64_t(chunk) * p.ts + slice) * kGranule;
 
             float sc[NT][4];
@@ -283,8 +306,8 @@ struct StepWarp {
             for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.0f;
 #pragma unroll
             for (int half = 0; half < kHalves; ++half) {
-                const uint32_t wa[4] = {kr[half][0].x, kr[half][0].y, kr[half][0].z, kr[half][0].w};
-                const uint32_t wb[4] = {kr[half][1].x, kr[half][1].y, kr[half][1].z, kr[half][1].w};
+                const uint4 ka = read_shared(at + half * 1024), kb = read_shared(at + half * 1024 + 512);
+                const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
                     const uint32_t a0 = half2_of_codes(uint16_t(wa[w])), a2 = half2_of_codes(uint16_t(wa[w] >> 16));
@@ -294,8 +317,6 @@ struct StepWarp {
                         mma16816(sc[nt], a0, a1, a2, a3, qb[nt][half * 4 + w][0], qb[nt][half * 4 + w][1]);
                 }
             }
-            load_keys(next);
-
             // Edge: tokens that some row does not see, or a page that is not there.
             const bool edge = dead || base + kGranule > first_seen;
             bool grow = false;
@@ -351,6 +372,9 @@ struct StepWarp {
                 pb[nt][1] = transpose8x8(pack_half2(w[2] * part, w[3] * part));
             }
 
+            uint4 vr[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) vr[i] = read_shared(at + (kHalves * 2 + i) * 512);
             const auto add_values = [&](const uint4 (&v)[4], const uint32_t (&b)[NT][2]) {
                 const uint32_t w[4][4] = {{v[0].x, v[0].y, v[0].z, v[0].w}, {v[1].x, v[1].y, v[1].z, v[1].w},
                                           {v[2].x, v[2].y, v[2].z, v[2].w}, {v[3].x, v[3].y, v[3].z, v[3].w}};
@@ -384,9 +408,8 @@ struct StepWarp {
                     add_values(v, b);
                 }
             }
-            load_values(next);
-            now = next;
         }
+        copies_done<0>();
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -401,7 +424,10 @@ struct StepWarp {
 template <int D, int NT>
 struct StepShared {
     static constexpr int kPitch = D + 4;
-    float o[kWarps][8 * NT][kPitch];
+    union {
+        float o[kWarps][8 * NT][kPitch];   // once the granules are done with
+        char ring[kWarps][kAhead * 512 * (2 * (D / 64) + 4)];
+    };
     float2 ml[kWarps][8 * NT];
     int64_t scratch[kWarps];
     int64_t prefix[kWarps];
@@ -476,10 +502,13 @@ __global__ void __launch_bounds__(32 * kWarps, 1) step_kernel(const __grid_const
         }
         const int c1 = SPLIT ? int(min(int64_t(chunks), c0 + (end - pos))) : chunks;
         const int rows = q.rows * p.a.group;
-        const int hc = warp % p.hc, slice = warp / p.hc;
+        const int hc = warp % p.hc, slice = warp / p.hc;       // a warp without a slice only waits
+        StepWarp<T, D, NT> w;
         if (slice < p.ts) {
-            StepWarp<T, D, NT> w;
-            w.run(p, q, s, hg * p.hc + hc, slice, c0, c1);
+            w.run(p, q, s, hg * p.hc + hc, slice, c0, c1, uint32_t(__cvta_generic_to_shared(sh.ring[warp])));
+        }
+        __syncthreads();
+        if (slice < p.ts) {
             const int g = lane / 4, t = lane % 4;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -539,23 +568,26 @@ __global__ void __launch_bounds__(32 * kWarps, 1) step_kernel(const __grid_const
 }
 
 // Joins the parts of shared units, which lie in consecutive CTAs' slots. A warp a row where there are
-// few parts, else a CTA a row.
+// few parts, else a CTA a row, its warps a share of the parts each.
 constexpr int kJoinWarps = 8;
+constexpr int kJoinCtas = 6;               // an SM
 constexpr int kMostCtas = 512;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_constant__ AttendArgs a,
                                                                const __grid_constant__ Parts p, int ctas) {
     constexpr int kEach = D / 32;
+    using Piece = std::conditional_t<kEach == 4, float4, float2>;
     __shared__ SharedUnit units[kMostCtas];
     __shared__ int owner[kMostCtas];
     __shared__ int count, most;
     __shared__ float sums[kJoinWarps][D];
-    __shared__ float weight[kMostCtas], stat[kJoinWarps];
+    __shared__ float weight[kMostCtas], stat[2][kJoinWarps];
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (warp == 0) {
         int n = 0, parts = 0;
+#pragma unroll 5
         for (int i = lane; i < (ctas + 31) / 32 * 32; i += 32) {
             SharedUnit u{};
             if (i < ctas) u = p.units[i];
@@ -574,20 +606,23 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
     const bool alone = most <= 8;                                  // a warp a row
     const int first = alone ? blockIdx.x * kJoinWarps + warp : blockIdx.x;
     const int step = alone ? gridDim.x * kJoinWarps : gridDim.x;
-    const int slot_rows = p.heads * p.head_rows;
-    for (int task = first; task < count * slot_rows; task += step) {
-        const int k = task / slot_rows, in = task % slot_rows, h = in / p.head_rows, row = in % p.head_rows;
+    const int slot_rows = p.heads * p.head_rows, used = p.heads * p.used_rows;
+    for (int task = first; task < count * used; task += step) {
+        const int k = task / used, h = task % used / p.used_rows, row = task % p.used_rows;
         const SharedUnit u = units[k];
         if (row >= u.rows) continue;
+        const int in = h * p.head_rows + row;
         const auto at = [&](int f) { return int64_t(2 * (owner[k] + f) + (f == 0)) * slot_rows + in; };
+        const auto part = [&](int f) { return *reinterpret_cast<const Piece*>(p.sums + at(f) * D + lane * kEach); };
         float o[kEach] = {}, sum = 0.0f;
-        const auto add = [&](int f, float by) {
-            const float* from = p.sums + at(f) * D + lane * kEach;
+        const auto add = [&](const Piece& v, float by) {
+            const float* x = reinterpret_cast<const float*>(&v);
 #pragma unroll
-            for (int i = 0; i < kEach; ++i) o[i] += by * from[i];
+            for (int i = 0; i < kEach; ++i) o[i] += by * x[i];
         };
         if (alone) {
             const float2 ml = lane < u.parts ? p.ml[at(lane)] : make_float2(kLowest, 0.0f);
+            const Piece x = part(0), y = u.parts > 1 ? part(1) : Piece{};
             float top = ml.x;
 #pragma unroll
             for (int i = 4; i; i >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, i));
@@ -597,37 +632,50 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
 #pragma unroll
             for (int i = 4; i; i >>= 1) sum += __shfl_xor_sync(~0u, sum, i);
             sum = __shfl_sync(~0u, sum, 0);
-            for (int i = 0; i < u.parts; ++i) add(i, __shfl_sync(~0u, f, i));
+            add(x, __shfl_sync(~0u, f, 0));
+            add(y, __shfl_sync(~0u, f, 1));
+            for (int i = 2; i < u.parts; ++i) add(part(i), __shfl_sync(~0u, f, i));
         } else {
             float top = kLowest;
-            for (int i = threadIdx.x; i < u.parts; i += blockDim.x) top = fmaxf(top, p.ml[at(i)].x);
-            top = warp_max(top);
-            if (lane == 0) stat[warp] = top;
-            __syncthreads();
-            top = stat[0];
-            for (int w = 1; w < kJoinWarps; ++w) top = fmaxf(top, stat[w]);
-            __syncthreads();
             for (int i = threadIdx.x; i < u.parts; i += blockDim.x) {
                 const float2 ml = p.ml[at(i)];
-                const float f = exp2_fast(ml.x - top);
-                weight[i] = f;
-                sum += f * ml.y;
+                weight[i] = ml.x;
+                top = fmaxf(top, ml.x);
             }
+            top = warp_max(top);
+            if (lane == 0) stat[0][warp] = top;
+            __syncthreads();
+            top = stat[0][0];
+            for (int w = 1; w < kJoinWarps; ++w) top = fmaxf(top, stat[0][w]);
+            // Each warp its share of the parts, 8 on their way at a time.
+            for (int i = warp; i < u.parts; i += 8 * kJoinWarps) {
+                Piece v[8];
+                float by[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int f = i + j * kJoinWarps;
+                    v[j] = Piece{}, by[j] = 0.0f;
+                    if (f < u.parts) v[j] = part(f), by[j] = exp2_fast(weight[f] - top);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) add(v[j], by[j]);
+            }
+            for (int i = threadIdx.x; i < u.parts; i += blockDim.x)
+                sum += exp2_fast(weight[i] - top) * p.ml[at(i)].y;
 #pragma unroll
             for (int i = 16; i; i >>= 1) sum += __shfl_xor_sync(~0u, sum, i);
-            if (lane == 0) stat[warp] = sum;
-            __syncthreads();
-            sum = 0.0f;
-            for (int w = 0; w < kJoinWarps; ++w) sum += stat[w];
-#pragma unroll 4
-            for (int i = warp; i < u.parts; i += kJoinWarps) add(i, weight[i]);
+            if (lane == 0) stat[1][warp] = sum;
 #pragma unroll
             for (int i = 0; i < kEach; ++i) sums[warp][lane * kEach + i] = o[i];
             __syncthreads();
+            if (warp == 0) {
+                sum = 0.0f;
+                for (int w = 0; w < kJoinWarps; ++w) sum += stat[1][w];
 #pragma unroll
-            for (int i = 0; i < kEach; ++i) {
-                o[i] = 0.0f;
-                for (int w = 0; w < kJoinWarps; ++w) o[i] += sums[w][lane * kEach + i];
+                for (int i = 0; i < kEach; ++i) {
+                    o[i] = 0.0f;
+                    for (int w = 0; w < kJoinWarps; ++w) o[i] += sums[w][lane * kEach + i];
+                }
             }
             __syncthreads();
             if (warp) continue;
@@ -1623,6 +1671,7 @@ struct Plan {
     bool stepped, chunked;    // whether each kernel runs
     bool split, wide;         // the step kernel's units are cut; more than 8 rows a head
     int step_rows;
+    int most_rows;            // that a KV head of a sequence can have
     int64_t ctas, step_ctas;
     int64_t slots, sum_bytes, bytes;
 };
@@ -1640,6 +1689,7 @@ Plan plan_for(const Cache& c, const Batch& b, int q_heads, int sms) {
     const int group = q_heads / c.kv_heads;
     const int64_t most_rows = int64_t(group) * (b.max_query < b.rows ? b.max_query : b.rows);
     plan.chunked = most_rows > kStepRows;
+    plan.most_rows = int(most_rows);
     // With one sequence, the kernel for many rows takes it whatever it holds: one launch, not two.
     plan.stepped = group <= kStepRows && !(plan.chunked && b.seqs == 1);
     plan.step_rows = plan.stepped ? kStepRows : 0;
@@ -1698,18 +1748,18 @@ void launch_step(const Plan& plan, const StepArgs& p, cudaStream_t stream) {
 template <typename T, int D>
 void launch_attend(const Plan& plan, const AttendArgs& a, Parts parts, cudaStream_t stream) {
     const auto join = [&] {
-        launch(join_kernel<T, D>, plan.ctas, 32 * kJoinWarps, 0, stream, true, a, parts, int(plan.ctas));
+        launch(join_kernel<T, D>, plan.ctas * kJoinCtas, 32 * kJoinWarps, 0, stream, true, a, parts, int(plan.ctas));
     };
     if (plan.stepped) {
         StepArgs p = plan.step;
-        parts.heads = p.hc, parts.head_rows = kStepRows;
+        parts.heads = p.hc, parts.head_rows = kStepRows, parts.used_rows = plan.wide ? kStepRows : plan.most_rows;
         p.a = a, p.parts = parts;
         if (plan.wide) launch_step<T, D, 2>(plan, p, stream);
         else launch_step<T, D, 1>(plan, p, stream);
         if (plan.split) join();
     }
     if (plan.chunked) {
-        parts.heads = 1, parts.head_rows = kUnitRows;
+        parts.heads = 1, parts.head_rows = kUnitRows, parts.used_rows = plan.most_rows < kUnitRows ? plan.most_rows : kUnitRows;
         launch(chunk_kernel<T, D>, plan.ctas, kChunkThreads, sizeof(ChunkShared<D>) + 1024, stream, false,
                ChunkArgs{a, parts});
         join();
@@ -1762,7 +1812,7 @@ extern "C" int kvsnap_c8_attend(const kvsnap_c8_cache* cache, const kvsnap_c8_ba
         char* at = static_cast<char*>(workspace);
         const Parts parts{reinterpret_cast<float*>(at), reinterpret_cast<float2*>(at + plan.sum_bytes),
                           reinterpret_cast<SharedUnit*>(at + plan.sum_bytes + plan.slots * int64_t(sizeof(float2))),
-                          0, 0};
+                          0, 0, 0};
         by_type(type, cache->head_dim, [&](auto t, auto d) {
             launch_attend<decltype(t), decltype(d)::value>(plan, a, parts, reinterpret_cast<cudaStream_t>(stream));
         });
