@@ -83,17 +83,17 @@ struct Parts {
 //
 // Sequences with at most kStepRows rows a KV head (query heads of the group times
 // new tokens). Bound by the cache's bytes, so nothing but a page's codes is read,
-// once, by the lanes whose matrix fragments they are: with the keys as the 16-row
-// operand of m16n8k16, lane (g, t) needs 16 bytes of tokens' rows g, and with the
-// values' transpose, 16 dims of 4 tokens. Which token
-// is row g and which dim is row g of the transpose is free as long as both
-// products agree, so it is chosen to make every load a 16-byte one and every pair
-// of codes that a fragment register holds adjacent after one byte permute. The
-// scores come out transposed, [token][row], and one 8x8 transpose in registers
-// makes them the weights' fragment. Each lane copies its own bytes to shared memory
-// asynchronously, kAhead granules ahead, and reads back only those: no warp waits
-// for another, and 128 KB an SM are on their way at a time (loads to registers, a
-// granule ahead, kept 64 KB and reached 4.1 TB/s where this reaches 5.3).
+// once. A warp copies a granule of 16 tokens to its own shared memory
+// asynchronously, kAhead granules ahead, no warp waiting for another; 8 lanes copy
+// one token's line, as 16-byte requests are joined among 8 lanes (with lanes that
+// each fetched the codes of their own fragments, 32 bytes of a line a request, this
+// kernel reached 4.1 TB/s). With the keys as the 16-row operand of m16n8k16 a
+// lane (g, t) then needs 16 bytes of tokens' rows g, and with the values'
+// transpose, 16 dims of 4 tokens. Which token is row g and which dim is row g of
+// the transpose is free as long as both products agree, so it is chosen to make
+// every read a 16-byte one and every pair of codes that a fragment register holds
+// adjacent after one byte permute. The scores come out transposed, [token][row],
+// and one 8x8 transpose in registers makes them the weights' fragment.
 
 constexpr int kStepRows = 16;
 constexpr int kWarps = 16;                 // a CTA: HC heads x TS slices of a chunk
@@ -131,13 +131,18 @@ __device__ __forceinline__ uint4 load16(const char* at, bool there) {
     return v;
 }
 
-// N bytes to shared memory, or zeros, on their way until copies_done.
-template <int N>
+// 16 bytes to shared memory, or zeros, on their way until copies_done.
 __device__ __forceinline__ void copy_async(uint32_t to, const char* from, bool there) {
-    if constexpr (N == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
-    else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(there ? 8 : 0) : "memory");
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+
+// Where 16 bytes `chunk` of a token's D codes lie in a granule of one side: lines of 128 bytes, their 16-byte
+// places turned so that the 8 lanes of a read meet all banks. Such lanes read the keys of tokens 4 k and
+// 4 k + 1 (+ 2), and 2 chunks of the values of tokens i, 4 + i, 8 + i, 12 + i.
+template <int D, bool VALUES>
+__device__ __forceinline__ uint32_t in_granule(int token, int chunk) {
+    const int line = token * D / 128, place = token * D % 128 / 16 + chunk;
+    return uint32_t(line * 128 + (place ^ (VALUES ? token / 4 * 2 : D == 128 ? token % 2 * 4 : 0)) * 16);
 }
 
 // All of the thread's copies but its last n groups.
@@ -145,11 +150,23 @@ template <int N>
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void copies_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 
+__device__ __forceinline__ uint2 read_shared8(uint32_t at) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
+    return v;
+}
+
 __device__ __forceinline__ uint4 read_shared(uint32_t at) {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
     return v;
 }
+
+// Where a warp's granule of a chunk lies, and its scales. A page that is not there: off < 0.
+struct __align__(16) StepPage {
+    int64_t off;
+    float ks, vs;
+};
 
 // Chunks of a sequence: TS granules each; a sequence without tokens has one, whose rows become zeros.
 __device__ __forceinline__ int chunks_of(const StepArgs& p, int s, Sequence& q) {
@@ -172,14 +189,14 @@ __device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* scratch) {
 template <typename T, int D, int NT>
 struct StepWarp {
     static constexpr int kHalves = D / 64, kTiles = D / 16;
-    static constexpr uint32_t kGranuleBytes = 512 * (2 * kHalves + 4);
+    static constexpr uint32_t kSideBytes = kGranule * D, kGranuleBytes = 2 * kSideBytes;
     float o[NT][kTiles][4];                // (dim pair, row) sums, relative to m and vref
     float m[NT][2], l[NT][2];              // of rows 8 nt + 2 t, + 1
     float vref;                            // largest value scale so far
 
-    // `ring`: the warp's kAhead granules of shared memory, 16 bytes a lane and piece.
+    // `ring`: the warp's kAhead granules of shared memory; `pages`: what it knows of 64 chunks' pages.
     __device__ __forceinline__ void run(const StepArgs& p, const Sequence& q, int s, int head, int slice, int c0,
-                                        int c1, uint32_t ring) {
+                                        int c1, uint32_t ring, StepPage* pages) {
         const int lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
         const Cache& c = p.a.c;
         const int rows = q.rows * p.a.group, first_seen = q.length - q.rows + 1;
@@ -243,70 +260,82 @@ struct StepWarp {
 
         const int token_a = 4 * (g >> 1) + (g & 1);                            // of score row g; row g + 8: + 2
         const char* keys = reinterpret_cast<const char*>(c.codes) + head * c.head_pitch;
-        const char* k_lane = keys + token_a * c.token_pitch + 16 * t;
-        const char* v_lane = keys + c.side_pitch + 4 * t * c.token_pitch + (D / 8) * g;
-        const int64_t two_tokens = 2 * c.token_pitch;
+        const int stride = p.ts * kGranule, skip = slice * kGranule;
+        // What the lane copies: `kLines` times a chunk of a token, kAcross lanes a token.
+        constexpr int kAcross = D / 16, kLines = kGranule * kAcross / 32, kTokens = 32 / kAcross;
+        const char* const from = keys + lane / kAcross * c.token_pitch + lane % kAcross * 16;
+        // What it reads: keys of tokens token_a and token_a + 2, D / 8 values of tokens 4 t to 4 t + 3.
+        uint32_t k_read[kHalves][2], v_read[4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int half = 0; half < kHalves; ++half) k_read[half][i] = in_granule<D, false>(token_a + 2 * i, t + 4 * half);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            v_read[i] = kSideBytes + in_granule<D, true>(4 * t + i, D == 128 ? g : g / 2) + (D == 128 ? 0 : g % 2 * 8);
 
-        ring += lane * 16;
-        // Pages of 32 chunks at a time, one a lane: where the warp's granule lies, and its scales, now and of
-        // the 32 before, as copies run ahead of the products. A page that is not there has a negative scale.
-        int64_t off = -1;
-        float ks = 0.0f, vs = 0.0f, ks_before = 0.0f, vs_before = 0.0f;
-        int window = -1;
-        const auto copy = [&](int chunk) {
-            const int j = chunk - c0;
-            if (j / 32 != window) {
-                window = j / 32;
-                ks_before = ks, vs_before = vs;
-                const int64_t token = (int64_t(chunk + lane) * p.ts + slice) * kGranule;
-                off = -1, ks = 0.0f, vs = -1.0f;
-                if (chunk + lane < c1 && token < q.length) {
-                    const int64_t block = ints(p.a.b.table)[s * p.a.b.table_pitch + token / c.block_size];
-                    if (block < 0 || block >= c.blocks) {
-                        atomicOr(p.a.status, KVSNAP_DP_BAD_BLOCK);
-                    } else {
-                        off = block * c.block_pitch + token % c.block_size * c.token_pitch;
-                        const float* scales = reinterpret_cast<const float*>(c.scales) + block * 2 * c.kv_heads + head;
-                        ks = scales[0], vs = scales[c.kv_heads];
+        // Copies of the chunk `ahead` go to ring place `to`. Pages are looked up for 32 chunks at a time, a lane each.
+        int ahead = c0;
+        uint32_t to = ring;
+        const auto copy = [&] {
+            if (ahead < c1) {
+                const int j = ahead - c0;
+                if (j % 32 == 0) {
+                    const int token = (ahead + lane) * stride + skip;
+                    StepPage page{-1, 0.0f, 0.0f};
+                    if (ahead + lane < c1 && token < q.length) {
+                        const int64_t block = ints(p.a.b.table)[s * p.a.b.table_pitch + token / c.block_size];
+                        if (block < 0 || block >= c.blocks) {
+                            atomicOr(p.a.status, KVSNAP_DP_BAD_BLOCK);
+                        } else {
+                            page.off = block * c.block_pitch + token % c.block_size * c.token_pitch;
+                            const float* scales = reinterpret_cast<const float*>(c.scales) + block * 2 * c.kv_heads + head;
+                            page.ks = scales[0], page.vs = scales[c.kv_heads];
+                        }
                     }
+                    __syncwarp();
+                    pages[j % 64 + lane] = page;
+                    __syncwarp();
                 }
+                const int64_t found = pages[j % 64].off, at = max(found, int64_t(0));
+                const bool there = found >= 0;
+                __syncwarp();                            // the place's last readers are done
+#pragma unroll
+                for (int i = 0; i < kLines; ++i) {
+                    const int token = i * kTokens + lane / kAcross;
+                    const char* const line = from + (at + i * kTokens * c.token_pitch);
+                    copy_async(to + in_granule<D, false>(token, lane % kAcross), line, there);
+                    copy_async(to + kSideBytes + in_granule<D, true>(token, lane % kAcross), line + c.side_pitch, there);
+                }
+                ++ahead;
+                to = to == ring + (kAhead - 1) * kGranuleBytes ? ring : to + kGranuleBytes;
             }
-            const int64_t found = __shfl_sync(~0u, off, j % 32), at = max(found, int64_t(0));
-            const bool there = found >= 0;
-            const uint32_t to = ring + j % kAhead * kGranuleBytes;
-#pragma unroll
-            for (int half = 0; half < kHalves; ++half)
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    copy_async<16>(to + (half * 2 + i) * 512, k_lane + at + i * two_tokens + 64 * half, there);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                copy_async<D / 8>(to + (kHalves * 2 + i) * 512, v_lane + at + i * c.token_pitch, there);
+            copies_group();
         };
 
+#pragma unroll 1
+        for (int i = 0; i < kAhead - 1; ++i) copy();
+        uint32_t at = ring;
+        float limit[NT][2], v_by = 0.0f;             // m + kSlack; 1 / vref
 #pragma unroll
-        for (int i = 0; i < kAhead - 1; ++i) {
-            if (c0 + i < c1) copy(c0 + i);
-            copies_group();
-        }
+        for (int nt = 0; nt < NT; ++nt) limit[nt][0] = limit[nt][1] = kLowest;
+#pragma unroll 1
         for (int chunk = c0; chunk < c1; ++chunk) {
-            const int j = chunk - c0;
-            if (chunk + kAhead - 1 < c1) copy(chunk + kAhead - 1);
-            copies_group();
+            copy();
             copies_done<kAhead - 1>();
-            const uint32_t at = ring + j % kAhead * kGranuleBytes;
-            const bool old = j / 32 != window;
-            const float k_scale = __shfl_sync(~0u, old ? ks_before : ks, j % 32);
-            const float v_scale = __shfl_sync(~0u, old ? vs_before : vs, j % 32);
-            const bool dead = v_scale < 0.0f;
-            const int64_t base = (int64_t(chunk) * p.ts + slice) * kGranule;
+            __syncwarp();
+            const StepPage page = pages[(chunk - c0) % 64];
+            const int base = chunk * stride + skip;
 
-            float sc[NT][4];
+            // Two chains of products, so that one does not wait for the other.
+            float sc[NT][4], odd[NT][4];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.0f;
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sc[nt][i] = odd[nt][i] = 0.0f;
 #pragma unroll
             for (int half = 0; half < kHalves; ++half) {
-                const uint4 ka = read_shared(at + half * 1024), kb = read_shared(at + half * 1024 + 512);
+                const uint4 ka = read_shared(at + k_read[half][0]), kb = read_shared(at + k_read[half][1]);
                 const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
@@ -314,26 +343,49 @@ struct StepWarp {
                     const uint32_t a1 = half2_of_codes(uint16_t(wb[w])), a3 = half2_of_codes(uint16_t(wb[w] >> 16));
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
-                        mma16816(sc[nt], a0, a1, a2, a3, qb[nt][half * 4 + w][0], qb[nt][half * 4 + w][1]);
+                        mma16816(w % 2 ? odd[nt] : sc[nt], a0, a1, a2, a3, qb[nt][half * 4 + w][0], qb[nt][half * 4 + w][1]);
                 }
             }
-            // Edge: tokens that some row does not see, or a page that is not there.
-            const bool edge = dead || base + kGranule > first_seen;
-            bool grow = false;
+            uint4 vr[4];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (D == 128) {
+                    vr[i] = read_shared(at + v_read[i]);
+                } else {
+                    const uint2 x = read_shared8(at + v_read[i]);
+                    vr[i] = make_uint4(x.x, x.y, 0, 0);
+                }
+            }
+            at = at == ring + (kAhead - 1) * kGranuleBytes ? ring : at + kGranuleBytes;
+
+            // Edge: tokens that some row does not see, or a page that is not there.
+            const bool dead = page.off < 0, edge = dead || base + kGranule > first_seen;
+            bool grow = page.vs > vref;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const float f = factor[nt][i] * k_scale;
-                    sc[nt][i] *= f, sc[nt][2 + i] *= f;
-                    if (edge) {
+                    const float f = factor[nt][i] * page.ks;
+                    sc[nt][i] = (sc[nt][i] + odd[nt][i]) * f, sc[nt][2 + i] = (sc[nt][2 + i] + odd[nt][2 + i]) * f;
+                }
+            if (edge) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
                         if (dead || base + token_a >= seen[nt][i]) sc[nt][i] = -INFINITY;
                         if (dead || base + token_a + 2 >= seen[nt][i]) sc[nt][2 + i] = -INFINITY;
                     }
-                    grow |= fmaxf(sc[nt][i], sc[nt][2 + i]) > m[nt][i] + kSlack;
-                }
             }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) grow |= fmaxf(sc[nt][i], sc[nt][2 + i]) > limit[nt][i];
             if (__any_sync(~0u, grow)) {
+                // Weights carry the page's value scale relative to the largest so far, so fp16 holds them.
+                const float v_keep = page.vs > vref ? vref / page.vs : 1.0f;
+                vref = fmaxf(vref, page.vs);
+                v_by = vref > 0.0f ? 1.0f / vref : 0.0f;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -345,22 +397,13 @@ struct StepWarp {
                         top = fmaxf(top, m[nt][i]);
                         const float keep = exp2_fast(m[nt][i] - top);
                         m[nt][i] = top, l[nt][i] *= keep;
+                        limit[nt][i] = top + kSlack;
 #pragma unroll
-                        for (int mt = 0; mt < kTiles; ++mt) o[nt][mt][i] *= keep, o[nt][mt][2 + i] *= keep;
+                        for (int mt = 0; mt < kTiles; ++mt)
+                            o[nt][mt][i] *= keep * v_keep, o[nt][mt][2 + i] *= keep * v_keep;
                     }
             }
-            // Weights carry the page's value scale relative to the largest so far, so fp16 holds them.
-            if (v_scale > vref) {
-                const float keep = vref / v_scale;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int mt = 0; mt < kTiles; ++mt)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) o[nt][mt][i] *= keep;
-                vref = v_scale;
-            }
-            const float part = vref > 0.0f ? v_scale / vref : 0.0f;
+            const float part = page.vs * v_by;
             uint32_t pb[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -372,9 +415,6 @@ struct StepWarp {
                 pb[nt][1] = transpose8x8(pack_half2(w[2] * part, w[3] * part));
             }
 
-            uint4 vr[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) vr[i] = read_shared(at + (kHalves * 2 + i) * 512);
             const auto add_values = [&](const uint4 (&v)[4], const uint32_t (&b)[NT][2]) {
                 const uint32_t w[4][4] = {{v[0].x, v[0].y, v[0].z, v[0].w}, {v[1].x, v[1].y, v[1].z, v[1].w},
                                           {v[2].x, v[2].y, v[2].z, v[2].w}, {v[3].x, v[3].y, v[3].z, v[3].w}};
@@ -394,6 +434,7 @@ struct StepWarp {
             } else if (!dead) {
                 // One new token at a time, with the values it does not see left out: a weight of 0
                 // times what a masked slot holds (NaN, say) must not reach it.
+#pragma unroll 1
                 for (int i = 0; i < q.rows; ++i) {
                     if (first_seen + i <= base) continue;
                     uint4 v[4];
@@ -426,9 +467,10 @@ struct StepShared {
     static constexpr int kPitch = D + 4;
     union {
         float o[kWarps][8 * NT][kPitch];   // once the granules are done with
-        char ring[kWarps][kAhead * 512 * (2 * (D / 64) + 4)];
+        char ring[kWarps][kAhead * 2 * kGranule * D];
     };
     float2 ml[kWarps][8 * NT];
+    StepPage pages[kWarps][64];
     int64_t scratch[kWarps];
     int64_t prefix[kWarps];
     int64_t found_first;
@@ -505,7 +547,8 @@ __global__ void __launch_bounds__(32 * kWarps, 1) step_kernel(const __grid_const
         const int hc = warp % p.hc, slice = warp / p.hc;       // a warp without a slice only waits
         StepWarp<T, D, NT> w;
         if (slice < p.ts) {
-            w.run(p, q, s, hg * p.hc + hc, slice, c0, c1, uint32_t(__cvta_generic_to_shared(sh.ring[warp])));
+            w.run(p, q, s, hg * p.hc + hc, slice, c0, c1, uint32_t(__cvta_generic_to_shared(sh.ring[warp])),
+                  sh.pages[warp]);
         }
         __syncthreads();
         if (slice < p.ts) {
