@@ -49,10 +49,10 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
-__device__ __forceinline__ uint32_t half2_of_codes(uint16_t codes) {
-    uint32_t d;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(d) : "h"(codes));
-    return d;
+// Four codes as two pairs of fp16, exactly.
+__device__ __forceinline__ void halves_of_codes(uint32_t codes, uint32_t& low, uint32_t& high) {
+    asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\ncvt.rn.f16x2.e4m3x2 %1, b;\n}"
+        : "=r"(low), "=r"(high) : "r"(codes));
 }
 
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
@@ -261,18 +261,15 @@ struct StepWarp {
         const int token_a = 4 * (g >> 1) + (g & 1);                            // of score row g; row g + 8: + 2
         const char* keys = reinterpret_cast<const char*>(c.codes) + head * c.head_pitch;
         const int stride = p.ts * kGranule, skip = slice * kGranule;
-        // What the lane copies: `kLines` times a chunk of a token, kAcross lanes a token.
-        constexpr int kAcross = D / 16, kLines = kGranule * kAcross / 32, kTokens = 32 / kAcross;
-        const char* const from = keys + lane / kAcross * c.token_pitch + lane % kAcross * 16;
-        // What it reads: keys of tokens token_a and token_a + 2, D / 8 values of tokens 4 t to 4 t + 3.
-        uint32_t k_read[kHalves][2], v_read[4];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int half = 0; half < kHalves; ++half) k_read[half][i] = in_granule<D, false>(token_a + 2 * i, t + 4 * half);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            v_read[i] = kSideBytes + in_granule<D, true>(4 * t + i, D == 128 ? g : g / 2) + (D == 128 ? 0 : g % 2 * 8);
+        // What the lane copies: a chunk of each of kLines tokens, kAcross lanes a token; what it reads: keys of
+        // tokens token_a and token_a + 2, D / 8 values of tokens 4 t to 4 t + 3. Each is one place and, for the
+        // others, a constant away or in the line's other half (xor 64).
+        constexpr int kAcross = D / 16, kLines = kGranule * kAcross / 32;
+        const int first = lane / kAcross * kLines;
+        const char* const from = keys + first * c.token_pitch + lane % kAcross * 16;
+        const uint32_t k_put = in_granule<D, false>(first, lane % kAcross), v_put = in_granule<D, true>(first, lane % kAcross);
+        const uint32_t k_read = in_granule<D, false>(token_a, t);
+        const uint32_t v_read = kSideBytes + in_granule<D, true>(4 * t, D == 128 ? g : g / 2) + (D == 128 ? 0 : g % 2 * 8);
 
         // Copies of the chunk `ahead` go to ring place `to`. Pages are looked up for 32 chunks at a time, a lane each.
         int ahead = c0;
@@ -300,12 +297,15 @@ struct StepWarp {
                 const int64_t found = pages[j % 64].off, at = max(found, int64_t(0));
                 const bool there = found >= 0;
                 __syncwarp();                            // the place's last readers are done
+                const char* line = from + at;
 #pragma unroll
                 for (int i = 0; i < kLines; ++i) {
-                    const int token = i * kTokens + lane / kAcross;
-                    const char* const line = from + (at + i * kTokens * c.token_pitch);
-                    copy_async(to + in_granule<D, false>(token, lane % kAcross), line, there);
-                    copy_async(to + kSideBytes + in_granule<D, true>(token, lane % kAcross), line + c.side_pitch, there);
+                    // (keys and values swizzle by other bits of the token)
+                    const uint32_t k_to = D == 128 ? (to + k_put ^ i % 2 * 64) + i * 128 : to + k_put + i * 64;
+                    const uint32_t v_to = D == 128 ? to + v_put + i * 128 : to + v_put ^ i * 64;
+                    copy_async(k_to, line, there);
+                    copy_async(v_to + kSideBytes, line + c.side_pitch, there);
+                    line += c.token_pitch;
                 }
                 ++ahead;
                 to = to == ring + (kAhead - 1) * kGranuleBytes ? ring : to + kGranuleBytes;
@@ -335,12 +335,14 @@ struct StepWarp {
                 for (int i = 0; i < 4; ++i) sc[nt][i] = odd[nt][i] = 0.0f;
 #pragma unroll
             for (int half = 0; half < kHalves; ++half) {
-                const uint4 ka = read_shared(at + k_read[half][0]), kb = read_shared(at + k_read[half][1]);
+                const uint32_t read = at + k_read ^ half * 64;
+                const uint4 ka = read_shared(read), kb = read_shared(read + D * 2);
                 const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
-                    const uint32_t a0 = half2_of_codes(uint16_t(wa[w])), a2 = half2_of_codes(uint16_t(wa[w] >> 16));
-                    const uint32_t a1 = half2_of_codes(uint16_t(wb[w])), a3 = half2_of_codes(uint16_t(wb[w] >> 16));
+                    uint32_t a0, a1, a2, a3;
+                    halves_of_codes(wa[w], a0, a2);
+                    halves_of_codes(wb[w], a1, a3);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
                         mma16816(w % 2 ? odd[nt] : sc[nt], a0, a1, a2, a3, qb[nt][half * 4 + w][0], qb[nt][half * 4 + w][1]);
@@ -350,9 +352,9 @@ struct StepWarp {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if constexpr (D == 128) {
-                    vr[i] = read_shared(at + v_read[i]);
+                    vr[i] = read_shared(at + v_read + i * 128);
                 } else {
-                    const uint2 x = read_shared8(at + v_read[i]);
+                    const uint2 x = read_shared8((at + v_read ^ i % 2 * 64) + i / 2 * 128);
                     vr[i] = make_uint4(x.x, x.y, 0, 0);
                 }
             }
@@ -423,8 +425,9 @@ struct StepWarp {
                     const uint32_t pick = mt % 2 ? 0x7362 : 0x5140;
                     const uint32_t x = __byte_perm(w[0][mt / 2], w[1][mt / 2], pick);
                     const uint32_t y = __byte_perm(w[2][mt / 2], w[3][mt / 2], pick);
-                    const uint32_t a0 = half2_of_codes(uint16_t(x)), a1 = half2_of_codes(uint16_t(x >> 16));
-                    const uint32_t a2 = half2_of_codes(uint16_t(y)), a3 = half2_of_codes(uint16_t(y >> 16));
+                    uint32_t a0, a1, a2, a3;
+                    halves_of_codes(x, a0, a1);
+                    halves_of_codes(y, a2, a3);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][mt], a0, a1, a2, a3, b[nt][0], b[nt][1]);
                 }
@@ -1209,8 +1212,8 @@ __device__ __forceinline__ void convert_role(const ChunkArgs& p, ChunkShared<D>&
             uint32_t h[8];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                h[2 * j] = times_half2(half2_of_codes(uint16_t(x[j])), f);
-                h[2 * j + 1] = times_half2(half2_of_codes(uint16_t(x[j] >> 16)), f);
+                halves_of_codes(x[j], h[2 * j], h[2 * j + 1]);
+                h[2 * j] = times_half2(h[2 * j], f), h[2 * j + 1] = times_half2(h[2 * j + 1], f);
             }
             store_shared(to + swizzled<kStep>(token, 2 * piece), h[0], h[1], h[2], h[3]);
             store_shared(to + swizzled<kStep>(token, 2 * piece + 1), h[4], h[5], h[6], h[7]);
