@@ -97,7 +97,6 @@ struct Parts {
 
 constexpr int kStepRows = 16;
 constexpr int kWarps = 16;                 // a CTA: HC heads x TS slices of a chunk
-constexpr int kGranule = 16;               // tokens a warp takes at a time
 constexpr int kAhead = 3;                  // granules a warp holds: one in use, the others on their way
 constexpr float kLowest = -3e38f;          // the running maximum before any token
 constexpr float kSlack = 14.0f;            // log2 by which a weight may exceed 1 before sums are rescaled (fp16: 2^16)

@@ -61,68 +61,119 @@ __device__ __forceinline__ bool find_page(const Batch& b, int n, int64_t u, Page
     return true;
 }
 
-// The rotation of 8 consecutive elements [at, at + 8) of a head, from its row in memory.
+// 8 consecutive elements [at, at + 8) of a head's row, rotated. What they take from memory:
+struct Turned {
+    uint4 own, other;         // the elements, and those that they are turned with
+    float4 turn[4];           // (cos, sin) of their pairs
+};
+
+template <bool INTERLEAVED>
+__device__ __forceinline__ void fetch_turned(Turned& x, const char* row, int at, const float2* turn, int rotary_dim,
+                                             bool there) {
+    const bool turned = there && at < rotary_dim;
+    x.own = fetch16(row + 2 * at, there);
+    const int half = rotary_dim / 2;
+    const int pair = INTERLEAVED ? at / 2 : at < half ? at : at - half;
+    if (!INTERLEAVED) x.other = fetch16(row + 2 * (at < half ? at + half : at - half), turned);
+#pragma unroll
+    for (int i = 0; i < (INTERLEAVED ? 2 : 4); ++i) {
+        const uint4 t = fetch16(reinterpret_cast<const char*>(turn + pair + 2 * i), turned);
+        x.turn[i] = make_float4(__uint_as_float(t.x), __uint_as_float(t.y), __uint_as_float(t.z), __uint_as_float(t.w));
+    }
+}
+
 template <typename T, bool INTERLEAVED>
-__device__ __forceinline__ void load_rotated(const char* row, int at, const float2* turn, int rotary_dim,
-                                             float (&v)[8]) {
-    load8<T>(row + 2 * at, v);
-    if (!turn || at >= rotary_dim) return;
+__device__ __forceinline__ void turn8(const Turned& x, int at, int rotary_dim, float (&v)[8]) {
+    widen8<T>(x.own, v);
+    if (at >= rotary_dim) return;
     if (INTERLEAVED) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float2 t = turn[at / 2 + i];
+            const float c = i % 2 ? x.turn[i / 2].z : x.turn[i / 2].x, s = i % 2 ? x.turn[i / 2].w : x.turn[i / 2].y;
             const float a = v[2 * i], b = v[2 * i + 1];
-            v[2 * i] = a * t.x - b * t.y;
-            v[2 * i + 1] = b * t.x + a * t.y;
+            v[2 * i] = a * c - b * s;
+            v[2 * i + 1] = b * c + a * s;
         }
     } else {
-        const int half = rotary_dim / 2;
-        const bool low = at < half;
-        const int pair = low ? at : at - half;
+        const float sign = at < rotary_dim / 2 ? -1.0f : 1.0f;
         float w[8];
-        load8<T>(row + 2 * (low ? at + half : at - half), w);
+        widen8<T>(x.other, w);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float2 t = turn[pair + i];
-            v[i] = low ? v[i] * t.x - w[i] * t.y : v[i] * t.x + w[i] * t.y;
+            const float c = i % 2 ? x.turn[i / 2].z : x.turn[i / 2].x, s = i % 2 ? x.turn[i / 2].w : x.turn[i / 2].y;
+            v[i] = v[i] * c + sign * (w[i] * s);
         }
     }
 }
 
-constexpr int kHeld = 8;      // row groups of a page that a warp keeps in registers (64 values a lane)
+constexpr int kHeld = 8;      // row groups of a page that a warp keeps in registers, as they come
 
-// One warp: one page of one key or value head, or its query rows of one query head.
-// A row is D / 8 lanes of 8 elements, so a warp takes 256 / D rows a step.
+// The largest finite size among a warp's rows: of the 16-bit words as they are, and where that is no
+// finite number, once more without those that are not.
+template <typename T>
+__device__ __forceinline__ float largest(const uint4 (&raw)[kHeld]) {
+    uint32_t tops = 0;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+        tops = T::max_size(T::max_size(T::max_size(T::max_size(tops, raw[i].x), raw[i].y), raw[i].z), raw[i].w);
+    const float2 pair = T::wide(tops);
+    float top = warp_max(fmaxf(pair.x, pair.y));
+    if (top > 3.402823466e38f) {
+        top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            float v[8];
+            widen8<T>(raw[i], v);
+            top = max8(v, top);
+        }
+        top = warp_max(top);
+    }
+    return top;
+}
+
+// One warp: one page of one key or value head, or its query rows of one query head. A row is D / 8 lanes
+// of 8 elements, so a warp takes 256 / D rows a step. Bound by memory: loads are issued for several steps
+// before any is waited for, and predicated (where a branch around a load joins, the load is waited for).
+// Keys are read twice, the second time from the L1 or L2: rotated they would take twice the registers.
 template <typename T, int D, bool SINGLE, bool INTERLEAVED>
-__global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ AppendArgs a) {
-    constexpr int kLanes = D / 8, kRows = 32 / kLanes;
+__global__ void __launch_bounds__(256, 3) append_kernel(const __grid_constant__ AppendArgs a) {
+    constexpr int kLanes = D / 8, kRows = 32 / kLanes, kSteps = SINGLE ? 1 : 2;
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, n = a.c.block_size;
     const int slot = blockIdx.y * 8 + warp;
     if (slot >= 2 * a.c.kv_heads + a.q_heads) return;
     PageRun run;
     if (!find_page<SINGLE>(a.b, n, blockIdx.x, run, a.status)) return;
-    const int sub = lane / kLanes, at = lane % kLanes * 8;
-    const int64_t base = int64_t(run.page) * n;                        // position of the page's slot 0
+    const int sub = lane / kLanes, at = lane % kLanes * 8, end = run.first + run.count;
+    const int base = run.page * n;                                     // position of the page's slot 0
+    const int rotary_dim = a.rotary ? a.rotary_dim : 0;
+    if (a.rotary && base + end > a.positions && lane == 0) atomicOr(a.status, KVSNAP_C8_BAD_POSITION);
 
-    const auto turn = [&](int r) -> const float2* {                    // row r of the page
-        if (!a.rotary) return nullptr;
-        int64_t p = base + r;
-        if (p >= a.positions) {
-            atomicOr(a.status, KVSNAP_C8_BAD_POSITION);
-            p = a.positions - 1;
+    // Turned rows [run.first + sub, end), kSteps at a time, to `each`.
+    const auto for_turned = [&](const char* rows, int64_t pitch, auto each) {
+        for (int r = run.first + sub; r - sub < end; r += kSteps * kRows) {
+            Turned x[kSteps];
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                const int row = r + i * kRows;
+                const int64_t position = min(int64_t(base + row), a.positions - 1);
+                fetch_turned<INTERLEAVED>(x[i], rows + (run.row + (row - run.first)) * pitch, at,
+                                          a.rotary + position * (rotary_dim / 2), rotary_dim, row < end);
+            }
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                float v[8];
+                turn8<T, INTERLEAVED>(x[i], at, rotary_dim, v);
+                if (r + i * kRows < end) each(r + i * kRows, v);
+            }
         }
-        return a.rotary + p * (a.rotary_dim / 2);
     };
 
     if (slot >= 2 * a.c.kv_heads) {
         const int head = slot - 2 * a.c.kv_heads;
-        for (int r = run.first + sub; r < run.first + run.count; r += kRows) {
-            const int64_t row = run.row + (r - run.first);
-            float v[8];
-            load_rotated<T, INTERLEAVED>(a.query.at + row * a.query.token + head * a.query.head, at, turn(r),
-                                         a.rotary_dim, v);
-            store8<T>(a.query_out + ((row * a.q_heads + head) * D + at) * 2, v);
-        }
+        char* out = a.query_out + (int64_t(run.row) * a.q_heads + head) * (2 * D) + 2 * at;
+        for_turned(a.query.at + head * a.query.head, a.query.token, [&](int r, const float (&v)[8]) {
+            store8<T>(out + int64_t(r - run.first) * a.q_heads * (2 * D), v);
+        });
         return;
     }
 
@@ -135,41 +186,42 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
     char* codes = reinterpret_cast<char*>(a.c.codes) + side * a.c.side_pitch + block * a.c.block_pitch +
                   head * a.c.head_pitch + at;
     float* scale_at = reinterpret_cast<float*>(a.c.scales) + (block * 2 + side) * a.c.kv_heads + head;
-    const Rows& from = side ? a.value : a.key;
-    const char* rows = from.at + head * from.head;
-    const auto fetch = [&](int r, float (&v)[8]) {
-        const char* row = rows + (run.row + (r - run.first)) * from.token;
-        if (side) load8<T>(row + 2 * at, v);
-        else load_rotated<T, INTERLEAVED>(row, at, turn(r), a.rotary_dim, v);
-    };
-
-    const int end = run.first + run.count;
-    float kept[kHeld][8], amax = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-        const int r = run.first + i * kRows + sub;
-        if (r < end) {
-            fetch(r, kept[i]);
-            amax = max8(kept[i], amax);
-        }
-    }
-    for (int r = run.first + kHeld * kRows + sub; r < end; r += kRows) {
-        float v[8];
-        fetch(r, v);
-        amax = max8(v, amax);
-    }
     const float held = run.first ? *scale_at : 0.0f;
-    const float scale = fmaxf(held, needed_scale(warp_max(amax)));
-    const float by = inverse(scale);
+    float scale, by;
+    if (side == 0) {
+        const char* rows = a.key.at + head * a.key.head;
+        float top = 0.0f;
+        for_turned(rows, a.key.token, [&](int, const float (&v)[8]) { top = max8(v, top); });
+        scale = fmaxf(held, needed_scale(warp_max(top))), by = inverse(scale);
+        for_turned(rows, a.key.token, [&](int r, const float (&v)[8]) { store_codes(codes + r * a.c.token_pitch, v, by); });
+    } else {
+        const char* rows = a.value.at + head * a.value.head + 2 * at - run.first * a.value.token;
+        uint4 raw[kHeld];
+        float top = 0.0f;
+        for (int first = run.first + kHeld * kRows; first < end; first += kHeld * kRows) {     // rows too many to hold
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-        const int r = run.first + i * kRows + sub;
-        if (r < end) store_codes(codes + r * a.c.token_pitch, kept[i], by);
-    }
-    for (int r = run.first + kHeld * kRows + sub; r < end; r += kRows) {
-        float v[8];
-        fetch(r, v);
-        store_codes(codes + r * a.c.token_pitch, v, by);
+            for (int i = 0; i < kHeld; ++i) {
+                const int r = first + i * kRows + sub;
+                raw[i] = fetch16(rows + (run.row + int64_t(r)) * a.value.token, r < end);
+            }
+            top = fmaxf(top, largest<T>(raw));
+        }
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            const int r = run.first + i * kRows + sub;
+            raw[i] = fetch16(rows + (run.row + int64_t(r)) * a.value.token, r < end);
+        }
+        scale = fmaxf(held, needed_scale(fmaxf(top, largest<T>(raw)))), by = inverse(scale);
+        for (int first = run.first; first < end; first += kHeld * kRows) {
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i) {
+                const int r = first + i * kRows + sub;
+                if (first > run.first) raw[i] = fetch16(rows + (run.row + int64_t(r)) * a.value.token, r < end);
+                float v[8];
+                widen8<T>(raw[i], v);
+                if (r < end) store_codes(codes + r * a.c.token_pitch, v, by);
+            }
+        }
     }
     if (!run.first || scale > held) {
         for (int r = sub; r < run.first; r += kRows) {                 // older tokens, at the grown scale
@@ -192,7 +244,7 @@ struct ConvertArgs {
     uint32_t* status;
 };
 
-// One warp: one layer, block, side and head.
+// One warp: one layer, block, side and head. Grid: (block and head, layer and side).
 struct ConvertUnit {
     char *codes, *wide;
     float* scale;
@@ -200,15 +252,12 @@ struct ConvertUnit {
     int rows;                 // token slots that hold tokens
 };
 
-__device__ __forceinline__ bool convert_unit(const ConvertArgs& a, int64_t u, ConvertUnit& unit) {
-    const int head = int(u % a.kv_heads);
-    int64_t rest = u / a.kv_heads;
-    const int side = int(rest & 1);
-    rest >>= 1;
-    const int64_t i = rest % a.n;
-    const int layer = int(rest / a.n);
-    if (layer >= a.layers) return false;
-    const kvsnap_c8_pair& p = a.pairs[layer];
+__device__ __forceinline__ bool convert_unit(const ConvertArgs& a, ConvertUnit& unit) {
+    const uint32_t u = blockIdx.x * 8 + threadIdx.x / 32;
+    const int64_t i = u / a.kv_heads;
+    const int head = u % a.kv_heads, side = blockIdx.y & 1;
+    if (i >= a.n) return false;
+    const kvsnap_c8_pair& p = a.pairs[blockIdx.y / 2];
     const int64_t block = a.ids[i], from = a.wide_ids[i];
     if (block < 0 || block >= p.blocks || from < 0 || from >= p.wide_blocks) {
         if (threadIdx.x % 32 == 0) atomicOr(a.status, KVSNAP_DP_BAD_BLOCK);
@@ -223,53 +272,64 @@ __device__ __forceinline__ bool convert_unit(const ConvertArgs& a, int64_t u, Co
     return true;
 }
 
+// Bound by memory: a warp holds a page's head as it comes (32 registers), so that four CTAs an SM keep
+// 128 KB of loads on their way.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) compress_kernel(const __grid_constant__ ConvertArgs a) {
+__global__ void __launch_bounds__(256, 4) compress_kernel(const __grid_constant__ ConvertArgs a) {
     constexpr int kLanes = D / 8, kRows = 32 / kLanes;
     const int lane = threadIdx.x % 32, sub = lane / kLanes, at = lane % kLanes * 8;
     ConvertUnit unit;
-    if (!convert_unit(a, int64_t(blockIdx.x) * 8 + threadIdx.x / 32, unit)) return;
-    float kept[kHeld][8], amax = 0.0f;
+    if (!convert_unit(a, unit)) return;
+    const char* from = unit.wide + 2 * at;
+    uint4 raw[kHeld];
+    const auto fetch = [&](int first) {
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-        const int r = i * kRows + sub;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) kept[i][j] = 0.0f;
-        if (r < unit.rows) {
-            load8<T>(unit.wide + r * unit.wide_token + 2 * at, kept[i]);
-            amax = max8(kept[i], amax);
+        for (int i = 0; i < kHeld; ++i) {
+            const int r = first + i * kRows + sub;
+            raw[i] = fetch16(from + r * unit.wide_token, r < unit.rows);
         }
+    };
+    float top = 0.0f;
+    for (int first = kHeld * kRows; first < unit.rows; first += kHeld * kRows) {     // rows too many to hold
+        fetch(first);
+        top = fmaxf(top, largest<T>(raw));
     }
-    for (int r = kHeld * kRows + sub; r < unit.rows; r += kRows) {
-        float v[8];
-        load8<T>(unit.wide + r * unit.wide_token + 2 * at, v);
-        amax = max8(v, amax);
-    }
-    const float scale = needed_scale(warp_max(amax)), by = inverse(scale);
+    fetch(0);
+    const float scale = needed_scale(fmaxf(top, largest<T>(raw))), by = inverse(scale);
+    for (int first = 0; first < a.block_size; first += kHeld * kRows) {
+        if (first) fetch(first);
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-        const int r = i * kRows + sub;
-        if (r < a.block_size) store_codes(unit.codes + r * unit.token + at, kept[i], by);
-    }
-    for (int r = kHeld * kRows + sub; r < a.block_size; r += kRows) {
-        float v[8] = {};
-        if (r < unit.rows) load8<T>(unit.wide + r * unit.wide_token + 2 * at, v);
-        store_codes(unit.codes + r * unit.token + at, v, by);
+        for (int i = 0; i < kHeld; ++i) {
+            const int r = first + i * kRows + sub;
+            float v[8];
+            widen8<T>(raw[i], v);
+            if (r < a.block_size) store_codes(unit.codes + r * unit.token + at, v, by);
+        }
     }
     if (lane == 0) *unit.scale = scale;
 }
 
+// A lane takes 16 codes, so that both sides move in 16-byte accesses.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) expand_kernel(const __grid_constant__ ConvertArgs a) {
-    constexpr int kLanes = D / 8, kRows = 32 / kLanes;
-    const int lane = threadIdx.x % 32, sub = lane / kLanes, at = lane % kLanes * 8;
+__global__ void __launch_bounds__(256, 4) expand_kernel(const __grid_constant__ ConvertArgs a) {
+    constexpr int kLanes = D / 16, kRows = 32 / kLanes, kSteps = kGranule / kRows;
+    const int lane = threadIdx.x % 32, sub = lane / kLanes, at = lane % kLanes * 16;
     ConvertUnit unit;
-    if (!convert_unit(a, int64_t(blockIdx.x) * 8 + threadIdx.x / 32, unit)) return;
+    if (!convert_unit(a, unit)) return;
     const float scale = *unit.scale;
-    for (int r = sub; r < a.block_size; r += kRows) {
-        float v[8];
-        load_codes(unit.codes + r * unit.token + at, scale, v);
-        store8<T>(unit.wide + r * unit.wide_token + 2 * at, v);
+    for (int first = sub; first < a.block_size; first += kGranule) {
+        uint4 raw[kSteps];
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) raw[i] = fetch16(unit.codes + (first + i * kRows) * unit.token + at, true);
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            float v[8];
+            char* to = unit.wide + (first + i * kRows) * unit.wide_token + 2 * at;
+            widen_codes(make_uint2(raw[i].x, raw[i].y), scale, v);
+            store8<T>(to, v);
+            widen_codes(make_uint2(raw[i].z, raw[i].w), scale, v);
+            store8<T>(to + 16, v);
+        }
     }
 }
 
@@ -332,17 +392,17 @@ int convert(const kvsnap_c8_pair* pairs, int layers, int block_size, int kv_head
         check_type(type);
         require(head_dim == 64 || head_dim == 128, "head_dim must be 64 or 128");
         require(block_size > 0 && block_size % 16 == 0 && kv_heads > 0, "block_size must be a multiple of 16");
-        require(n < (1LL << 31) && 2 * n * layers / 8 * kv_heads < (1LL << 30), "too many blocks for one conversion");
+        require(n < (1LL << 31) && n * kv_heads < (1LL << 31) && layers <= 32767, "too many blocks for one conversion");
         return true;
     }, [&] {
         const ConvertArgs a{pairs, ids, wide_ids, n, valid, layers, block_size, kv_heads, status};
-        const int64_t ctas = (2 * n * layers * kv_heads + 7) / 8;
+        const dim3 grid(unsigned((n * kv_heads + 7) / 8), unsigned(2 * layers));
         by_type(type, head_dim, [&](auto t, auto d) {
             using T = decltype(t);
             constexpr int D = decltype(d)::value;
             const auto s = reinterpret_cast<cudaStream_t>(stream);
-            if (EXPAND) expand_kernel<T, D><<<unsigned(ctas), 256, 0, s>>>(a);
-            else compress_kernel<T, D><<<unsigned(ctas), 256, 0, s>>>(a);
+            if (EXPAND) expand_kernel<T, D><<<grid, 256, 0, s>>>(a);
+            else compress_kernel<T, D><<<grid, 256, 0, s>>>(a);
         });
         check(cudaGetLastError());
     });

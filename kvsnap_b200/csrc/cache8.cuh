@@ -55,6 +55,17 @@ struct Fp16 {
     }
 };
 
+constexpr int kGranule = 16;               // tokens that always lie in one page
+
+// 16 bytes, or zeros, predicated: where a branch around a load joins, the load is waited for.
+__device__ __forceinline__ uint4 fetch16(const char* at, bool there) {
+    uint4 v;
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %5, 0;\nmov.u32 %0, 0;\nmov.u32 %1, 0;\nmov.u32 %2, 0;\nmov.u32 %3, 0;\n"
+                 "@p ld.global.v4.u32 {%0,%1,%2,%3}, [%4];\n}"
+                 : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w) : "l"(at), "r"(uint32_t(there)));
+    return v;
+}
+
 // 8 consecutive 16-bit elements.
 template <typename T>
 __device__ __forceinline__ void widen8(const uint4& x, float (&v)[8]) {
@@ -82,15 +93,18 @@ __device__ __forceinline__ float2 from_e4m3x2(uint32_t v) {
     return __half22float2(__half2(h));
 }
 
-// 8 consecutive codes, times `by`.
-__device__ __forceinline__ void load_codes(const char* at, float by, float (&v)[8]) {
-    const uint2 x = *reinterpret_cast<const uint2*>(at);
+// 8 codes, times `by`.
+__device__ __forceinline__ void widen_codes(uint2 x, float by, float (&v)[8]) {
     const uint32_t w[4] = {x.x & 0xFFFFu, x.x >> 16, x.y & 0xFFFFu, x.y >> 16};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float2 p = from_e4m3x2(w[i]);
         v[2 * i] = p.x * by, v[2 * i + 1] = p.y * by;
     }
+}
+
+__device__ __forceinline__ void load_codes(const char* at, float by, float (&v)[8]) {
+    widen_codes(*reinterpret_cast<const uint2*>(at), by, v);
 }
 
 // Nearest codes of v * by (ties to even); beyond +-448, infinities included, +-448.
