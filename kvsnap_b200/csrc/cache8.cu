@@ -12,9 +12,9 @@ struct AppendArgs {
     Batch b;
     Rows key, value, query;
     char* query_out;
-    const float2* rotary;     // [positions][rotary_dim / 2] (cos, sin); NULL: no rotation
+    const float2* rotary;     // [positions][rotary_dim / 2] (cos, sin)
     int64_t positions;
-    int rotary_dim, q_heads;
+    int rotary_dim, q_heads;  // 0: no rotation; no queries
     uint32_t* status;
 };
 
@@ -61,48 +61,43 @@ __device__ __forceinline__ bool find_page(const Batch& b, int n, int64_t u, Page
     return true;
 }
 
-// 8 consecutive elements [at, at + 8) of a head's row, rotated. What they take from memory:
-struct Turned {
-    uint4 own, other;         // the elements, and those that they are turned with
-    float4 turn[4];           // (cos, sin) of their pairs
+// (cos, sin) of the pairs of elements [at, at + 8) of a row.
+struct Turn {
+    uint4 x[4];
 };
 
 template <bool INTERLEAVED>
-__device__ __forceinline__ void fetch_turned(Turned& x, const char* row, int at, const float2* turn, int rotary_dim,
-                                             bool there) {
-    const bool turned = there && at < rotary_dim;
-    x.own = fetch16(row + 2 * at, there);
-    const int half = rotary_dim / 2;
-    const int pair = INTERLEAVED ? at / 2 : at < half ? at : at - half;
-    if (!INTERLEAVED) x.other = fetch16(row + 2 * (at < half ? at + half : at - half), turned);
+__device__ __forceinline__ void fetch_turn(Turn& turn, const AppendArgs& a, int64_t position, int at, bool there) {
+    const int half = a.rotary_dim / 2, pair = INTERLEAVED ? at / 2 : at < half ? at : at - half;
+    const char* from = reinterpret_cast<const char*>(a.rotary + min(position, a.positions - 1) * half + pair);
 #pragma unroll
-    for (int i = 0; i < (INTERLEAVED ? 2 : 4); ++i) {
-        const uint4 t = fetch16(reinterpret_cast<const char*>(turn + pair + 2 * i), turned);
-        x.turn[i] = make_float4(__uint_as_float(t.x), __uint_as_float(t.y), __uint_as_float(t.z), __uint_as_float(t.w));
-    }
+    for (int i = 0; i < (INTERLEAVED ? 2 : 4); ++i) turn.x[i] = fetch16(from + 16 * i, there && at < a.rotary_dim);
 }
 
+// 8 consecutive elements [at, at + 8) of a head's row, rotated (rotary_dim 0: as they are). The lane `mate`
+// has the elements that they are turned with; every lane of the warp is here.
 template <typename T, bool INTERLEAVED>
-__device__ __forceinline__ void turn8(const Turned& x, int at, int rotary_dim, float (&v)[8]) {
-    widen8<T>(x.own, v);
-    if (at >= rotary_dim) return;
+__device__ __forceinline__ void turn8(const uint4& own, const Turn& turn, int at, int rotary_dim, int mate,
+                                      float (&v)[8]) {
+    widen8<T>(own, v);
+    const float* cs = reinterpret_cast<const float*>(turn.x);
     if (INTERLEAVED) {
+        if (at >= rotary_dim) return;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float c = i % 2 ? x.turn[i / 2].z : x.turn[i / 2].x, s = i % 2 ? x.turn[i / 2].w : x.turn[i / 2].y;
-            const float a = v[2 * i], b = v[2 * i + 1];
-            v[2 * i] = a * c - b * s;
-            v[2 * i + 1] = b * c + a * s;
+            const float p = v[2 * i], q = v[2 * i + 1];
+            v[2 * i] = p * cs[2 * i] - q * cs[2 * i + 1];
+            v[2 * i + 1] = q * cs[2 * i] + p * cs[2 * i + 1];
         }
     } else {
+        const uint4 other = make_uint4(__shfl_sync(~0u, own.x, mate), __shfl_sync(~0u, own.y, mate),
+                                       __shfl_sync(~0u, own.z, mate), __shfl_sync(~0u, own.w, mate));
+        if (at >= rotary_dim) return;
         const float sign = at < rotary_dim / 2 ? -1.0f : 1.0f;
         float w[8];
-        widen8<T>(x.other, w);
+        widen8<T>(other, w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float c = i % 2 ? x.turn[i / 2].z : x.turn[i / 2].x, s = i % 2 ? x.turn[i / 2].w : x.turn[i / 2].y;
-            v[i] = v[i] * c + sign * (w[i] * s);
-        }
+        for (int i = 0; i < 8; ++i) v[i] = v[i] * cs[2 * i] + sign * (w[i] * cs[2 * i + 1]);
     }
 }
 
@@ -131,49 +126,49 @@ __device__ __forceinline__ float largest(const uint4 (&raw)[kHeld]) {
     return top;
 }
 
-// One warp: one page of one key or value head, or its query rows of one query head. A row is D / 8 lanes
-// of 8 elements, so a warp takes 256 / D rows a step. Bound by memory: loads are issued for several steps
-// before any is waited for, and predicated (where a branch around a load joins, the load is waited for).
-// Keys are read twice, the second time from the L1 or L2: rotated they would take twice the registers.
+// One CTA: a page, and 8 key or value heads, a warp each, or 8 query heads, of which each warp has some
+// rows (of a single row, a head). A row is D / 8 lanes of 8 elements, so a warp takes 256 / D rows a step. Bound by memory: a warp's
+// loads are issued together (4 KB of keys or values, 2 KB of queries), and predicated. A row's angles are
+// fetched once for 8 query heads. Keys are held as they come and turned twice, for the scale and for the
+// codes: turned they would take twice the registers.
 template <typename T, int D, bool SINGLE, bool INTERLEAVED>
 __global__ void __launch_bounds__(256, 3) append_kernel(const __grid_constant__ AppendArgs a) {
-    constexpr int kLanes = D / 8, kRows = 32 / kLanes, kSteps = SINGLE ? 1 : 2;
+    constexpr int kLanes = D / 8, kRows = 32 / kLanes, kTogether = SINGLE ? 1 : 4;
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, n = a.c.block_size;
-    const int slot = blockIdx.y * 8 + warp;
-    if (slot >= 2 * a.c.kv_heads + a.q_heads) return;
+    const int kv_ctas = (2 * a.c.kv_heads + 7) / 8, slot = blockIdx.y * 8 + warp;
+    const bool queries = blockIdx.y >= kv_ctas;
+    if (!queries && slot >= 2 * a.c.kv_heads) return;
     PageRun run;
     if (!find_page<SINGLE>(a.b, n, blockIdx.x, run, a.status)) return;
     const int sub = lane / kLanes, at = lane % kLanes * 8, end = run.first + run.count;
-    const int base = run.page * n;                                     // position of the page's slot 0
-    const int rotary_dim = a.rotary ? a.rotary_dim : 0;
-    if (a.rotary && base + end > a.positions && lane == 0) atomicOr(a.status, KVSNAP_C8_BAD_POSITION);
+    const int64_t base = int64_t(run.page) * n;                        // position of the page's slot 0
+    if (a.rotary_dim && base + end > a.positions && threadIdx.x == 0) atomicOr(a.status, KVSNAP_C8_BAD_POSITION);
+    const int reach = a.rotary_dim / 16;                               // lanes to the other half of a pair
+    const int mate = at >= a.rotary_dim ? lane : at < a.rotary_dim / 2 ? lane + reach : lane - reach;
 
-    // Turned rows [run.first + sub, end), kSteps at a time, to `each`.
-    const auto for_turned = [&](const char* rows, int64_t pitch, auto each) {
-        for (int r = run.first + sub; r - sub < end; r += kSteps * kRows) {
-            Turned x[kSteps];
+    if (queries) {
+        // (one row: a head a warp)
+        const int head = (blockIdx.y - kv_ctas) * 8 + (SINGLE ? warp : 0), heads = min(SINGLE ? 1 : 8, a.q_heads - head);
+        for (int first = run.first + (SINGLE ? 0 : warp * kRows); first < end; first += 8 * kRows) {
+            const int r = first + sub;
+            const int64_t row = run.row + (r - run.first);
+            const char* from = a.query.at + row * a.query.token + head * a.query.head + 2 * at;
+            char* to = a.query_out + (row * a.q_heads + head) * (2 * D) + 2 * at;
+            Turn turn;
+            fetch_turn<INTERLEAVED>(turn, a, base + r, at, r < end);
+            for (int h = 0; h < heads; h += kTogether) {
+                uint4 raw[kTogether];
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-                const int row = r + i * kRows;
-                const int64_t position = min(int64_t(base + row), a.positions - 1);
-                fetch_turned<INTERLEAVED>(x[i], rows + (run.row + (row - run.first)) * pitch, at,
-                                          a.rotary + position * (rotary_dim / 2), rotary_dim, row < end);
-            }
+                for (int i = 0; i < kTogether; ++i)
+                    raw[i] = fetch16(from + (h + i) * a.query.head, r < end && h + i < heads);
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-                float v[8];
-                turn8<T, INTERLEAVED>(x[i], at, rotary_dim, v);
-                if (r + i * kRows < end) each(r + i * kRows, v);
+                for (int i = 0; i < kTogether; ++i) {
+                    float v[8];
+                    turn8<T, INTERLEAVED>(raw[i], turn, at, a.rotary_dim, mate, v);
+                    if (r < end && h + i < heads) store8<T>(to + (h + i) * (2 * D), v);
+                }
             }
         }
-    };
-
-    if (slot >= 2 * a.c.kv_heads) {
-        const int head = slot - 2 * a.c.kv_heads;
-        char* out = a.query_out + (int64_t(run.row) * a.q_heads + head) * (2 * D) + 2 * at;
-        for_turned(a.query.at + head * a.query.head, a.query.token, [&](int r, const float (&v)[8]) {
-            store8<T>(out + int64_t(r - run.first) * a.q_heads * (2 * D), v);
-        });
         return;
     }
 
@@ -186,42 +181,48 @@ __global__ void __launch_bounds__(256, 3) append_kernel(const __grid_constant__ 
     char* codes = reinterpret_cast<char*>(a.c.codes) + side * a.c.side_pitch + block * a.c.block_pitch +
                   head * a.c.head_pitch + at;
     float* scale_at = reinterpret_cast<float*>(a.c.scales) + (block * 2 + side) * a.c.kv_heads + head;
+    const Rows& from = side ? a.value : a.key;
+    const char* rows = from.at + head * from.head + 2 * at + (run.row - run.first) * from.token;
     const float held = run.first ? *scale_at : 0.0f;
-    float scale, by;
-    if (side == 0) {
-        const char* rows = a.key.at + head * a.key.head;
-        float top = 0.0f;
-        for_turned(rows, a.key.token, [&](int, const float (&v)[8]) { top = max8(v, top); });
-        scale = fmaxf(held, needed_scale(warp_max(top))), by = inverse(scale);
-        for_turned(rows, a.key.token, [&](int r, const float (&v)[8]) { store_codes(codes + r * a.c.token_pitch, v, by); });
-    } else {
-        const char* rows = a.value.at + head * a.value.head + 2 * at - run.first * a.value.token;
-        uint4 raw[kHeld];
-        float top = 0.0f;
-        for (int first = run.first + kHeld * kRows; first < end; first += kHeld * kRows) {     // rows too many to hold
-#pragma unroll
-            for (int i = 0; i < kHeld; ++i) {
-                const int r = first + i * kRows + sub;
-                raw[i] = fetch16(rows + (run.row + int64_t(r)) * a.value.token, r < end);
-            }
-            top = fmaxf(top, largest<T>(raw));
-        }
-#pragma unroll
-        for (int i = 0; i < kHeld; ++i) {
-            const int r = run.first + i * kRows + sub;
-            raw[i] = fetch16(rows + (run.row + int64_t(r)) * a.value.token, r < end);
-        }
-        scale = fmaxf(held, needed_scale(fmaxf(top, largest<T>(raw)))), by = inverse(scale);
+    uint4 raw[kHeld];
+    float top = 0.0f, scale = 0.0f, by = 0.0f;
+    const bool turned = side == 0 && a.rotary_dim;
+    // The largest size of all rows, then their codes; rows too many to hold are fetched twice.
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {
         for (int first = run.first; first < end; first += kHeld * kRows) {
+            if (pass == 0 || run.count > kHeld * kRows) {
 #pragma unroll
-            for (int i = 0; i < kHeld; ++i) {
-                const int r = first + i * kRows + sub;
-                if (first > run.first) raw[i] = fetch16(rows + (run.row + int64_t(r)) * a.value.token, r < end);
-                float v[8];
-                widen8<T>(raw[i], v);
-                if (r < end) store_codes(codes + r * a.c.token_pitch, v, by);
+                for (int i = 0; i < kHeld; ++i) {
+                    const int r = first + i * kRows + sub;
+                    raw[i] = fetch16(rows + r * from.token, r < end);
+                }
+            }
+            if (turned) {
+#pragma unroll
+                for (int i = 0; i < kHeld; ++i) {
+                    const int r = first + i * kRows + sub;
+                    if (first + i * kRows >= end) break;
+                    Turn turn;
+                    float v[8];
+                    fetch_turn<INTERLEAVED>(turn, a, base + r, at, r < end);
+                    turn8<T, INTERLEAVED>(raw[i], turn, at, a.rotary_dim, mate, v);
+                    if (pass == 0) top = max8(v, top);
+                    else if (r < end) store_codes(codes + r * a.c.token_pitch, v, by);
+                }
+            } else if (pass == 0) {
+                top = fmaxf(top, largest<T>(raw));
+            } else {
+#pragma unroll
+                for (int i = 0; i < kHeld; ++i) {
+                    const int r = first + i * kRows + sub;
+                    float v[8];
+                    widen8<T>(raw[i], v);
+                    if (r < end) store_codes(codes + r * a.c.token_pitch, v, by);
+                }
             }
         }
+        if (pass == 0) scale = fmaxf(held, needed_scale(warp_max(top))), by = inverse(scale);
     }
     if (!run.first || scale > held) {
         for (int r = sub; r < run.first; r += kRows) {                 // older tokens, at the grown scale
@@ -359,10 +360,10 @@ extern "C" int kvsnap_c8_append(const kvsnap_c8_cache* cache, const kvsnap_c8_ba
                            {static_cast<const char*>(value), value_token, value_head},
                            {static_cast<const char*>(query), query_token, query_head},
                            static_cast<char*>(query_out), reinterpret_cast<const float2*>(rotary), positions,
-                           rotary_dim, query ? q_heads : 0, status};
+                           rotary ? rotary_dim : 0, query ? q_heads : 0, status};
         const bool single = batch->max_query <= 1;
         const int64_t units = single ? batch->seqs : batch->rows / cache->block_size + 2LL * batch->seqs;
-        const dim3 grid(unsigned(units), unsigned((2 * cache->kv_heads + a.q_heads + 7) / 8));
+        const dim3 grid(unsigned(units), unsigned((2 * cache->kv_heads + 7) / 8 + (a.q_heads + 7) / 8));
         by_type(type, cache->head_dim, [&](auto t, auto d) {
             using T = decltype(t);
             constexpr int D = decltype(d)::value;
