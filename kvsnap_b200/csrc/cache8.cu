@@ -53,7 +53,7 @@ __device__ __forceinline__ bool find_page(const Batch& b, int n, int64_t u, Page
     const int held = max(length - (to - from), 0);        // tokens before the new ones
     run.seq = s;
     run.page = held / n + k;
-    const int64_t base = int64_t(run.page) * n;
+    const int base = run.page * n;
     if (base >= length) return false;
     run.first = k ? 0 : held - int(base);
     run.count = min(n, int(length - base)) - run.first;
@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(256, 3) append_kernel(const __grid_constant__ 
     PageRun run;
     if (!find_page<SINGLE>(a.b, n, blockIdx.x, run, a.status)) return;
     const int sub = lane / kLanes, at = lane % kLanes * 8, end = run.first + run.count;
-    const int64_t base = int64_t(run.page) * n;                        // position of the page's slot 0
+    const int base = run.page * n;                               // position of the page's slot 0
     if (a.rotary_dim && base + end > a.positions && threadIdx.x == 0) atomicOr(a.status, KVSNAP_C8_BAD_POSITION);
     const int reach = a.rotary_dim / 16;                               // lanes to the other half of a pair
     const int mate = at >= a.rotary_dim ? lane : at < a.rotary_dim / 2 ? lane + reach : lane - reach;
