@@ -46,12 +46,20 @@ def rotary_table(positions, rotary_dim, base=10000.0, *, device="cuda"):
     return torch.stack((angle.cos(), angle.sin()), dim=-1).to(torch.float32)
 
 
-def _type_of(tensor):
+def _type_of(dtype):
     import torch
-    kinds = {torch.bfloat16: _abi.C8_BF16, torch.float16: _abi.C8_FP16}
-    if tensor.dtype not in kinds:
-        raise ValueError(f"16-bit rows are bfloat16 or float16, not {tensor.dtype}")
-    return kinds[tensor.dtype]
+    if dtype is torch.bfloat16:
+        return _abi.C8_BF16
+    if dtype is torch.float16:
+        return _abi.C8_FP16
+    raise ValueError(f"16-bit rows are bfloat16 or float16, not {dtype}")
+
+
+def _raw_stream():
+    """The function from a device's index to its current stream's handle."""
+    import torch
+    # current_stream() makes a Stream object a call, 2.3 us of a 12 us append.
+    return getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
 class PagedBatch:
@@ -80,14 +88,18 @@ class PagedBatch:
             raise ValueError("max_query must be a non-negative int")
         self.table, self.start, self.lengths, self.max_query = table, start, lengths, max_query
         self.device, self.seqs = table.device, seqs
-        self._record = _abi.C8Batch(table=table.data_ptr(), start=start.data_ptr(), lengths=lengths.data_ptr(),
-                                    table_pitch=table.stride(0), width=table.shape[1], seqs=seqs)
+        self._addresses = (table.data_ptr(), start.data_ptr(), lengths.data_ptr(), table.stride(0), table.shape[1], seqs)
+        self._records, self._workspaces = {}, {}
 
     def _for(self, rows):
-        record = self._record
-        limit = rows if self.max_query is None else self.max_query
-        return _abi.C8Batch(record.table, record.start, record.lengths, record.table_pitch, record.width, record.seqs,
-                            rows, limit)
+        """The call's record for tensors of ``rows`` rows (a few row counts are kept: they are the caller's steps)."""
+        record = self._records.get(rows)
+        if record is None:
+            if len(self._records) > 64:
+                self._records.clear()
+            record = _abi.C8Batch(*self._addresses, rows, rows if self.max_query is None else self.max_query)
+            self._records[rows] = record
+        return record
 
 
 class PagedCache8:
@@ -130,10 +142,11 @@ class PagedCache8:
                 raise ValueError(f"layer {name}: codes must have a contiguous head_dim and 16-byte aligned strides")
             self._records[name] = _abi.C8Cache(tensor.data_ptr(), scale.data_ptr(), *pitches[:4], tensor.shape[1],
                                                *shape[2:], self.device.index, 0)
-        self._lib = _dp(_load())
+        self._lib, self._current_stream, self._index = _dp(_load()), _raw_stream(), first.device.index
         if not hasattr(self._lib, "kvsnap_c8_append"):
             raise RuntimeError("the CUDA library has no 8-bit cache kernels; rebuild with python -m kvsnap_b200.build")
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._status_at = self.status.data_ptr()
 
     @classmethod
     def allocate(cls, layers, blocks, block_size, kv_heads, head_dim, *, device="cuda"):
@@ -155,15 +168,16 @@ class PagedCache8:
         """(address, token pitch, head pitch) in bytes of ``[rows, heads, head_dim]`` 16-bit rows."""
         if tensor.device != self.device:
             raise ValueError(f"{what} must be on {self.device}")
-        if tensor.ndim != 3 or tensor.shape[2] != self.head_dim or (heads and tensor.shape[1] != heads):
+        shape = tensor.shape
+        if len(shape) != 3 or shape[2] != self.head_dim or (heads and shape[1] != heads):
             raise ValueError(f"{what} must be [rows, {heads or 'heads'}, {self.head_dim}]")
         token, head, element = tensor.stride()
         at = tensor.data_ptr()
         if element != 1 or token < 0 or head < 0:
             raise ValueError(f"{what} must have a contiguous head_dim")
-        token = 2 * token if tensor.shape[0] > 1 else 0      # an axis of one element is never stepped along
-        head = 2 * head if tensor.shape[1] > 1 else 0
-        if at % 16 or token % 16 or head % 16:
+        token = 2 * token if shape[0] > 1 else 0             # an axis of one element is never stepped along
+        head = 2 * head if shape[1] > 1 else 0
+        if (at | token | head) & 15:
             raise ValueError(f"{what} must be 16-byte aligned in every row")
         return at, token, head
 
@@ -171,10 +185,6 @@ class PagedCache8:
         if batch.device != self.device:
             raise ValueError(f"the batch must be on {self.device}")
         return batch._for(rows)
-
-    def _stream(self):
-        import torch
-        return torch.cuda.current_stream(self.device).cuda_stream
 
     def _check(self, rc):
         if rc < 0:
@@ -196,35 +206,39 @@ class PagedCache8:
         the page's scale holds; NaN stays NaN; neither sets a scale.
         """
         import torch
-        cache = self._layer(layer)
-        rows = key.shape[0]
-        kind = _type_of(key)
+        cache, dtype = self._layer(layer), key.dtype
+        rows, kind = key.shape[0], _type_of(dtype)
         k, v = self._rows("key", key, self.kv_heads), self._rows("value", value, self.kv_heads)
-        if value.dtype != key.dtype or value.shape[0] != rows:
+        if value.dtype is not dtype or value.shape[0] != rows:
             raise ValueError("key and value must have the same rows and type")
-        q, q_heads, out = (None, 0, 0), 0, None
+        q, q_heads, out, out_at = (None, 0, 0), 0, None, None
         if query is not None:
-            q = self._rows("query", query)
-            if query.dtype != key.dtype or query.shape[0] != rows or not query.shape[1]:
+            q, shape = self._rows("query", query), query.shape
+            if query.dtype is not dtype or shape[0] != rows or not shape[1]:
                 raise ValueError("query must have the keys' rows and type, and at least one head")
-            q_heads = query.shape[1]
+            q_heads = shape[1]
         table, positions, rotary_dim = None, 0, 0
         if rotary is not None:
-            if rotary.dtype != torch.float32 or rotary.ndim != 3 or rotary.shape[2] != 2 or rotary.device != self.device \
+            if rotary.dtype is not torch.float32 or rotary.ndim != 3 or rotary.device != self.device \
                     or not rotary.is_contiguous():
                 raise ValueError(f"rotary must be a contiguous float32 [positions, rotary_dim / 2, 2] on {self.device}")
-            table, positions, rotary_dim = rotary.data_ptr(), rotary.shape[0], 2 * rotary.shape[1]
+            positions, half, two = rotary.shape
+            table, rotary_dim = rotary.data_ptr(), 2 * half
+            if two != 2:
+                raise ValueError("rotary must hold (cos, sin) in its last axis")
             if rotary_dim <= 0 or rotary_dim % 16 or rotary_dim > self.head_dim or not positions:
                 raise ValueError("rotary_dim must be a multiple of 16 up to head_dim, for at least one position")
             if table % 16:
                 raise ValueError("rotary must be 16-byte aligned")
         elif query is not None:
             raise ValueError("query is only rotated: it needs rotary")
+        record = self._batch(batch, rows)
         if query is not None:
-            out = torch.empty(query.shape, dtype=query.dtype, device=self.device)
-        self._check(self._lib.kvsnap_c8_append(cache, self._batch(batch, rows), kind, *k, *v, *q, q_heads,
-                                               0 if out is None else out.data_ptr(), table, positions, rotary_dim,
-                                               bool(interleaved), self.status.data_ptr(), self._stream()))
+            out = torch.empty_like(query, memory_format=torch.contiguous_format)
+            out_at = out.data_ptr()
+        self._check(self._lib.kvsnap_c8_append(cache, record, kind, *k, *v, *q, q_heads, out_at, table, positions,
+                                               rotary_dim, bool(interleaved), self._status_at,
+                                               self._current_stream(self._index)))
         return out
 
     def attend(self, layer, query, batch, *, scale=None, out=None):
@@ -237,27 +251,36 @@ class PagedCache8:
         without it). Sums and the softmax's statistics are 32-bit; weights and cached values meet in 16 bits.
         """
         import torch
-        cache = self._layer(layer)
-        kind, q = _type_of(query), self._rows("query", query)
-        rows, q_heads = query.shape[:2]
+        cache, dtype, shape = self._layer(layer), query.dtype, query.shape
+        kind, q = _type_of(dtype), self._rows("query", query)
+        rows, q_heads, _ = shape
         if not q_heads or q_heads % self.kv_heads:
             raise ValueError("query heads must be a multiple of the KV heads")
-        if out is None:
-            out = torch.empty(query.shape, dtype=query.dtype, device=self.device)
-        elif out.shape != query.shape or out.dtype != query.dtype or out.device != self.device or not out.is_contiguous():
-            raise ValueError("out must be a contiguous tensor of the query's shape, type and device")
-        elif out.data_ptr() % 16:
-            raise ValueError("out must be 16-byte aligned")
         scale = self.head_dim ** -0.5 if scale is None else float(scale)
         if not 0.0 <= scale < 3.4e38:
             raise ValueError("scale must be finite and not negative")
-        record, size = self._batch(batch, rows), C.c_size_t()
-        self._check(self._lib.kvsnap_c8_attend_workspace(cache, record, q_heads, size))
+        if out is not None:
+            if out.shape != shape or out.dtype is not dtype or out.device != self.device or not out.is_contiguous():
+                raise ValueError("out must be a contiguous tensor of the query's shape, type and device")
+            if out.data_ptr() % 16:
+                raise ValueError("out must be 16-byte aligned")
+        record = self._batch(batch, rows)
+        # What a call of these sizes needs is asked once.
+        sizes = (rows, q_heads, self.kv_heads, self.head_dim, self.block_size)
+        size = batch._workspaces.get(sizes)
+        if size is None:
+            needed = C.c_size_t()
+            self._check(self._lib.kvsnap_c8_attend_workspace(cache, record, q_heads, needed))
+            if len(batch._workspaces) > 64:
+                batch._workspaces.clear()
+            size = batch._workspaces[sizes] = needed.value
+        if out is None:
+            out = torch.empty_like(query, memory_format=torch.contiguous_format)
         # A workspace of the call's own, from the stream's (or the capture's) memory: no two calls share one.
-        workspace = torch.empty(size.value, dtype=torch.uint8, device=self.device) if size.value else None
+        workspace = self.status.new_empty(size // 4) if size else None
         self._check(self._lib.kvsnap_c8_attend(cache, record, kind, *q, q_heads, scale, out.data_ptr(),
-                                               workspace.data_ptr() if size.value else None, size.value,
-                                               self.status.data_ptr(), self._stream()))
+                                               workspace.data_ptr() if size else None, size, self._status_at,
+                                               self._current_stream(self._index)))
         return out
 
     def converter(self, caches):
@@ -294,7 +317,7 @@ class CacheConverter:
                 raise ValueError("one CUDA device required")
             if wide.ndim != 5 or wide.shape[0] != 2 or tuple(wide.shape[2:]) != geometry:
                 raise ValueError(f"layer {name}: 16-bit cache must be [2, blocks, {geometry[0]}, {geometry[1]}, {geometry[2]}]")
-            kinds.add(_type_of(wide))
+            kinds.add(_type_of(wide.dtype))
             pitches = [2 * p for p in wide.stride()]
             if pitches[4] != 2 or wide.data_ptr() % 16 or any(p % 16 or p < 0 for p in pitches[:4]):
                 raise ValueError(f"layer {name}: 16-bit cache must have a contiguous head_dim and 16-byte aligned strides")
@@ -308,24 +331,25 @@ class CacheConverter:
             raise ValueError("16-bit caches must have one type")
         self._kind = kinds.pop()
         self._pairs = torch.frombuffer(bytearray(bytes(pairs)), dtype=torch.uint8).to(cache.device)
+        self._pairs_at = self._pairs.data_ptr()
 
     def _ids(self, ids):
         import torch
         if not isinstance(ids, torch.Tensor):
             ids = torch.tensor(list(ids), dtype=torch.int64).to(self.cache.device)
-        if ids.dtype != torch.int64 or ids.ndim != 1 or ids.device != self.cache.device or not ids.is_contiguous():
+        if ids.dtype is not torch.int64 or ids.ndim != 1 or ids.device != self.cache.device or not ids.is_contiguous():
             raise ValueError(f"block ids are a list or a contiguous 1-D int64 tensor on {self.cache.device}")
         return ids
 
     def _call(self, entry, source, target, *valid):
-        source, target = self._ids(source), self._ids(target)
-        if source.numel() != target.numel():
-            raise ValueError("one source per block is required")
         cache = self.cache
-        cache._check(getattr(cache._lib, entry)(self._pairs.data_ptr(), len(self.caches), cache.block_size,
-                                                cache.kv_heads, cache.head_dim, self._kind, source.data_ptr(),
-                                                target.data_ptr(), source.numel(), *valid, cache.status.data_ptr(),
-                                                cache.device.index, cache._stream()))
+        source, target = self._ids(source), self._ids(target)
+        count = source.shape[0]
+        if target.shape[0] != count:
+            raise ValueError("one source per block is required")
+        cache._check(entry(self._pairs_at, len(self.caches), cache.block_size, cache.kv_heads, cache.head_dim, self._kind,
+                           source.data_ptr(), target.data_ptr(), count, *valid, cache._status_at, cache._index,
+                           cache._current_stream(cache._index)))
 
     def compress(self, source_blocks, blocks, num_kv_tokens=None):
         """16-bit blocks ``source_blocks[i]`` into 8-bit blocks ``blocks[i]``, with new scales.
@@ -336,9 +360,9 @@ class CacheConverter:
         """
         if num_kv_tokens is not None and (type(num_kv_tokens) is not int or num_kv_tokens < 0):
             raise ValueError("num_kv_tokens must be a non-negative int")
-        self._call("kvsnap_c8_compress", source_blocks, blocks, -1 if num_kv_tokens is None else num_kv_tokens)
+        self._call(self.cache._lib.kvsnap_c8_compress, source_blocks, blocks, -1 if num_kv_tokens is None else num_kv_tokens)
 
     def expand(self, blocks, target_blocks):
         """8-bit blocks ``blocks[i]`` into 16-bit blocks ``target_blocks[i]``: exact in bfloat16 up to its
         smallest normal number, rounded once in float16."""
-        self._call("kvsnap_c8_expand", blocks, target_blocks)
+        self._call(self.cache._lib.kvsnap_c8_expand, blocks, target_blocks)

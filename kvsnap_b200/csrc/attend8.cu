@@ -71,6 +71,21 @@ struct SharedUnit {
     int parts;                // CTAs that share it, from this one on; 0: none
 };
 
+// Work of `total`, cut evenly over at most `most` CTAs (a piece of at least 1 each).
+struct Cut {
+    uint32_t ctas, each, more;     // pieces of each + 1, then of each
+
+    __device__ __forceinline__ Cut(uint32_t total, uint32_t most) : ctas(min(total, most)) {
+        each = ctas ? total / ctas : 0, more = ctas ? total % ctas : 0;
+    }
+    __device__ __forceinline__ uint32_t begin(uint32_t cta) const { return cta * each + min(cta, more); }
+    // The CTA that place `at` is of.
+    __device__ __forceinline__ uint32_t of(uint32_t at) const {
+        const uint32_t long_ones = more * (each + 1);
+        return at < long_ones ? at / (each + 1) : more + (at - long_ones) / each;
+    }
+};
+
 struct Parts {
     float* sums;              // [2 * CTAs][slot rows][D]
     float2* ml;               // their maxima and weights' sums
@@ -97,6 +112,7 @@ struct Parts {
 
 constexpr int kStepRows = 16;
 constexpr int kWarps = 16;                 // a CTA: HC heads x TS slices of a chunk
+constexpr int kSpread = 48;                // units of few sequences that heads are spread for
 constexpr int kAhead = 3;                  // granules a warp holds: one in use, the others on their way
 constexpr float kLowest = -3e38f;          // the running maximum before any token
 constexpr float kSlack = 14.0f;            // log2 by which a weight may exceed 1 before sums are rescaled (fp16: 2^16)
@@ -173,17 +189,6 @@ __device__ __forceinline__ int chunks_of(const StepArgs& p, int s, Sequence& q) 
     return max(1, (q.length + p.ts * kGranule - 1) / (p.ts * kGranule));
 }
 
-__device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* scratch) {
-#pragma unroll
-    for (int k = 16; k; k >>= 1) v += __shfl_xor_sync(~0u, v, k);
-    if (threadIdx.x % 32 == 0) scratch[threadIdx.x / 32] = v;
-    __syncthreads();
-    v = 0;
-    for (int w = 0; w < int(blockDim.x) / 32; ++w) v += scratch[w];
-    __syncthreads();
-    return v;
-}
-
 // One warp's share of chunks [c0, c1) of one head of one sequence.
 template <typename T, int D, int NT>
 struct StepWarp {
@@ -207,54 +212,6 @@ struct StepWarp {
             for (int mt = 0; mt < kTiles; ++mt)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) o[nt][mt][i] = 0.0f;
-        }
-
-        // Queries as fp16, each row times a power of two that brings its largest element to
-        // [2^14, 2^15): bf16's exponents do not fit fp16, and what then falls below fp16's
-        // normal numbers is under 2^-28 of the row's largest.
-        uint32_t qb[NT][kHalves * 4][2];
-        float factor[NT][2];               // of rows 8 nt + 2 t, + 1: scores' factor
-        int seen[NT][2];                   // tokens that those rows see
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int r = nt * 8 + g;
-            float v[kHalves][16], top = 0.0f;
-#pragma unroll
-            for (int half = 0; half < kHalves; ++half) {
-                if (r < rows) {
-                    const char* at = p.a.query.at + int64_t(q.row + r / p.a.group) * p.a.query.token +
-                                     int64_t(head * p.a.group + r % p.a.group) * p.a.query.head + 128 * half + 32 * t;
-                    float w[8];
-                    load8<T>(at, w);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[half][i] = w[i];
-                    load8<T>(at + 16, w);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[half][8 + i] = w[i];
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) v[half][i] = 0.0f;
-                }
-#pragma unroll
-                for (int i = 0; i < 16; ++i) top = fmaxf(top, finite_size(v[half][i]));
-            }
-            top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-            const int e = max(int(__float_as_uint(top) >> 23), 27);          // biased
-            const float up = __uint_as_float(uint32_t(127 + 14 + 127 - e) << 23);
-            const float down = __uint_as_float(uint32_t(max(e - 14, 1)) << 23) * p.a.scale;
-#pragma unroll
-            for (int half = 0; half < kHalves; ++half)
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    qb[nt][half * 4 + w][0] = pack_half2(v[half][4 * w] * up, v[half][4 * w + 1] * up);
-                    qb[nt][half * 4 + w][1] = pack_half2(v[half][4 * w + 2] * up, v[half][4 * w + 3] * up);
-                }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                factor[nt][i] = __shfl_sync(~0u, down, (2 * t + i) * 4);
-                seen[nt][i] = first_seen + (nt * 8 + 2 * t + i) / p.a.group;
-            }
         }
 
         const int token_a = 4 * (g >> 1) + (g & 1);                            // of score row g; row g + 8: + 2
@@ -314,6 +271,55 @@ struct StepWarp {
 
 #pragma unroll 1
         for (int i = 0; i < kAhead - 1; ++i) copy();
+
+        // Queries as fp16, each row times a power of two that brings its largest element to
+        // [2^14, 2^15): bf16's exponents do not fit fp16, and what then falls below fp16's
+        // normal numbers is under 2^-28 of the row's largest.
+        uint32_t qb[NT][kHalves * 4][2];
+        float factor[NT][2];               // of rows 8 nt + 2 t, + 1: scores' factor
+        int seen[NT][2];                   // tokens that those rows see
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int r = nt * 8 + g;
+            float v[kHalves][16], top = 0.0f;
+#pragma unroll
+            for (int half = 0; half < kHalves; ++half) {
+                if (r < rows) {
+                    const char* at = p.a.query.at + int64_t(q.row + r / p.a.group) * p.a.query.token +
+                                     int64_t(head * p.a.group + r % p.a.group) * p.a.query.head + 128 * half + 32 * t;
+                    float w[8];
+                    load8<T>(at, w);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[half][i] = w[i];
+                    load8<T>(at + 16, w);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[half][8 + i] = w[i];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) v[half][i] = 0.0f;
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, finite_size(v[half][i]));
+            }
+            top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+            const int e = max(int(__float_as_uint(top) >> 23), 27);          // biased
+            const float up = __uint_as_float(uint32_t(127 + 14 + 127 - e) << 23);
+            const float down = __uint_as_float(uint32_t(max(e - 14, 1)) << 23) * p.a.scale;
+#pragma unroll
+            for (int half = 0; half < kHalves; ++half)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    qb[nt][half * 4 + w][0] = pack_half2(v[half][4 * w] * up, v[half][4 * w + 1] * up);
+                    qb[nt][half * 4 + w][1] = pack_half2(v[half][4 * w + 2] * up, v[half][4 * w + 3] * up);
+                }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                factor[nt][i] = __shfl_sync(~0u, down, (2 * t + i) * 4);
+                seen[nt][i] = first_seen + (nt * 8 + 2 * t + i) / p.a.group;
+            }
+        }
+
         uint32_t at = ring;
         float limit[NT][2], v_by = 0.0f;             // m + kSlack; 1 / vref
 #pragma unroll
@@ -473,9 +479,8 @@ struct StepShared {
     };
     float2 ml[kWarps][8 * NT];
     StepPage pages[kWarps][64];
-    int64_t scratch[kWarps];
-    int64_t prefix[kWarps];
-    int64_t found_first;
+    uint32_t sums[2][kWarps];
+    uint32_t found_first;
     int found;
 };
 
@@ -494,47 +499,62 @@ __global__ void __launch_bounds__(32 * kWarps, 1) step_kernel(const __grid_const
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, seqs = p.a.b.seqs;
     asm volatile("griddepcontrol.launch_dependents;");
 
-    int64_t total = 0, ctas = 0, pos = 0, end = 0;
+    uint32_t pos = 0, end = 1, cut_total = 0;
     int s = 0, hg = 0, c0 = 0;
     Sequence q;
     if (SPLIT) {
         if (threadIdx.x == 0) p.parts.units[blockIdx.x].parts = 0;
-        int64_t mine = 0;
-        for (int i = threadIdx.x; i < seqs; i += blockDim.x) mine += int64_t(chunks_of(p, i, q)) * p.hg;
-        total = block_sum(mine, sh.scratch);
-        ctas = min(int64_t(gridDim.x), total);                     // that have work: a chunk at least
-        if (blockIdx.x >= ctas) return;
-        pos = total * blockIdx.x / ctas, end = total * (blockIdx.x + 1) / ctas;
-        // The sequence that chunk `pos` lies in, and the chunk at which it begins.
-        int64_t before = 0;
-        for (int tile = 0; tile < seqs; tile += blockDim.x) {
-            const int i = tile + threadIdx.x;
-            const int64_t n = i < seqs ? int64_t(chunks_of(p, i, q)) * p.hg : 0;
-            int64_t sum = n;
+        // All chunks; those of up to 512 sequences are summed and found in one pass.
+        uint32_t mine = 0;
+        for (int i = threadIdx.x; i < seqs; i += blockDim.x) mine += chunks_of(p, i, q) * p.hg;
+        uint32_t sum = mine;
 #pragma unroll
-            for (int k = 1; k < 32; k <<= 1) {
-                const int64_t up = __shfl_up_sync(~0u, sum, k);
-                if (lane >= k) sum += up;
-            }
-            if (lane == 31) sh.prefix[warp] = sum;
+        for (int k = 1; k < 32; k <<= 1) {
+            const uint32_t up = __shfl_up_sync(~0u, sum, k);
+            if (lane >= k) sum += up;
+        }
+        if (lane == 31) sh.sums[0][warp] = sum;
+        __syncthreads();
+        uint32_t low = 0;
+        for (int w = 0; w < kWarps; ++w) {
+            if (w == warp) low = cut_total;
+            cut_total += sh.sums[0][w];
+        }
+        const Cut cut(cut_total, gridDim.x);
+        if (blockIdx.x >= cut.ctas) return;
+        pos = cut.begin(blockIdx.x), end = cut.begin(blockIdx.x + 1);
+        if (seqs <= int(blockDim.x)) {
+            const uint32_t first = low + sum - mine;
+            if (mine && first <= pos && pos < first + mine) sh.found = threadIdx.x, sh.found_first = first;
             __syncthreads();
-            int64_t all = 0, low = before;
-            for (int w = 0; w < kWarps; ++w) {
-                if (w == warp) low = before + all;
-                all += sh.prefix[w];
+        } else {
+            uint32_t before = 0;
+            for (int tile = 0; tile < seqs && before <= pos; tile += blockDim.x) {
+                const int i = tile + threadIdx.x;
+                const uint32_t n = i < seqs ? chunks_of(p, i, q) * p.hg : 0;
+                sum = n;
+#pragma unroll
+                for (int k = 1; k < 32; k <<= 1) {
+                    const uint32_t up = __shfl_up_sync(~0u, sum, k);
+                    if (lane >= k) sum += up;
+                }
+                if (lane == 31) sh.sums[1][warp] = sum;
+                __syncthreads();
+                low = before;
+                for (int w = 0; w < kWarps; ++w) {
+                    if (w < warp) low += sh.sums[1][w];
+                    before += sh.sums[1][w];
+                }
+                const uint32_t first = low + sum - n;
+                if (n && first <= pos && pos < first + n) sh.found = i, sh.found_first = first;
+                __syncthreads();
             }
-            const int64_t first = low + sum - n;
-            if (n && first <= pos && pos < first + n) sh.found = i, sh.found_first = first;
-            before += all;
-            __syncthreads();
-            if (before > pos) break;
         }
         s = sh.found;
-        const int n = chunks_of(p, s, q);
-        hg = int((pos - sh.found_first) / n), c0 = int((pos - sh.found_first) % n);
+        const uint32_t n = chunks_of(p, s, q), within = pos - sh.found_first;
+        hg = within / n, c0 = within % n;
     } else {
         s = blockIdx.x / p.hg, hg = blockIdx.x % p.hg;
-        end = 1;
     }
 
     while (pos < end && s < seqs) {
@@ -544,7 +564,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1) step_kernel(const __grid_const
             ++s;
             continue;
         }
-        const int c1 = SPLIT ? int(min(int64_t(chunks), c0 + (end - pos))) : chunks;
+        const int c1 = SPLIT ? min(chunks, c0 + int(end - pos)) : chunks;
         const int rows = q.rows * p.a.group;
         const int hc = warp % p.hc, slice = warp / p.hc;       // a warp without a slice only waits
         StepWarp<T, D, NT> w;
@@ -600,8 +620,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1) step_kernel(const __grid_const
         }
         if (SPLIT) {
             if (!whole && c0 == 0 && threadIdx.x == 0) {
-                const int64_t past = pos + chunks;                             // the unit's end
-                const int last = int((past * ctas - 1) / total);
+                const int last = Cut(cut_total, gridDim.x).of(pos + chunks - 1);       // who ends the unit
                 p.parts.units[blockIdx.x] = SharedUnit{q.row, hg * p.hc, 0, rows, last - int(blockIdx.x) + 1};
             }
             __syncthreads();
@@ -842,7 +861,7 @@ struct ChunkControl {
     uint32_t tensor;                       // tensor memory's address
     volatile int stop;                     // a wait ran out
     int64_t counts[kScanned], scratch[32];
-    int64_t total, ctas, pos, until, base, sought, scanned;      // pos to until: this CTA's part of the total cost
+    int64_t total, pos, until, base, sought, scanned;      // pos to until: this CTA's part of the total cost
     int s, head, tile;
 };
 
@@ -1560,7 +1579,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs& p, ChunkShared<D>&
         if (!whole) {
             if (lane < rows) p.parts.ml[slot + lane] = make_float2(m, l);
             if (begin == 0 && threadIdx.x == 0) {
-                const int last = int((u.stop * sh.c.ctas - 1) / sh.c.total);
+                const int last = Cut(uint32_t(sh.c.total), gridDim.x).of(uint32_t(u.stop - 1));
                 p.parts.units[blockIdx.x] =
                     SharedUnit{u.q.row, u.head, u.first, u.rows, last - int(blockIdx.x) + 1};
             }
@@ -1590,9 +1609,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
     int64_t total = 0;
     for (int w = 0; w < kAll; ++w) total += sh.c.scratch[w];
     total *= a.c.kv_heads;
-    const int64_t ctas = min(int64_t(gridDim.x), total);
-    if (blockIdx.x >= ctas) return;
-    const int64_t pos = total * blockIdx.x / ctas, end = total * (blockIdx.x + 1) / ctas;
+    const Cut cut(uint32_t(total), gridDim.x);
+    if (blockIdx.x >= cut.ctas) return;
+    const int64_t pos = cut.begin(blockIdx.x), end = cut.begin(blockIdx.x + 1);
     int64_t before = 0;
     for (int base = 0; base < seqs; base += kScanned) {
         for (int s = warp; s < kScanned; s += kAll) {
@@ -1667,7 +1686,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
             barrier_init(&sh.c.unit_free[i], 9);         // 8 warps of rows, and the issue
         }
         barrier_init(&sh.c.drained, 1);
-        sh.c.total = total, sh.c.ctas = ctas, sh.c.pos = pos, sh.c.until = end;
+        sh.c.total = total, sh.c.pos = pos, sh.c.until = end;
         for (int i = 0; i < kNanUnits; ++i) sh.c.nan_unit[i] = 0;
         sh.c.stop = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -1739,7 +1758,15 @@ Plan plan_for(const Cache& c, const Batch& b, int q_heads, int sms) {
     plan.stepped = group <= kStepRows && !(plan.chunked && b.seqs == 1);
     plan.step_rows = plan.stepped ? kStepRows : 0;
     plan.wide = most_rows > 8;
-    for (p.hc = c.kv_heads < 8 ? c.kv_heads : 8; c.kv_heads % p.hc; --p.hc) {}
+    // Heads a CTA: up to 8, whose lines of a token lie side by side; but few sequences are spread over CTAs by
+    // heads, so that a unit's tokens are cut among fewer CTAs (with 8, a 32k step of one sequence left 148
+    // parts of each row to join, and a 129-token one was one CTA's).
+    p.hc = 1;
+    for (int heads = 8; heads > 1; --heads)
+        if (c.kv_heads % heads == 0 && int64_t(b.seqs) * (c.kv_heads / heads) >= kSpread) {
+            p.hc = heads;
+            break;
+        }
     p.ts = kWarps / p.hc, p.hg = c.kv_heads / p.hc;
     const int64_t most = (int64_t(b.width) * c.block_size + p.ts * kGranule - 1) / (p.ts * kGranule);
     // Up to 8 chunks a unit, a CTA each: cutting them would cost more (a scan of the lengths,
@@ -1817,6 +1844,12 @@ void check_attend(const Cache* cache, const Batch* batch, int q_heads) {
     require(q_heads > 0 && q_heads % cache->kv_heads == 0, "query heads must be a multiple of the KV heads");
     require(int64_t(batch->seqs) * cache->kv_heads < (1LL << 30) && int64_t(batch->rows) * q_heads < (1LL << 30),
             "too many sequences or rows for one attention");
+    // All the work of a call is counted in 32 bits: granules of each head, steps of each 256 rows and head.
+    const double granules = double(batch->width) * cache->block_size / kGranule + 1;
+    const double units = double(batch->rows) * (q_heads / cache->kv_heads) / kUnitRows + batch->seqs;
+    require(batch->seqs * granules * cache->kv_heads < 2147483648.0 &&
+                units * cache->kv_heads * (granules * kGranule / kStep + kUnitCost + 1) < 2147483648.0,
+            "too much work for one attention");
 }
 
 }  // namespace
