@@ -463,6 +463,21 @@ def _split_paged(caches, block_size):
     return views
 
 
+def _block_views(scales):
+    """Registered views of an 8-bit cache's scales: ``[B, 2, H]`` float32 becomes ``name.scale``, ``[B, 1, 1, 2 H]``.
+
+    One token slot a block, which no tail zeroing reaches: a partly filled
+    block's scales stay.
+    """
+    views = {}
+    for name, tensor in (scales or {}).items():
+        shape = tuple(getattr(tensor, "shape", ()))
+        if len(shape) != 3 or shape[1] != 2 or not tensor.is_contiguous():
+            raise ValueError(f"scales of {name} must be contiguous [blocks, 2, kv_heads]")
+        views[f"{name}.scale"] = tensor.view(shape[0], 1, 1, 2 * shape[2])
+    return views
+
+
 def _layer_record(name, tensor, block_size, device):
     """The reference's record of one registered layer view, after its checks (reference dataplane.py:230-247).
 
@@ -585,6 +600,11 @@ class TorchBlockDataPlane:
     ``shared_name`` puts the pinned pool in POSIX shared memory of that name, so
     that other workers restore its host-tier blocks in place
     (:mod:`kvsnap_b200.sharedtier`).
+
+    ``scales`` (layer name -> contiguous float32 ``[blocks, 2, kv_heads]``): the
+    scales of caches held in 8 bits (:mod:`kvsnap_b200.cache8`), saved and
+    restored with their blocks; the packed block then has a ``name.scale`` span
+    a layer.
     """
 
     save_mode = "staged"
@@ -593,15 +613,20 @@ class TorchBlockDataPlane:
     sha_sms = 16
 
     def __init__(self, caches, block_size, capacity_bytes, *, save_mode=None, restore_mode=None, ctas=0,
-                 staging_bytes=512 << 20, shared_name=None, column_landing="kernel"):
+                 staging_bytes=512 << 20, shared_name=None, column_landing="kernel", scales=None):
         import torch
         if not caches:
             raise ValueError("empty KV cache registration")
         self.torch = torch
-        self.caches = dict(sorted(_split_paged(caches, block_size).items()))
+        views, block_views = _split_paged(caches, block_size), _block_views(scales)
+        if views.keys() & block_views.keys():
+            raise ValueError("a layer's name collides with another's scales")
+        self.block_views = frozenset(block_views)
+        self.caches = dict(sorted({**views, **block_views}.items()))
         self.block_size = block_size
         device = next(iter(self.caches.values())).device
-        self.layers = [_layer_record(name, tensor, block_size, device) for name, tensor in self.caches.items()]
+        self.layers = [_layer_record(name, tensor, 1 if name in self.block_views else block_size, device)
+                       for name, tensor in self.caches.items()]
         self.block_bytes = sum(layer["bytes"] for layer in self.layers)
         self.save_mode = save_mode or self.save_mode
         self.restore_mode = restore_mode or self.restore_mode

@@ -138,6 +138,8 @@ class Regrouper:
     def __init__(self, plane, plan: RegroupPlan, rank: int, *, group=None, is_destination=None):
         import torch
         from .dataplane import _dp
+        if getattr(plane, "block_views", None):
+            raise ValueError("a plane with 8-bit scales cannot be regrouped: its scale spans are not cut by head")
         self.plane, self.plan, self.rank, self.group = plane, plan, rank, group
         self.lib = _dp(plane.pool.lib)
         self.device = plane._device()

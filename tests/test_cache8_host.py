@@ -258,3 +258,39 @@ def test_calls_of_nothing_need_no_device():
 
 def test_structures_have_the_header_s_sizes():
     assert C.sizeof(_abi.C8Cache) == 72 and C.sizeof(_abi.C8Batch) == 48 and C.sizeof(_abi.C8Pair) == 96
+
+
+# ---- registration with the data plane ----------------------------------------------------------
+
+
+def test_the_data_plane_registers_codes_and_scales():
+    from kvsnap_b200.dataplane import TorchBlockDataPlane
+    codes = {f"layers.{i}": layer(blocks=5, heads=4, dim=128) for i in range(2)}
+    scales = {name: OnCuda(torch.zeros((5, 2, 4))) for name in codes}
+
+    class View(OnCuda):
+        def view(self, *shape):
+            return View(self._tensor.view(*shape))
+
+        def __getitem__(self, i):
+            return View(self._tensor[i])
+
+        def permute(self, *dims):
+            return View(self._tensor.permute(*dims))
+
+    wrap = lambda tensors: {name: View(t._tensor) for name, t in tensors.items()}   # noqa: E731
+    with patch("kvsnap_b200.dataplane.CudaPool"):
+        plane = TorchBlockDataPlane(wrap(codes), 16, 1 << 20, scales=wrap(scales))
+        assert [l["name"] for l in plane.layers] == ["layers.0.k", "layers.0.scale", "layers.0.v", "layers.1.k",
+                                                     "layers.1.scale", "layers.1.v"]
+        assert [l["bytes"] for l in plane.layers[:3]] == [16 * 4 * 128, 2 * 4 * 4, 16 * 4 * 128]
+        assert plane.layers[1]["shape"] == [1, 1, 8]
+        for bad in (torch.zeros((5, 4, 2)).transpose(1, 2), torch.zeros((5, 8)), torch.zeros((5, 3, 4))):
+            with pytest.raises(ValueError, match="scales"):
+                TorchBlockDataPlane(wrap(codes), 16, 1 << 20, scales={"layers.0": View(bad)})
+        with pytest.raises(ValueError, match="collides"):
+            TorchBlockDataPlane({"a": View(torch.zeros((2, 4, 16, 2, 64))), "a.scale": View(torch.zeros((4, 2, 16, 64)))},
+                                16, 1 << 20, scales={"a": View(torch.zeros((4, 2, 2)))})
+        from kvsnap_b200.reshard import Regrouper
+        with pytest.raises(ValueError, match="regrouped"):
+            Regrouper(plane, None, 0)

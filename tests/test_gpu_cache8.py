@@ -598,3 +598,104 @@ def test_no_rows_and_no_sequences():
         assert cache.attend("l", q, batch).shape == q.shape
         cache.append("l", k, k, batch)
     cache.check()
+
+
+# ---- a session's way: filled, saved, restored elsewhere, read on -----------------------------------
+
+
+@pytest.mark.parametrize("heads,staging", [(8, 512 << 20), (1, 512 << 20), (2, 1 << 20)])
+def test_a_session_is_saved_and_restored_in_8_bits(heads, staging):
+    """Prompt, save to pinned memory (codes, scales, checksums), restore into other blocks, next turn, step.
+
+    The packed blocks are the cache's own bytes with the last block's free slots zeroed; what is attended to
+    after the restore is bit for bit what it was before.
+    """
+    import hashlib
+
+    from kvsnap_b200.cache8 import PagedBatch, PagedCache8, rotary_table
+    from kvsnap_b200.dataplane import TorchBlockDataPlane
+    from oracle import oracle
+    names, dim, group, length = [f"layers.{i}" for i in range(3)], 128, 4, 403
+    count = -(-length // 16)
+    cache = PagedCache8.allocate(names, 120, 16, heads, dim)
+    for name in names:                                       # what earlier sessions left
+        cache.codes[name].view(torch.uint8).random_(0, 0x7E)
+        cache.scales[name].fill_(2.0 ** -3)
+    gen = torch.Generator().manual_seed(heads)
+    order = torch.randperm(120, generator=gen).tolist()
+    saved, restored, more = order[:count], order[count:2 * count], order[2 * count:2 * count + 3]
+    rotary = rotary_table(1024, dim, 1e6)
+
+    def batch(blocks, new, total):
+        return PagedBatch(torch.tensor([blocks], dtype=torch.int32).cuda(), torch.tensor([0, new], dtype=torch.int32).cuda(),
+                          torch.tensor([total], dtype=torch.int32).cuda(), max_query=new)
+
+    def turn(blocks, new, total, seed):
+        g = torch.Generator().manual_seed(seed)
+        outs = []
+        for name in names:
+            q, k, v = (torch.randn((new, h, dim), generator=g).to(torch.bfloat16).cuda() for h in (heads * group, heads, heads))
+            b = batch(blocks, new, total)
+            outs.append(cache.attend(name, cache.append(name, k, v, b, query=q, rotary=rotary), b))
+        return outs
+
+    turn(saved, length, length, 1)
+    cache.check()
+    before = {name: (cache.codes[name].view(torch.uint8).cpu(), cache.scales[name].cpu()) for name in names}
+    plane = TorchBlockDataPlane(cache.codes, 16, 64 << 20, scales=cache.scales, staging_bytes=staging)
+    try:
+        plane.warm_up()
+        size = plane.block_bytes
+        assert size == 3 * (2 * 16 * heads * dim + 8 * heads)
+        pinned = plane.pool.reserve(size * count)
+        targets = [(pinned, i * size) for i in range(count)]
+        digests = []
+        plane.save_gather(saved, targets, length, digests=digests)
+        packed = [pinned.read_range(i * size, size) for i in range(count)]
+        for i, block in enumerate(saved):
+            expected = b""
+            for name in names:
+                codes, scales = before[name]
+                sides = codes[:, block].clone()
+                if i == count - 1:
+                    sides[:, length % 16:] = 0
+                expected += sides[0].numpy().tobytes() + scales[block].numpy().tobytes() + sides[1].numpy().tobytes()
+            assert packed[i] == expected
+            assert digests[i] == (hashlib.sha256(expected).hexdigest(), oracle.crc32c(expected))
+        expected = turn(saved + more[:1], 9, length + 9, 2) + turn(saved + more[:1], 1, length + 10, 3)
+        plane.load_scatter(restored, targets, expected_crc32c=[c for _, c in digests])
+        again = turn(restored + more[1:2], 9, length + 9, 2) + turn(restored + more[1:2], 1, length + 10, 3)
+        for a, b in zip(again, expected):
+            assert torch.equal(a, b)
+        cache.check()
+        pinned.close()
+    finally:
+        plane.close()
+
+
+def test_a_16_bit_session_goes_on_in_8_bits():
+    """Blocks of a 16-bit cache compressed, attended to and expanded: what is read is what the codes stand for."""
+    from kvsnap_b200.cache8 import PagedBatch, PagedCache8
+    names, heads, dim, length = ["a", "b"], 2, 64, 70
+    wide = {name: torch.randn((2, 9, 16, heads, dim), device="cuda").to(torch.float16) for name in names}
+    cache = PagedCache8.allocate(names, 9, 16, heads, dim)
+    converter = cache.converter(wide)
+    source, blocks = [8, 0, 3, 5, 1], [2, 7, 4, 0, 6]
+    converter.compress(source, blocks, length)
+    batch = PagedBatch(torch.tensor([blocks], dtype=torch.int32).cuda(), torch.tensor([0, 1], dtype=torch.int32).cuda(),
+                       torch.tensor([length], dtype=torch.int32).cuda(), max_query=1)
+    q = torch.randn((1, 4, dim), device="cuda").to(torch.float16)
+    for name in names:
+        got = cache.attend(name, q, batch).cpu().double()
+        expected, bound = attend(q.cpu(), cache.codes[name].view(torch.uint8).cpu(), cache.scales[name].cpu(), [blocks],
+                                 [0, 1], [length], 16, dim ** -0.5)
+        assert ((got - expected).abs() <= bound).all()
+    back = {name: torch.zeros_like(t) for name, t in wide.items()}
+    cache.converter(back).expand(blocks, source)
+    cache.check()
+    for name in names:
+        values = wide[name][:, source].cpu().double().flatten(1, 2)[:, :length]
+        off = (back[name][:, source].cpu().double().flatten(1, 2)[:, :length] - values).abs()
+        # half a step of the format, or of its smallest numbers at the block's scale (amax < 8: 2^-5)
+        assert (off <= torch.maximum(2.0 ** -4 * values.abs(), torch.full_like(values, 2.0 ** -15))).all()
+        assert (back[name][:, source].cpu().flatten(1, 2)[:, length:] == 0).all()
