@@ -151,6 +151,10 @@ __device__ __forceinline__ void copy_async(uint32_t to, const char* from, bool t
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
 }
 
+__device__ __forceinline__ void copy_async4(uint32_t to, const float* from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+}
+
 // Where 16 bytes `chunk` of a token's D codes lie in a granule of one side: lines of 128 bytes, their 16-byte
 // places turned so that the 8 lanes of a read meet all banks. Such lanes read the keys of tokens 4 k and
 // 4 k + 1 (+ 2), and 2 chunks of the values of tokens i, 4 + i, 8 + i, 12 + i.
@@ -235,19 +239,23 @@ struct StepWarp {
                 const int j = ahead - c0;
                 if (j % 32 == 0) {
                     const int token = (ahead + lane) * stride + skip;
-                    StepPage page{-1, 0.0f, 0.0f};
+                    int64_t place = -1;
+                    const uint32_t entry = uint32_t(__cvta_generic_to_shared(pages + j % 64 + lane));
+                    __syncwarp();
                     if (ahead + lane < c1 && token < q.length) {
                         const int64_t block = ints(p.a.b.table)[s * p.a.b.table_pitch + token / c.block_size];
                         if (block < 0 || block >= c.blocks) {
                             atomicOr(p.a.status, KVSNAP_DP_BAD_BLOCK);
                         } else {
-                            page.off = block * c.block_pitch + token % c.block_size * c.token_pitch;
+                            place = block * c.block_pitch + token % c.block_size * c.token_pitch;
+                            // Its scales come with the codes: nothing waits for them here.
                             const float* scales = reinterpret_cast<const float*>(c.scales) + block * 2 * c.kv_heads + head;
-                            page.ks = scales[0], page.vs = scales[c.kv_heads];
+                            copy_async4(entry + 8, scales);
+                            copy_async4(entry + 12, scales + c.kv_heads);
                         }
                     }
-                    __syncwarp();
-                    pages[j % 64 + lane] = page;
+                    pages[j % 64 + lane].off = place;
+                    if (place < 0) pages[j % 64 + lane].ks = pages[j % 64 + lane].vs = 0.0f;
                     __syncwarp();
                 }
                 const int64_t found = pages[j % 64].off, at = max(found, int64_t(0));
@@ -478,6 +486,7 @@ struct StepShared {
         char ring[kWarps][kAhead * 2 * kGranule * D];
     };
     float2 ml[kWarps][8 * NT];
+    float2 joined[8][8 * NT];              // a head's row: maximum over the slices, sum
     StepPage pages[kWarps][64];
     uint32_t sums[2][kWarps];
     uint32_t found_first;
@@ -504,26 +513,33 @@ __global__ void __launch_bounds__(32 * kWarps, 1) step_kernel(const __grid_const
     Sequence q;
     if (SPLIT) {
         if (threadIdx.x == 0) p.parts.units[blockIdx.x].parts = 0;
-        // All chunks; those of up to 512 sequences are summed and found in one pass.
+        // All chunks; those of up to 512 sequences are summed and found in one pass, one's need no sum.
         uint32_t mine = 0;
-        for (int i = threadIdx.x; i < seqs; i += blockDim.x) mine += chunks_of(p, i, q) * p.hg;
-        uint32_t sum = mine;
+        if (seqs == 1) mine = chunks_of(p, 0, q) * p.hg;
+        else for (int i = threadIdx.x; i < seqs; i += blockDim.x) mine += chunks_of(p, i, q) * p.hg;
+        uint32_t sum = mine, low = 0;
+        if (seqs == 1) {
+            cut_total = mine;
+        } else {
 #pragma unroll
-        for (int k = 1; k < 32; k <<= 1) {
-            const uint32_t up = __shfl_up_sync(~0u, sum, k);
-            if (lane >= k) sum += up;
-        }
-        if (lane == 31) sh.sums[0][warp] = sum;
-        __syncthreads();
-        uint32_t low = 0;
-        for (int w = 0; w < kWarps; ++w) {
-            if (w == warp) low = cut_total;
-            cut_total += sh.sums[0][w];
+            for (int k = 1; k < 32; k <<= 1) {
+                const uint32_t up = __shfl_up_sync(~0u, sum, k);
+                if (lane >= k) sum += up;
+            }
+            if (lane == 31) sh.sums[0][warp] = sum;
+            __syncthreads();
+            for (int w = 0; w < kWarps; ++w) {
+                if (w == warp) low = cut_total;
+                cut_total += sh.sums[0][w];
+            }
         }
         const Cut cut(cut_total, gridDim.x);
         if (blockIdx.x >= cut.ctas) return;
         pos = cut.begin(blockIdx.x), end = cut.begin(blockIdx.x + 1);
-        if (seqs <= int(blockDim.x)) {
+        if (seqs == 1) {
+            if (threadIdx.x == 0) sh.found = 0, sh.found_first = 0;
+            __syncthreads();
+        } else if (seqs <= int(blockDim.x)) {
             const uint32_t first = low + sum - mine;
             if (mine && first <= pos && pos < first + mine) sh.found = threadIdx.x, sh.found_first = first;
             __syncthreads();
@@ -590,32 +606,41 @@ __global__ void __launch_bounds__(32 * kWarps, 1) step_kernel(const __grid_const
             }
         }
         __syncthreads();
-        // Join the slices, 4 dims of one row and head a thread.
+        // Join the slices: their factors, then 4 dims of one row and head a thread.
+        for (int i = threadIdx.x; i < p.hc * rows; i += blockDim.x) {
+            const int row = i % rows, h = i / rows;
+            float top = kLowest, sum = 0.0f;
+            for (int k = 0; k < p.ts; ++k) top = fmaxf(top, sh.ml[k * p.hc + h][row].x);
+            for (int k = 0; k < p.ts; ++k) {
+                float2& ml = sh.ml[k * p.hc + h][row];
+                ml.x = exp2_fast(ml.x - top);
+                sum += ml.x * ml.y;
+            }
+            sh.joined[h][row] = make_float2(top, sum);
+        }
+        __syncthreads();
         const bool whole = !SPLIT || (c0 == 0 && c1 == chunks);
         const int slot = 2 * int(blockIdx.x) + (c0 == 0);
         for (int i = threadIdx.x; i < p.hc * rows * (D / 4); i += blockDim.x) {
             const int at = i % (D / 4) * 4, row = i / (D / 4) % rows, h = i / (D / 4) / rows;
-            float top = kLowest;
-            for (int k = 0; k < p.ts; ++k) top = fmaxf(top, sh.ml[k * p.hc + h][row].x);
-            float sum = 0.0f;
             float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll 4
             for (int k = 0; k < p.ts; ++k) {
-                const float2 ml = sh.ml[k * p.hc + h][row];
-                const float f = exp2_fast(ml.x - top);
+                const float f = sh.ml[k * p.hc + h][row].x;
                 const float4 v = *reinterpret_cast<const float4*>(&sh.o[k * p.hc + h][row][at]);
-                sum += f * ml.y;
                 o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;
             }
+            const float2 all = sh.joined[h][row];
             const int head = hg * p.hc + h;
             if (whole) {
-                // l is 0 only for a row that sees nothing
-                const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
+                // the sum is 0 only for a row that sees nothing
+                const float by = all.y == 0.0f ? 0.0f : 1.0f / all.y;
                 const int64_t to = int64_t(q.row + row / p.a.group) * p.a.q_heads + head * p.a.group + row % p.a.group;
                 store4<T>(p.a.out + (to * D + at) * 2, make_float4(o.x * by, o.y * by, o.z * by, o.w * by));
             } else {
                 const int64_t to = (int64_t(slot) * p.hc + h) * kStepRows + row;
                 *reinterpret_cast<float4*>(p.parts.sums + to * D + at) = o;
-                if (at == 0) p.parts.ml[to] = make_float2(top, sum);
+                if (at == 0) p.parts.ml[to] = all;
             }
         }
         if (SPLIT) {
@@ -631,126 +656,72 @@ __global__ void __launch_bounds__(32 * kWarps, 1) step_kernel(const __grid_const
     }
 }
 
-// Joins the parts of shared units, which lie in consecutive CTAs' slots. A warp a row where there are
-// few parts, else a CTA a row, its warps a share of the parts each.
+// Joins the parts of the shared unit that CTA blockIdx.x of the kernel before began, which lie in
+// consecutive CTAs' slots. Where units have few parts (WIDE false) a warp takes a row, else a CTA does,
+// its warps a share of the parts each.
 constexpr int kJoinWarps = 8;
-constexpr int kJoinCtas = 6;               // an SM
-constexpr int kMostCtas = 512;
 
-template <typename T, int D>
+template <typename T, int D, bool WIDE>
 __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_constant__ AttendArgs a,
-                                                               const __grid_constant__ Parts p, int ctas) {
+                                                               const __grid_constant__ Parts p) {
     constexpr int kEach = D / 32;
     using Piece = std::conditional_t<kEach == 4, float4, float2>;
-    __shared__ SharedUnit units[kMostCtas];
-    __shared__ int owner[kMostCtas];
-    __shared__ int count, most;
     __shared__ float sums[kJoinWarps][D];
-    __shared__ float weight[kMostCtas], stat[2][kJoinWarps];
+    __shared__ float stat[kJoinWarps];
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const int task = WIDE ? blockIdx.y : blockIdx.y * kJoinWarps + warp;       // a row of one of the heads
+    const int h = task / p.used_rows, row = task % p.used_rows;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (warp == 0) {
-        int n = 0, parts = 0;
-#pragma unroll 5
-        for (int i = lane; i < (ctas + 31) / 32 * 32; i += 32) {
-            SharedUnit u{};
-            if (i < ctas) u = p.units[i];
-            const uint32_t hit = __ballot_sync(~0u, u.parts > 0);
-            if (u.parts > 0) {
-                const int at = n + __popc(hit & ((1u << lane) - 1));
-                units[at] = u, owner[at] = i;
-                parts = max(parts, u.parts);
-            }
-            n += __popc(hit);
+    const SharedUnit u = p.units[blockIdx.x];
+    if (u.parts == 0 || h >= p.heads || row >= u.rows) return;
+    const int slot_rows = p.heads * p.head_rows, in = h * p.head_rows + row;
+    const auto at = [&](int f) { return int64_t(2 * (int(blockIdx.x) + f) + (f == 0)) * slot_rows + in; };
+    const auto part = [&](int f) { return *reinterpret_cast<const Piece*>(p.sums + at(f) * D + lane * kEach); };
+    float o[kEach] = {}, top = kLowest, sum = 0.0f;
+    const auto add = [&](const Piece& v, float by) {
+        const float* x = reinterpret_cast<const float*>(&v);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) o[i] += by * x[i];
+    };
+    // The maximum of all parts; then a warp's parts (of WIDE every eighth), 4 on their way at a time.
+    for (int i = lane; i < u.parts; i += 32) top = fmaxf(top, p.ml[at(i)].x);
+    const int first = WIDE ? warp : 0, step = WIDE ? kJoinWarps : 1;
+    for (int i = first; i < u.parts; i += 4 * step) {
+        Piece v[4];
+        float2 ml[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int f = min(i + j * step, u.parts - 1);
+            v[j] = part(f), ml[j] = p.ml[at(f)];
         }
-        parts = __reduce_max_sync(~0u, parts);
-        if (lane == 0) count = n, most = parts;
-    }
-    __syncthreads();
-    const bool alone = most <= 8;                                  // a warp a row
-    const int first = alone ? blockIdx.x * kJoinWarps + warp : blockIdx.x;
-    const int step = alone ? gridDim.x * kJoinWarps : gridDim.x;
-    const int slot_rows = p.heads * p.head_rows, used = p.heads * p.used_rows;
-    for (int task = first; task < count * used; task += step) {
-        const int k = task / used, h = task % used / p.used_rows, row = task % p.used_rows;
-        const SharedUnit u = units[k];
-        if (row >= u.rows) continue;
-        const int in = h * p.head_rows + row;
-        const auto at = [&](int f) { return int64_t(2 * (owner[k] + f) + (f == 0)) * slot_rows + in; };
-        const auto part = [&](int f) { return *reinterpret_cast<const Piece*>(p.sums + at(f) * D + lane * kEach); };
-        float o[kEach] = {}, sum = 0.0f;
-        const auto add = [&](const Piece& v, float by) {
-            const float* x = reinterpret_cast<const float*>(&v);
+        if (i == first) top = warp_max(top);
 #pragma unroll
-            for (int i = 0; i < kEach; ++i) o[i] += by * x[i];
-        };
-        if (alone) {
-            const float2 ml = lane < u.parts ? p.ml[at(lane)] : make_float2(kLowest, 0.0f);
-            const Piece x = part(0), y = u.parts > 1 ? part(1) : Piece{};
-            float top = ml.x;
-#pragma unroll
-            for (int i = 4; i; i >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, i));
-            top = __shfl_sync(~0u, top, 0);
-            const float f = exp2_fast(ml.x - top);
-            sum = lane < u.parts ? f * ml.y : 0.0f;
-#pragma unroll
-            for (int i = 4; i; i >>= 1) sum += __shfl_xor_sync(~0u, sum, i);
-            sum = __shfl_sync(~0u, sum, 0);
-            add(x, __shfl_sync(~0u, f, 0));
-            add(y, __shfl_sync(~0u, f, 1));
-            for (int i = 2; i < u.parts; ++i) add(part(i), __shfl_sync(~0u, f, i));
-        } else {
-            float top = kLowest;
-            for (int i = threadIdx.x; i < u.parts; i += blockDim.x) {
-                const float2 ml = p.ml[at(i)];
-                weight[i] = ml.x;
-                top = fmaxf(top, ml.x);
-            }
-            top = warp_max(top);
-            if (lane == 0) stat[0][warp] = top;
-            __syncthreads();
-            top = stat[0][0];
-            for (int w = 1; w < kJoinWarps; ++w) top = fmaxf(top, stat[0][w]);
-            // Each warp its share of the parts, 8 on their way at a time.
-            for (int i = warp; i < u.parts; i += 8 * kJoinWarps) {
-                Piece v[8];
-                float by[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int f = i + j * kJoinWarps;
-                    v[j] = Piece{}, by[j] = 0.0f;
-                    if (f < u.parts) v[j] = part(f), by[j] = exp2_fast(weight[f] - top);
-                }
-#pragma unroll
-                for (int j = 0; j < 8; ++j) add(v[j], by[j]);
-            }
-            for (int i = threadIdx.x; i < u.parts; i += blockDim.x)
-                sum += exp2_fast(weight[i] - top) * p.ml[at(i)].y;
-#pragma unroll
-            for (int i = 16; i; i >>= 1) sum += __shfl_xor_sync(~0u, sum, i);
-            if (lane == 0) stat[1][warp] = sum;
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) sums[warp][lane * kEach + i] = o[i];
-            __syncthreads();
-            if (warp == 0) {
-                sum = 0.0f;
-                for (int w = 0; w < kJoinWarps; ++w) sum += stat[1][w];
-#pragma unroll
-                for (int i = 0; i < kEach; ++i) {
-                    o[i] = 0.0f;
-                    for (int w = 0; w < kJoinWarps; ++w) o[i] += sums[w][lane * kEach + i];
-                }
-            }
-            __syncthreads();
-            if (warp) continue;
+        for (int j = 0; j < 4; ++j) {
+            const float by = i + j * step < u.parts ? exp2_fast(ml[j].x - top) : 0.0f;
+            add(v[j], by);
+            sum += by * ml[j].y;
         }
-        const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
-        const int r = u.first + row;
-        const int64_t to = int64_t(u.row + r / a.group) * a.q_heads + (u.head + h) * a.group + r % a.group;
-        char* out = a.out + (to * D + lane * kEach) * 2;
-        if constexpr (kEach == 4) store4<T>(out, make_float4(o[0] * by, o[1] * by, o[2] * by, o[3] * by));
-        else *reinterpret_cast<uint32_t*>(out) = T::pack(o[0] * by, o[1] * by);
     }
+    if (WIDE) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) sums[warp][lane * kEach + i] = o[i];
+        if (lane == 0) stat[warp] = sum;
+        __syncthreads();
+        if (warp) return;
+        sum = 0.0f;
+        for (int w = 0; w < kJoinWarps; ++w) sum += stat[w];
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            o[i] = 0.0f;
+            for (int w = 0; w < kJoinWarps; ++w) o[i] += sums[w][lane * kEach + i];
+        }
+    }
+    const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const int r = u.first + row;
+    const int64_t to = int64_t(u.row + r / a.group) * a.q_heads + (u.head + h) * a.group + r % a.group;
+    char* out = a.out + (to * D + lane * kEach) * 2;
+    if constexpr (kEach == 4) store4<T>(out, make_float4(o[0] * by, o[1] * by, o[2] * by, o[3] * by));
+    else *reinterpret_cast<uint32_t*>(out) = T::pack(o[0] * by, o[1] * by);
 }
 
 // ---- many rows: chunks and prompts --------------------------------------------------------
@@ -1736,7 +1707,7 @@ struct Plan {
     bool split, wide;         // the step kernel's units are cut; more than 8 rows a head
     int step_rows;
     int most_rows;            // that a KV head of a sequence can have
-    int64_t ctas, step_ctas;
+    int64_t ctas, step_ctas, step_units;
     int64_t slots, sum_bytes, bytes;
 };
 
@@ -1772,8 +1743,9 @@ Plan plan_for(const Cache& c, const Batch& b, int q_heads, int sms) {
     // Up to 8 chunks a unit, a CTA each: cutting them would cost more (a scan of the lengths,
     // parts and their join) than a few granules in turn.
     plan.split = most > 8;
-    plan.ctas = sms < kMostCtas ? sms : kMostCtas;
-    plan.step_ctas = plan.split ? plan.ctas : int64_t(b.seqs) * p.hg;
+    plan.ctas = sms;
+    plan.step_units = int64_t(b.seqs) * p.hg;
+    plan.step_ctas = plan.split ? plan.ctas : plan.step_units;
     const int64_t step_slot = plan.stepped && plan.split ? p.hc * kStepRows : 0;
     const int64_t chunk_slot = plan.chunked ? kUnitRows : 0;
     // The two kernels and their joins run one after the other: they use the same bytes.
@@ -1798,10 +1770,10 @@ void allow_shared(const void* kernel, int bytes) {
 }
 
 template <typename K, typename... A>
-void launch(K kernel, int64_t ctas, int threads, size_t shared, cudaStream_t stream, bool after, const A&... args) {
+void launch(K kernel, dim3 grid, int threads, size_t shared, cudaStream_t stream, bool after, const A&... args) {
     if (shared > 48 << 10) allow_shared(reinterpret_cast<const void*>(kernel), int(shared));
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3(unsigned(ctas)), config.blockDim = dim3(unsigned(threads));
+    config.gridDim = grid, config.blockDim = dim3(unsigned(threads));
     config.dynamicSmemBytes = shared, config.stream = stream;
     cudaLaunchAttribute attribute{};
     attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1813,14 +1785,17 @@ void launch(K kernel, int64_t ctas, int threads, size_t shared, cudaStream_t str
 template <typename T, int D, int NT>
 void launch_step(const Plan& plan, const StepArgs& p, cudaStream_t stream) {
     const size_t shared = sizeof(StepShared<D, NT>);
-    if (plan.split) launch(step_kernel<T, D, NT, true>, plan.step_ctas, 32 * kWarps, shared, stream, false, p);
-    else launch(step_kernel<T, D, NT, false>, plan.step_ctas, 32 * kWarps, shared, stream, false, p);
+    if (plan.split) launch(step_kernel<T, D, NT, true>, dim3(unsigned(plan.step_ctas)), 32 * kWarps, shared, stream, false, p);
+    else launch(step_kernel<T, D, NT, false>, dim3(unsigned(plan.step_ctas)), 32 * kWarps, shared, stream, false, p);
 }
 
 template <typename T, int D>
 void launch_attend(const Plan& plan, const AttendArgs& a, Parts parts, cudaStream_t stream) {
-    const auto join = [&] {
-        launch(join_kernel<T, D>, plan.ctas * kJoinCtas, 32 * kJoinWarps, 0, stream, true, a, parts, int(plan.ctas));
+    // `units` of the step kernel bound how many parts a unit has.
+    const auto join = [&](int64_t units) {
+        const unsigned rows = unsigned(parts.heads * parts.used_rows), ctas = unsigned(plan.ctas);
+        if (units * 8 <= plan.ctas) launch(join_kernel<T, D, true>, dim3(ctas, rows), 32 * kJoinWarps, 0, stream, true, a, parts);
+        else launch(join_kernel<T, D, false>, dim3(ctas, (rows + kJoinWarps - 1) / kJoinWarps), 32 * kJoinWarps, 0, stream, true, a, parts);
     };
     if (plan.stepped) {
         StepArgs p = plan.step;
@@ -1828,13 +1803,13 @@ void launch_attend(const Plan& plan, const AttendArgs& a, Parts parts, cudaStrea
         p.a = a, p.parts = parts;
         if (plan.wide) launch_step<T, D, 2>(plan, p, stream);
         else launch_step<T, D, 1>(plan, p, stream);
-        if (plan.split) join();
+        if (plan.split) join(plan.step_units);
     }
     if (plan.chunked) {
         parts.heads = 1, parts.head_rows = kUnitRows, parts.used_rows = plan.most_rows < kUnitRows ? plan.most_rows : kUnitRows;
-        launch(chunk_kernel<T, D>, plan.ctas, kChunkThreads, sizeof(ChunkShared<D>) + 1024, stream, false,
+        launch(chunk_kernel<T, D>, dim3(unsigned(plan.ctas)), kChunkThreads, sizeof(ChunkShared<D>) + 1024, stream, false,
                ChunkArgs{a, parts});
-        join();
+        join(plan.ctas);
     }
 }
 
