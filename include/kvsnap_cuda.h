@@ -364,6 +364,7 @@ typedef struct kvsnap_c8_cache {
  * start[seqs] on belong to nobody. A row whose position would be negative
  * (lengths[s] below the row count, 0 for a padded entry) is not in the cache.
  * All three arrays are device memory, read by the kernels, never by the host.
+ * A table row holds at most 2^30 tokens.
  */
 typedef struct kvsnap_c8_batch {
     int64_t table, start, lengths;      /* device addresses of int32 arrays */
@@ -433,7 +434,8 @@ typedef struct kvsnap_c8_pair {
  * launch: pairs is a device array of `layers`, wide_ids and ids device int64
  * arrays of n block ids. compress writes blocks ids[i] from wide_ids[i]; token
  * slots from valid_tokens on (counted over the n blocks; negative: none) become
- * zeros. expand writes blocks wide_ids[i] from ids[i], rounded once.
+ * zeros. expand writes blocks wide_ids[i] from ids[i], rounded once. No block
+ * may be written twice in one call.
  */
 int kvsnap_c8_compress(const kvsnap_c8_pair* pairs, int layers, int block_size, int kv_heads, int head_dim, int type,
                        const int64_t* wide_ids, const int64_t* ids, int64_t n, int64_t valid_tokens,

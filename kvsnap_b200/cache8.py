@@ -356,7 +356,7 @@ class CacheConverter:
 
         ``num_kv_tokens``: tokens that the blocks hold, in order; slots behind the last become zeros, as a
         save zeroes them (None: every slot counts). Block ids are lists, or int64 tensors on the cache's
-        device (no copy then). A target block named twice holds either source.
+        device (no copy then). A target block must not be named twice.
         """
         if num_kv_tokens is not None and (type(num_kv_tokens) is not int or num_kv_tokens < 0):
             raise ValueError("num_kv_tokens must be a non-negative int")

@@ -1815,7 +1815,7 @@ void launch_attend(const Plan& plan, const AttendArgs& a, Parts parts, cudaStrea
 
 void check_attend(const Cache* cache, const Batch* batch, int q_heads) {
     check_cache(cache);
-    check_batch(batch);
+    check_batch(batch, cache);
     require(q_heads > 0 && q_heads % cache->kv_heads == 0, "query heads must be a multiple of the KV heads");
     require(int64_t(batch->seqs) * cache->kv_heads < (1LL << 30) && int64_t(batch->rows) * q_heads < (1LL << 30),
             "too many sequences or rows for one attention");
@@ -1833,6 +1833,7 @@ extern "C" int kvsnap_c8_attend_workspace(const kvsnap_c8_cache* cache, const kv
                                           size_t* bytes) {
     return on_device(cache ? cache->device : 0, [&] {
         check_attend(cache, batch, q_heads);
+        require(bytes, "the workspace's size needs a place");
         *bytes = 0;
         return batch->rows && batch->seqs;
     }, [&] {

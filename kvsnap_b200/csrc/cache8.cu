@@ -343,7 +343,7 @@ extern "C" int kvsnap_c8_append(const kvsnap_c8_cache* cache, const kvsnap_c8_ba
                                 int interleaved, uint32_t* status, uintptr_t stream) {
     return on_device(cache ? cache->device : 0, [&] {
         check_cache(cache);
-        check_batch(batch);
+        check_batch(batch, cache);
         require(status, "the append needs a status word");
         if (!batch->rows || !batch->seqs) return false;
         check_rows(key, key_token, key_head);

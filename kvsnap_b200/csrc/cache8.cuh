@@ -200,9 +200,11 @@ void check_cache(const Cache* c) {
             "the 8-bit cache's codes must be 16-byte aligned");
 }
 
-void check_batch(const Batch* b) {
+void check_batch(const Batch* b, const Cache* c) {
     require(b && (!b->seqs || (b->start && b->lengths && (b->table || !b->width))), "the batch has no tables");
     require(b->seqs >= 0 && b->rows >= 0 && b->width >= 0 && b->max_query >= 0, "invalid batch");
+    // the kernels count a sequence's tokens in 32 bits, some of them past its end
+    require(int64_t(b->width) * c->block_size <= 1LL << 30, "the block table holds more than 2^30 tokens a sequence");
 }
 
 void check_rows(const void* at, int64_t token, int64_t head) {

@@ -217,6 +217,7 @@ def append(lib, cache, batch, type=0, key=4096, pitch=256, q_heads=0, query=None
     (c_cache(token_pitch=8), c_batch(), {}, "aligned"),
     (c_cache(), c_batch(table=0), {}, "no tables"),
     (c_cache(), c_batch(seqs=-1), {}, "invalid batch"),
+    (c_cache(), c_batch(width=(1 << 26) + 1), {}, "2^30 tokens"),
     (c_cache(), c_batch(), {"key": 4104}, "aligned"),
     (c_cache(), c_batch(), {"key": None}, "aligned"),
     (c_cache(), c_batch(), {"pitch": 24}, "aligned"),
@@ -247,6 +248,16 @@ def test_the_library_refuses_attentions_and_conversions():
         assert message in lib.kvsnap_cuda_error().decode()
         assert lib.kvsnap_c8_expand(4096, 1, size, heads, dim, type, 4096, 4096, n, 4096, 0, 0) == -1
         assert message in lib.kvsnap_cuda_error().decode()
+
+
+def test_the_workspace_s_size_needs_a_place_and_bounded_work():
+    lib = library()
+    assert lib.kvsnap_c8_attend_workspace(c_cache(), c_batch(), 4, None) == -1
+    assert "place" in lib.kvsnap_cuda_error().decode()
+    size = C.c_size_t(7)
+    assert lib.kvsnap_c8_attend_workspace(c_cache(), c_batch(rows=0), 4, size) == 0 and size.value == 0
+    assert lib.kvsnap_c8_attend_workspace(c_cache(), c_batch(seqs=1 << 20, width=1 << 20), 4, size) == -1
+    assert "too much work" in lib.kvsnap_cuda_error().decode()
 
 
 def test_calls_of_nothing_need_no_device():

@@ -533,6 +533,55 @@ def test_two_graphs_and_two_streams_do_not_share_workspaces():
         assert torch.equal(out, want)
 
 
+def test_calls_run_on_the_current_stream():
+    """Inputs made on a side stream behind a long queue of work, used there without a wait: order is the stream's."""
+    p = Paged([(1, 300), (20, 77)])
+    before = (p.codes_gpu.clone(), p.scales_gpu.clone())
+    run = step(p)
+    expected = run().clone()
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    p.codes_gpu.zero_(), p.scales_gpu.zero_()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        x = torch.randn((4096, 4096), device="cuda")
+        for _ in range(20):
+            x = x @ x * 1e-3
+        p.codes_gpu.copy_(before[0]), p.scales_gpu.copy_(before[1])
+        got = run()
+    side.synchronize()
+    assert torch.equal(got, expected)
+    p.cache.check()
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    """No kernel of the cache has run in the process: a capture of the first step replays right."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = """
+import torch
+import test_gpu_cache8 as t
+p = t.Paged([(1, 700), (40, 50)], heads=2)
+before = (p.codes_gpu.clone(), p.scales_gpu.clone())
+run = t.step(p)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = run()
+graph.replay()
+first = out.clone()
+p.codes_gpu.copy_(before[0]), p.scales_gpu.copy_(before[1])
+assert torch.equal(run(), first) and first.isfinite().all() and first.any()
+p.cache.check()
+print("captured first")
+"""
+    here = Path(__file__).resolve().parent
+    got = subprocess.run([sys.executable, "-c", code], cwd=here, env={**__import__("os").environ, "PYTHONPATH": f"{here}:{here.parent}"},
+                         capture_output=True, text=True, timeout=300)
+    assert "captured first" in got.stdout, got.stderr[-2000:]
+
+
 def test_a_bad_block_is_skipped_and_reported():
     """A block id outside the cache: recorded, its tokens left out, everything else as without it."""
     p = Paged([(1, 40), (1, 70), (3, 33)], heads=2)
