@@ -61,43 +61,49 @@ __device__ __forceinline__ bool find_page(const Batch& b, int n, int64_t u, Page
     return true;
 }
 
-// (cos, sin) of the pairs of elements [at, at + 8) of a row.
-struct Turn {
-    uint4 x[4];
+// A lane's 8 elements of a row of rotated heads: 4 from `low` on and 4 from `high` on, 4 whole pairs, so that
+// nothing passes between lanes and a row's angles are read once: of a row of 16 lanes each reads 8 bytes
+// of two lines, and 32 bytes of angles. Elements from rotary_dim on, and interleaved pairs, lie together.
+struct Place {
+    int low, high, pair;
+    bool turned;
+
+    __device__ __forceinline__ Place(int lane, int rotary_dim, bool interleaved) : pair(4 * lane) {
+        turned = 8 * lane < rotary_dim;
+        const bool apart = turned && !interleaved;
+        low = apart ? 4 * lane : 8 * lane, high = apart ? rotary_dim / 2 + 4 * lane : 8 * lane + 4;
+    }
 };
 
-template <bool INTERLEAVED>
-__device__ __forceinline__ void fetch_turn(Turn& turn, const AppendArgs& a, int64_t position, int at, bool there) {
-    const int half = a.rotary_dim / 2, pair = INTERLEAVED ? at / 2 : at < half ? at : at - half;
-    const char* from = reinterpret_cast<const char*>(a.rotary + min(position, a.positions - 1) * half + pair);
+// (cos, sin) of a lane's 4 pairs.
+struct Turn {
+    uint4 x[2];
+};
+
+__device__ __forceinline__ void fetch_turn(Turn& turn, const AppendArgs& a, int64_t position, const Place& at,
+                                           bool there) {
+    const float2* from = a.rotary + min(position, a.positions - 1) * (a.rotary_dim / 2) + at.pair;
 #pragma unroll
-    for (int i = 0; i < (INTERLEAVED ? 2 : 4); ++i) turn.x[i] = fetch16(from + 16 * i, there && at < a.rotary_dim);
+    for (int i = 0; i < 2; ++i) turn.x[i] = fetch16(reinterpret_cast<const char*>(from + 2 * i), there && at.turned);
 }
 
-// 8 consecutive elements [at, at + 8) of a head's row, rotated (rotary_dim 0: as they are). The lane `mate`
-// has the elements that they are turned with; every lane of the warp is here.
+__device__ __forceinline__ uint4 fetch_place(const char* row, const Place& at, bool there) {
+    const uint2 low = fetch8(row + 2 * at.low, there), high = fetch8(row + 2 * at.high, there);
+    return make_uint4(low.x, low.y, high.x, high.y);
+}
+
 template <typename T, bool INTERLEAVED>
-__device__ __forceinline__ void turn8(const uint4& own, const Turn& turn, int at, int rotary_dim, int mate,
-                                      float (&v)[8]) {
-    widen8<T>(own, v);
+__device__ __forceinline__ void turn8(const uint4& raw, const Turn& turn, const Place& at, float (&v)[8]) {
+    widen8<T>(raw, v);
+    if (!at.turned) return;
     const float* cs = reinterpret_cast<const float*>(turn.x);
-    if (INTERLEAVED) {
-        if (at >= rotary_dim) return;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float p = v[2 * i], q = v[2 * i + 1];
-            v[2 * i] = p * cs[2 * i] - q * cs[2 * i + 1];
-            v[2 * i + 1] = q * cs[2 * i] + p * cs[2 * i + 1];
-        }
-    } else {
-        const uint4 other = make_uint4(__shfl_sync(~0u, own.x, mate), __shfl_sync(~0u, own.y, mate),
-                                       __shfl_sync(~0u, own.z, mate), __shfl_sync(~0u, own.w, mate));
-        if (at >= rotary_dim) return;
-        const float sign = at < rotary_dim / 2 ? -1.0f : 1.0f;
-        float w[8];
-        widen8<T>(other, w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = v[i] * cs[2 * i] + sign * (w[i] * cs[2 * i + 1]);
+    for (int i = 0; i < 4; ++i) {
+        float& p = v[INTERLEAVED ? 2 * i : i];
+        float& q = v[INTERLEAVED ? 2 * i + 1 : 4 + i];
+        const float x = p, y = q;
+        p = x * cs[2 * i] - y * cs[2 * i + 1];
+        q = y * cs[2 * i] + x * cs[2 * i + 1];
     }
 }
 
@@ -132,8 +138,8 @@ __device__ __forceinline__ float largest(const uint4 (&raw)[kHeld]) {
 // fetched once for 8 query heads. Keys are held as they come and turned twice, for the scale and for the
 // codes: turned they would take twice the registers.
 template <typename T, int D, bool SINGLE, bool INTERLEAVED>
-__global__ void __launch_bounds__(256, 3) append_kernel(const __grid_constant__ AppendArgs a) {
-    constexpr int kLanes = D / 8, kRows = 32 / kLanes, kTogether = SINGLE ? 1 : 4;
+__global__ void __launch_bounds__(256, 2) append_kernel(const __grid_constant__ AppendArgs a) {
+    constexpr int kLanes = D / 8, kRows = 32 / kLanes, kTogether = SINGLE ? 1 : 8;
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, n = a.c.block_size;
     const int kv_ctas = (2 * a.c.kv_heads + 7) / 8, slot = blockIdx.y * 8 + warp;
     const bool queries = blockIdx.y >= kv_ctas;
@@ -143,8 +149,7 @@ __global__ void __launch_bounds__(256, 3) append_kernel(const __grid_constant__ 
     const int sub = lane / kLanes, at = lane % kLanes * 8, end = run.first + run.count;
     const int base = run.page * n;                               // position of the page's slot 0
     if (a.rotary_dim && base + end > a.positions && threadIdx.x == 0) atomicOr(a.status, KVSNAP_C8_BAD_POSITION);
-    const int reach = a.rotary_dim / 16;                               // lanes to the other half of a pair
-    const int mate = at >= a.rotary_dim ? lane : at < a.rotary_dim / 2 ? lane + reach : lane - reach;
+    const Place place(lane % kLanes, a.rotary_dim, INTERLEAVED);
 
     if (queries) {
         // (one row: a head a warp)
@@ -152,20 +157,24 @@ __global__ void __launch_bounds__(256, 3) append_kernel(const __grid_constant__ 
         for (int first = run.first + (SINGLE ? 0 : warp * kRows); first < end; first += 8 * kRows) {
             const int r = first + sub;
             const int64_t row = run.row + (r - run.first);
-            const char* from = a.query.at + row * a.query.token + head * a.query.head + 2 * at;
-            char* to = a.query_out + (row * a.q_heads + head) * (2 * D) + 2 * at;
+            const char* from = a.query.at + row * a.query.token + head * a.query.head;
+            char* to = a.query_out + (row * a.q_heads + head) * (2 * D);
             Turn turn;
-            fetch_turn<INTERLEAVED>(turn, a, base + r, at, r < end);
+            fetch_turn(turn, a, base + r, place, r < end);
             for (int h = 0; h < heads; h += kTogether) {
                 uint4 raw[kTogether];
 #pragma unroll
                 for (int i = 0; i < kTogether; ++i)
-                    raw[i] = fetch16(from + (h + i) * a.query.head, r < end && h + i < heads);
+                    raw[i] = fetch_place(from + (h + i) * a.query.head, place, r < end && h + i < heads);
 #pragma unroll
                 for (int i = 0; i < kTogether; ++i) {
                     float v[8];
-                    turn8<T, INTERLEAVED>(raw[i], turn, at, a.rotary_dim, mate, v);
-                    if (r < end && h + i < heads) store8<T>(to + (h + i) * (2 * D), v);
+                    turn8<T, INTERLEAVED>(raw[i], turn, place, v);
+                    if (r < end && h + i < heads) {
+                        char* const out = to + (h + i) * (2 * D);
+                        *reinterpret_cast<uint2*>(out + 2 * place.low) = make_uint2(T::pack(v[0], v[1]), T::pack(v[2], v[3]));
+                        *reinterpret_cast<uint2*>(out + 2 * place.high) = make_uint2(T::pack(v[4], v[5]), T::pack(v[6], v[7]));
+                    }
                 }
             }
         }
@@ -179,10 +188,10 @@ __global__ void __launch_bounds__(256, 3) append_kernel(const __grid_constant__ 
         return;
     }
     char* codes = reinterpret_cast<char*>(a.c.codes) + side * a.c.side_pitch + block * a.c.block_pitch +
-                  head * a.c.head_pitch + at;
+                  head * a.c.head_pitch;
     float* scale_at = reinterpret_cast<float*>(a.c.scales) + (block * 2 + side) * a.c.kv_heads + head;
     const Rows& from = side ? a.value : a.key;
-    const char* rows = from.at + head * from.head + 2 * at + (run.row - run.first) * from.token;
+    const char* rows = from.at + head * from.head + (run.row - run.first) * from.token;
     const float held = run.first ? *scale_at : 0.0f;
     uint4 raw[kHeld];
     float top = 0.0f, scale = 0.0f, by = 0.0f;
@@ -195,7 +204,8 @@ __global__ void __launch_bounds__(256, 3) append_kernel(const __grid_constant__ 
 #pragma unroll
                 for (int i = 0; i < kHeld; ++i) {
                     const int r = first + i * kRows + sub;
-                    raw[i] = fetch16(rows + r * from.token, r < end);
+                    if (turned) raw[i] = fetch_place(rows + r * from.token, place, r < end);
+                    else raw[i] = fetch16(rows + r * from.token + 2 * at, r < end);
                 }
             }
             if (turned) {
@@ -205,10 +215,15 @@ __global__ void __launch_bounds__(256, 3) append_kernel(const __grid_constant__ 
                     if (first + i * kRows >= end) break;
                     Turn turn;
                     float v[8];
-                    fetch_turn<INTERLEAVED>(turn, a, base + r, at, r < end);
-                    turn8<T, INTERLEAVED>(raw[i], turn, at, a.rotary_dim, mate, v);
-                    if (pass == 0) top = max8(v, top);
-                    else if (r < end) store_codes(codes + r * a.c.token_pitch, v, by);
+                    fetch_turn(turn, a, base + r, place, r < end);
+                    turn8<T, INTERLEAVED>(raw[i], turn, place, v);
+                    if (pass == 0) {
+                        top = max8(v, top);
+                    } else if (r < end) {
+                        const uint2 both = codes_of(v, by);
+                        *reinterpret_cast<uint32_t*>(codes + r * a.c.token_pitch + place.low) = both.x;
+                        *reinterpret_cast<uint32_t*>(codes + r * a.c.token_pitch + place.high) = both.y;
+                    }
                 }
             } else if (pass == 0) {
                 top = fmaxf(top, largest<T>(raw));
@@ -218,7 +233,7 @@ __global__ void __launch_bounds__(256, 3) append_kernel(const __grid_constant__ 
                     const int r = first + i * kRows + sub;
                     float v[8];
                     widen8<T>(raw[i], v);
-                    if (r < end) store_codes(codes + r * a.c.token_pitch, v, by);
+                    if (r < end) store_codes(codes + r * a.c.token_pitch + at, v, by);
                 }
             }
         }
@@ -227,8 +242,8 @@ __global__ void __launch_bounds__(256, 3) append_kernel(const __grid_constant__ 
     if (!run.first || scale > held) {
         for (int r = sub; r < run.first; r += kRows) {                 // older tokens, at the grown scale
             float v[8];
-            load_codes(codes + r * a.c.token_pitch, held, v);
-            store_codes(codes + r * a.c.token_pitch, v, by);
+            load_codes(codes + r * a.c.token_pitch + at, held, v);
+            store_codes(codes + r * a.c.token_pitch + at, v, by);
         }
         __syncwarp();
         if (lane == 0) *scale_at = scale;
@@ -310,26 +325,26 @@ __global__ void __launch_bounds__(256, 4) compress_kernel(const __grid_constant_
     if (lane == 0) *unit.scale = scale;
 }
 
-// A lane takes 16 codes, so that both sides move in 16-byte accesses.
+// 8 codes a lane, so that a store instruction's 16 bytes a lane are whole lines (16 codes a lane wrote
+// every other 16 bytes: 5.1 TB/s where this reaches 6.6).
 template <typename T, int D>
 __global__ void __launch_bounds__(256, 4) expand_kernel(const __grid_constant__ ConvertArgs a) {
-    constexpr int kLanes = D / 16, kRows = 32 / kLanes, kSteps = kGranule / kRows;
-    const int lane = threadIdx.x % 32, sub = lane / kLanes, at = lane % kLanes * 16;
+    constexpr int kLanes = D / 8, kRows = 32 / kLanes, kSteps = kGranule / kRows;
+    const int lane = threadIdx.x % 32, sub = lane / kLanes, at = lane % kLanes * 8;
     ConvertUnit unit;
     if (!convert_unit(a, unit)) return;
     const float scale = *unit.scale;
     for (int first = sub; first < a.block_size; first += kGranule) {
-        uint4 raw[kSteps];
+        uint2 raw[kSteps];
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) raw[i] = fetch16(unit.codes + (first + i * kRows) * unit.token + at, true);
+        for (int i = 0; i < kSteps; ++i) raw[i] = fetch8(unit.codes + (first + i * kRows) * unit.token + at, true);
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
             float v[8];
+            widen_codes(raw[i], scale, v);
             char* to = unit.wide + (first + i * kRows) * unit.wide_token + 2 * at;
-            widen_codes(make_uint2(raw[i].x, raw[i].y), scale, v);
-            store8<T>(to, v);
-            widen_codes(make_uint2(raw[i].z, raw[i].w), scale, v);
-            store8<T>(to + 16, v);
+            const uint4 x = make_uint4(T::pack(v[0], v[1]), T::pack(v[2], v[3]), T::pack(v[4], v[5]), T::pack(v[6], v[7]));
+            *reinterpret_cast<uint4*>(to) = x;
         }
     }
 }

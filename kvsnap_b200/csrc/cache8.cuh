@@ -66,6 +66,14 @@ __device__ __forceinline__ uint4 fetch16(const char* at, bool there) {
     return v;
 }
 
+__device__ __forceinline__ uint2 fetch8(const char* at, bool there) {
+    uint2 v;
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %3, 0;\nmov.u32 %0, 0;\nmov.u32 %1, 0;\n"
+                 "@p ld.global.v2.u32 {%0,%1}, [%2];\n}"
+                 : "=&r"(v.x), "=&r"(v.y) : "l"(at), "r"(uint32_t(there)));
+    return v;
+}
+
 // 8 consecutive 16-bit elements.
 template <typename T>
 __device__ __forceinline__ void widen8(const uint4& x, float (&v)[8]) {
@@ -108,12 +116,16 @@ __device__ __forceinline__ void load_codes(const char* at, float by, float (&v)[
 }
 
 // Nearest codes of v * by (ties to even); beyond +-448, infinities included, +-448.
-__device__ __forceinline__ void store_codes(char* at, const float (&v)[8], float by) {
+__device__ __forceinline__ uint2 codes_of(const float (&v)[8], float by) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
         w[i] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * i] * by, v[2 * i + 1] * by), __NV_SATFINITE, __NV_E4M3);
-    *reinterpret_cast<uint2*>(at) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+    return make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+}
+
+__device__ __forceinline__ void store_codes(char* at, const float (&v)[8], float by) {
+    *reinterpret_cast<uint2*>(at) = codes_of(v, by);
 }
 
 // ---- scales ------------------------------------------------------------------------
