@@ -97,8 +97,13 @@ struct Parts {
 // ---- few rows: decode -------------------------------------------------------------------
 //
 // Sequences with at most kStepRows rows a KV head (query heads of the group times
-// new tokens). Bound by the cache's bytes, so nothing but a page's codes is read,
-// once. A warp copies a granule of 16 tokens to its own shared memory
+// new tokens): what m16n8k16 products take without idle rows, while the kernel below works on 256 rows
+// whatever there are (16 sequences of 8000 tokens with 8 rows a head: 61 us, there 153; with 16 rows 113).
+// Bound by the cache's bytes, so nothing but a page's codes is read, once: a step of 64 sessions of 512 to
+// 8192 tokens with 8 heads of 128, 372 MB, takes 79 us, 4.7 TB/s, of which the loop over granules runs at 86 %
+// of the rate of a plain copy, and the rest is the scan for a CTA's chunks (2 us), the first copies'
+// way and the merge of a CTA's slices (2 us a unit). With few sequences those are what bounds it: 27 us for
+// one of 32k tokens, whose 67 MB are 10 us. A warp copies a granule of 16 tokens to its own shared memory
 // asynchronously, kAhead granules ahead, no warp waiting for another; 8 lanes copy
 // one token's line, as 16-byte requests are joined among 8 lanes (with lanes that
 // each fetched the codes of their own fragments, 32 bytes of a line a request, this
@@ -658,7 +663,8 @@ __global__ void __launch_bounds__(32 * kWarps, 1) step_kernel(const __grid_const
 
 // Joins the parts of the shared unit that CTA blockIdx.x of the kernel before began, which lie in
 // consecutive CTAs' slots. Where units have few parts (WIDE false) a warp takes a row, else a CTA does,
-// its warps a share of the parts each.
+// its warps a share of the parts each. Bound by the way to a part and back, 4 parts at once: 6 to 8 us
+// with nothing in the caches, of which the launch is hidden behind the kernel before.
 constexpr int kJoinWarps = 8;
 
 template <typename T, int D, bool WIDE>
@@ -726,8 +732,11 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
 
 // ---- many rows: chunks and prompts --------------------------------------------------------
 //
-// Sequences that the kernel above does not take. Bound by the tensor cores: 4 D operations a
-// query head and visible token, in two products of fp16 operands with 32-bit sums in tensor memory.
+// Sequences that the kernel above does not take. 4 D operations a query head and visible token, in two
+// products of fp16 operands with 32-bit sums in tensor memory: 0.66 to 0.70 ms for an 8k prompt of 32 heads
+// of 128, 790 to 830 TFLOP/s, half of what a plain product reaches. What bounds it are the softmax warps: the
+// weights' exponentials and what surrounds them take about 1900 clocks a step of both row tiles, the
+// tensor cores' part 1300. Chunks that do not fill 256 rows pay for the rows that they lack.
 // A CTA takes 256 rows (two tiles of 128) of one KV head in steps of 64 tokens:
 //   warp 13     looks up the pages of coming steps and their scales;
 //   warps 8-11  load a step's codes, one step ahead, turn them to fp16 and lay them out for the tensor
@@ -739,7 +748,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
 // (4 x 64). With one step of 128 tokens instead, scores and softmax took turns: 1.02 ms for an 8k
 // prompt of 32 heads.
 // The running maximum follows a row's true maximum only when that exceeds it by 2^14 (weights stay
-// within fp16), so sums in tensor memory are rarely touched. A page's scale goes into the conversion
+// within fp16), so sums in tensor memory are rarely touched (followed at every step: an 8k prompt 738 us,
+// so 662). A page's scale goes into the conversion
 // relative to the largest key scale of the tile (which multiplies S) and the largest value scale so
 // far (which divides O at the end): powers of two, exact in fp16.
 
@@ -749,7 +759,8 @@ constexpr int kStep = 64;                  // tokens a step
 constexpr int kGranules = kStep / kGranule;
 constexpr int kStages = 4;                 // steps of keys and of values in shared memory
 // What a unit costs besides its steps (queries in, sums out, the pipeline's filling), in steps: work is
-// cut by steps and this, as a CTA with many short units was 1.6 times as long as others without it.
+// cut by steps and this (by steps alone an 8k prompt takes 778 us, so 662: a CTA with many short units was
+// 1.6 times as long as others).
 constexpr int kUnitCost = 8;
 constexpr int kConvertWarps = 4, kIssueWarp = 12, kLookWarp = 13, kChunkThreads = 512;
 constexpr int kLooked = 16;                // steps looked up ahead
@@ -968,7 +979,7 @@ __device__ __forceinline__ void mma_tensor(uint32_t d, uint32_t a, uint32_t b, u
                  ::"r"(d), "r"(a), "r"(b), "r"(what), "r"(add), "r"(chosen), "r"(kMatrixHigh) : "memory");
 }
 
-// 32 columns of the warp's 32 rows of tensor memory, a row a lane.
+// Columns of the warp's 32 rows of tensor memory, a row a lane.
 __device__ __forceinline__ void tensor_load(uint32_t at, float (&v)[32]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
@@ -988,6 +999,7 @@ __device__ __forceinline__ void tensor_load(uint32_t at, float (&v)[16]) {
         : "r"(at));
 }
 
+// The loads so far, and that `v` comes from them.
 __device__ __forceinline__ void tensor_loaded(float (&v)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
         : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
@@ -1061,7 +1073,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return d;
 }
 
-// The loads so far, and that `v` comes from them.
 __device__ __forceinline__ void tensor_loaded(float (&v)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
         : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
@@ -1725,13 +1736,15 @@ Plan plan_for(const Cache& c, const Batch& b, int q_heads, int sms) {
     const int64_t most_rows = int64_t(group) * (b.max_query < b.rows ? b.max_query : b.rows);
     plan.chunked = most_rows > kStepRows;
     plan.most_rows = int(most_rows);
-    // With one sequence, the kernel for many rows takes it whatever it holds: one launch, not two.
+    // With one sequence, the kernel for many rows takes it whatever it holds: one launch, not two (a prompt
+    // of 300 tokens 29.3 us, else 32.8).
     plan.stepped = group <= kStepRows && !(plan.chunked && b.seqs == 1);
     plan.step_rows = plan.stepped ? kStepRows : 0;
     plan.wide = most_rows > 8;
     // Heads a CTA: up to 8, whose lines of a token lie side by side; but few sequences are spread over CTAs by
-    // heads, so that a unit's tokens are cut among fewer CTAs (with 8, a 32k step of one sequence left 148
-    // parts of each row to join, and a 129-token one was one CTA's).
+    // heads, so that a unit's tokens are cut among fewer CTAs (of 8 heads, 1 sequence of 8191 tokens takes
+    // 15.1 us, with all heads in a CTA 21.0, and 16 sequences 60.5 and 66.5; with a head a CTA 48 sequences
+    // of 4000 take 87.5, and 81.9 by this rule, 64 of 200 29.4 and 17.0).
     p.hc = 1;
     for (int heads = 8; heads > 1; --heads)
         if (c.kv_heads % heads == 0 && int64_t(b.seqs) * (c.kv_heads / heads) >= kSpread) {
@@ -1740,11 +1753,16 @@ Plan plan_for(const Cache& c, const Batch& b, int q_heads, int sms) {
         }
     p.ts = kWarps / p.hc, p.hg = c.kv_heads / p.hc;
     const int64_t most = (int64_t(b.width) * c.block_size + p.ts * kGranule - 1) / (p.ts * kGranule);
-    // Up to 8 chunks a unit, a CTA each: cutting them would cost more (a scan of the lengths,
-    // parts and their join) than a few granules in turn.
-    plan.split = most > 8;
     plan.ctas = sms;
     plan.step_units = int64_t(b.seqs) * p.hg;
+    // Cutting the chunks evenly over the CTAs costs a scan of the lengths, merges of parts and a join: as
+    // much as 4 chunks in turn, more with more units, up to 20. It saves at most the longest unit's chunks
+    // less an even share, taken at half of what the table could hold. Cut and uncut, in us: 1 sequence of
+    // 1300 tokens 13.7 and 15.0, of 4000 14.3 and 23.3; 64 of 300 24.5 and 19.1, of 1000 41.4 and 41.7; of
+    // mixed lengths up to 1000 29.5 and 39.7; 128 of 700 47.8 and 40.7.
+    const int64_t waves = (plan.step_units + sms - 1) / sms;
+    const int64_t costs = 4 + (plan.step_units < 96 ? plan.step_units : 96) / 6;
+    plan.split = most * (2 * sms * waves - plan.step_units) > costs * 2 * sms;
     plan.step_ctas = plan.split ? plan.ctas : plan.step_units;
     const int64_t step_slot = plan.stepped && plan.split ? p.hc * kStepRows : 0;
     const int64_t chunk_slot = plan.chunked ? kUnitRows : 0;
@@ -1791,7 +1809,8 @@ void launch_step(const Plan& plan, const StepArgs& p, cudaStream_t stream) {
 
 template <typename T, int D>
 void launch_attend(const Plan& plan, const AttendArgs& a, Parts parts, cudaStream_t stream) {
-    // `units` of the step kernel bound how many parts a unit has.
+    // Few units have many parts each, and a CTA joins a row (8 units' 8191 tokens 15.1 us, a warp a row 17.0);
+    // many have few, and a warp does (chunks of 128 tokens in 24 sequences 282 us, a CTA a row 360).
     const auto join = [&](int64_t units) {
         const unsigned rows = unsigned(parts.heads * parts.used_rows), ctas = unsigned(plan.ctas);
         if (units * 8 <= plan.ctas) launch(join_kernel<T, D, true>, dim3(ctas, rows), 32 * kJoinWarps, 0, stream, true, a, parts);

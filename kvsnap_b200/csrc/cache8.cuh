@@ -90,12 +90,6 @@ __device__ __forceinline__ void load8(const char* at, float (&v)[8]) {
     widen8<T>(*reinterpret_cast<const uint4*>(at), v);
 }
 
-template <typename T>
-__device__ __forceinline__ void store8(char* at, const float (&v)[8]) {
-    *reinterpret_cast<uint4*>(at) =
-        make_uint4(T::pack(v[0], v[1]), T::pack(v[2], v[3]), T::pack(v[4], v[5]), T::pack(v[6], v[7]));
-}
-
 __device__ __forceinline__ float2 from_e4m3x2(uint32_t v) {
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(v), __NV_E4M3);
     return __half22float2(__half2(h));
