@@ -15,8 +15,9 @@ the host link in half the time, scales included.
     out = cache.attend(name, query, batch)
 
 Every call runs on the caller's current stream of the cache's device, allocates only its outputs and
-workspaces there, never waits for the GPU, and can be captured into a CUDA graph. Tables and lengths are
-read on the GPU; what a kernel finds wrong with them it skips and records, and ``check()`` raises.
+workspaces there, never waits for the GPU, and can be captured into a CUDA graph (block ids given as lists
+are copied to the GPU first: both need tensors). Tables and lengths are read on the GPU; what a kernel finds
+wrong with them it skips and records, and ``check()`` raises. For serving: no gradients are taken.
 """
 from __future__ import annotations
 
@@ -84,6 +85,8 @@ class PagedBatch:
         seqs = lengths.shape[0]
         if table.shape[0] != seqs or start.shape[0] != seqs + 1:
             raise ValueError("table, start and lengths must describe the same sequences")
+        if max(table.shape) >= 1 << 30:
+            raise ValueError("the block table is too large")
         if max_query is not None and (type(max_query) is not int or max_query < 0):
             raise ValueError("max_query must be a non-negative int")
         self.table, self.start, self.lengths, self.max_query = table, start, lengths, max_query
@@ -97,7 +100,7 @@ class PagedBatch:
         if record is None:
             if len(self._records) > 64:
                 self._records.clear()
-            record = _abi.C8Batch(*self._addresses, rows, rows if self.max_query is None else self.max_query)
+            record = _abi.C8Batch(*self._addresses, rows, rows if self.max_query is None else min(rows, self.max_query))
             self._records[rows] = record
         return record
 
@@ -288,7 +291,9 @@ class PagedCache8:
         return CacheConverter(self, caches)
 
     def check(self):
-        """Wait for the calls so far and raise ``ValueError`` if a kernel met an argument it had to skip."""
+        """Wait for the calls so far, on all streams, and raise ``ValueError`` if a kernel met an argument it had to skip."""
+        import torch
+        torch.cuda.synchronize(self.device)
         found = int(self.status.item())
         if found:
             self.status.zero_()
@@ -356,7 +361,7 @@ class CacheConverter:
 
         ``num_kv_tokens``: tokens that the blocks hold, in order; slots behind the last become zeros, as a
         save zeroes them (None: every slot counts). Block ids are lists, or int64 tensors on the cache's
-        device (no copy then). A target block must not be named twice.
+        device. A target block must not be named twice.
         """
         if num_kv_tokens is not None and (type(num_kv_tokens) is not int or num_kv_tokens < 0):
             raise ValueError("num_kv_tokens must be a non-negative int")

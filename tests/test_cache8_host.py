@@ -132,6 +132,13 @@ def test_appends_it_refuses(make, change, match):
         make().append("l", arguments.pop("key"), arguments.pop("value"), batch(), **arguments)
 
 
+def test_a_bound_of_rows_beyond_32_bits():
+    """The C record's fields have 32 bits: a bound above the call's rows says no more than they do."""
+    assert [batch(max_query=q)._for(7).max_query for q in (None, 2, 7, 2 ** 32 + 1)] == [7, 2, 7, 7]
+    with pytest.raises(ValueError, match="too large"):
+        batch(seqs=1, width=1 << 30)
+
+
 def test_layers_and_devices_it_refuses(make):
     cache = make()
     with pytest.raises(KeyError, match="nowhere"):

@@ -147,6 +147,15 @@ def test_attend_chunk(shape, sequences):
     check_attend(Paged(sequences, dim=dim, block_size=block_size, heads=heads, poison=True), dtype, group)
 
 
+@pytest.mark.parametrize("count,longest,heads,group", [
+    (64, 300, 8, 4), (64, 900, 8, 2), (130, 250, 8, 1), (12, 2100, 8, 4), (3, 2600, 8, 2), (160, 100, 1, 8), (5, 1500, 3, 4)])
+def test_attend_steps_cut_or_not(count, longest, heads, group):
+    """Batches on both sides of the rule that cuts a step's work: many units of several chunks, uneven and even."""
+    even, uneven = [(1, longest)] * count, [(1 + s % 2, s * 37 % longest) for s in range(count)]
+    for sequences in (even, uneven):
+        check_attend(Paged(sequences, dim=64, heads=heads, poison=True), torch.bfloat16, group)
+
+
 @pytest.mark.parametrize("order", ["sides", "heads", "beside"])
 @pytest.mark.parametrize("sequences", [[(1, 200), (1, 31)], [(40, 75), (2, 9)]], ids=str)
 def test_attend_storage_orders(order, sequences):
@@ -552,6 +561,21 @@ def test_calls_run_on_the_current_stream():
     side.synchronize()
     assert torch.equal(got, expected)
     p.cache.check()
+
+
+def test_check_waits_for_calls_on_other_streams():
+    p = Paged([(1, 40), (1, 70)], heads=2)
+    p.batch.table[1, 2] = -1
+    q = p.random(4, torch.bfloat16)[1]
+    x = torch.randn((8192, 8192), device="cuda")
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(20):                                 # tens of milliseconds ahead of the call
+            x @ x
+        p.cache.attend("l", q, p.batch)
+    with pytest.raises(ValueError, match="block id"):
+        p.cache.check()
 
 
 def test_the_first_call_of_a_process_may_be_captured():
