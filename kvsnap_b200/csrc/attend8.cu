@@ -5,10 +5,7 @@
 // meet queries and weights as fp16 (e4m3 is exact in it) in matrix instructions
 // with 32-bit sums; a page's key scale multiplies its scores, its value scale its
 // weights, both in 32 bits.
-#include <mutex>
-#include <set>
 #include <type_traits>
-#include <utility>
 
 #include "cache8.cuh"
 
@@ -1773,31 +1770,6 @@ Plan plan_for(const Cache& c, const Batch& b, int q_heads, int sms) {
                                   plan.ctas * int64_t(sizeof(SharedUnit))
                             : 0;
     return plan;
-}
-
-// Raise a kernel's shared memory limit on the current device, once per kernel and device.
-void allow_shared(const void* kernel, int bytes) {
-    static std::mutex mu;
-    static std::set<std::pair<const void*, int>> done;
-    int device = 0;
-    check(cudaGetDevice(&device));
-    std::lock_guard<std::mutex> hold(mu);
-    if (done.count({kernel, device})) return;
-    check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    done.insert({kernel, device});
-}
-
-template <typename K, typename... A>
-void launch(K kernel, dim3 grid, int threads, size_t shared, cudaStream_t stream, bool after, const A&... args) {
-    if (shared > 48 << 10) allow_shared(reinterpret_cast<const void*>(kernel), int(shared));
-    cudaLaunchConfig_t config{};
-    config.gridDim = grid, config.blockDim = dim3(unsigned(threads));
-    config.dynamicSmemBytes = shared, config.stream = stream;
-    cudaLaunchAttribute attribute{};
-    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attribute.val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = &attribute, config.numAttrs = after ? 1 : 0;
-    check(cudaLaunchKernelEx(&config, kernel, args...));
 }
 
 template <typename T, int D, int NT>

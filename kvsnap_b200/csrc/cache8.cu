@@ -111,18 +111,18 @@ constexpr int kHeld = 8;      // row groups of a page that a warp keeps in regis
 
 // The largest finite size among a warp's rows: of the 16-bit words as they are, and where that is no
 // finite number, once more without those that are not.
-template <typename T>
-__device__ __forceinline__ float largest(const uint4 (&raw)[kHeld]) {
+template <typename T, int N>
+__device__ __forceinline__ float largest(const uint4 (&raw)[N]) {
     uint32_t tops = 0;
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i)
+    for (int i = 0; i < N; ++i)
         tops = T::max_size(T::max_size(T::max_size(T::max_size(tops, raw[i].x), raw[i].y), raw[i].z), raw[i].w);
     const float2 pair = T::wide(tops);
     float top = warp_max(fmaxf(pair.x, pair.y));
     if (top > 3.402823466e38f) {
         top = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kHeld; ++i) {
+        for (int i = 0; i < N; ++i) {
             float v[8];
             widen8<T>(raw[i], v);
             top = max8(v, top);
@@ -132,58 +132,78 @@ __device__ __forceinline__ float largest(const uint4 (&raw)[kHeld]) {
     return top;
 }
 
-// One CTA: a page, and 8 key or value heads, a warp each, or 8 query heads, of which each warp has some
-// rows (of a single row, a head). A row is D / 8 lanes of 8 elements, so a warp takes 256 / D rows a step.
-// Turned: (x cos - y sin, y cos + x sin) of each pair, in 32 bits. Bound by memory: a warp's loads are
-// issued together (4 KB of keys or values, 2 KB of queries), and predicated. A row's angles are fetched once
-// for 8 query heads. Keys are held as they come and turned twice, for the scale and for the codes: turned
-// they would take twice the registers. An 8k prompt of 32 and 8 heads of 128 takes 49 us, 3.8 TB/s of its
-// 184 MB (half of the plain copy's rate: 16 warps an SM wait for their loads; with registers for 24 a part
-// of the pages held was spilled), a token of each of 64 sequences 7.5 us, which is a launch and two
-// fetches, one after the other, with nothing in the caches.
+template <int N>
+__device__ __forceinline__ float largest(const float (&v)[N][8]) {
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(v[i][k]));        // of a number and NaN, the number
+    top = warp_max(top);
+    if (top > 3.402823466e38f) {
+        top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) top = max8(v[i], top);
+        top = warp_max(top);
+    }
+    return top;
+}
+
+// Append: one CTA takes page blockIdx.x and 8 key or value heads, a warp each, or 8 query heads. A row is
+// D / 8 lanes of 8 elements, so a warp takes 256 / D rows at a time. Turned: (x cos - y sin, y cos + x sin) of
+// each pair, in 32 bits. Bound by memory, so all loads of a warp are issued together, predicated. Keys and
+// values hold a page's rows in registers from their fetch to their codes, as the scale needs all rows
+// first (128 registers a thread); queries are turned as they come (64). An 8k prompt of 32 and 8 heads of
+// 128: the queries' 134 MB in 20 us, 6.6 TB/s; the keys' and values' 50 MB in 18 us, bound by the way of the
+// loads of 16 warps an SM (turned twice from what had come, for the scale and for the codes, 28 us).
+
+// 8 query heads of a page's rows from 8 y on, of which each warp takes some rows (of a single row, a head). A
+// row's angles are fetched once for the 8.
 template <typename T, int D, bool SINGLE, bool INTERLEAVED>
-__global__ void __launch_bounds__(256, 2) append_kernel(const __grid_constant__ AppendArgs a) {
+__device__ __forceinline__ void turn_queries(const AppendArgs& a, int y) {
     constexpr int kLanes = D / 8, kRows = 32 / kLanes, kTogether = SINGLE ? 1 : 8;
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, n = a.c.block_size;
-    const int kv_ctas = (2 * a.c.kv_heads + 7) / 8, slot = blockIdx.y * 8 + warp;
-    const bool queries = blockIdx.y >= kv_ctas;
-    if (!queries && slot >= 2 * a.c.kv_heads) return;
+    PageRun run;
+    if (!find_page<SINGLE>(a.b, n, blockIdx.x, run, a.status)) return;
+    const int sub = lane / kLanes, end = run.first + run.count;
+    const int base = run.page * n;                               // position of the page's slot 0
+    const Place place(lane % kLanes, a.rotary_dim, INTERLEAVED);
+    const int head = y * 8 + (SINGLE ? warp : 0), heads = min(SINGLE ? 1 : 8, a.q_heads - head);
+    for (int first = run.first + (SINGLE ? 0 : warp * kRows); first < end; first += 8 * kRows) {
+        const int r = first + sub;
+        const int64_t row = run.row + (r - run.first);
+        const char* from = a.query.at + row * a.query.token + head * a.query.head;
+        char* to = a.query_out + (row * a.q_heads + head) * (2 * D);
+        Turn turn;
+        fetch_turn(turn, a, base + r, place, r < end);
+        uint4 raw[kTogether];
+#pragma unroll
+        for (int i = 0; i < kTogether; ++i) raw[i] = fetch_place(from + i * a.query.head, place, r < end && i < heads);
+#pragma unroll
+        for (int i = 0; i < kTogether; ++i) {
+            float v[8];
+            turn8<T, INTERLEAVED>(raw[i], turn, place, v);
+            if (r < end && i < heads) {
+                char* const out = to + i * (2 * D);
+                *reinterpret_cast<uint2*>(out + 2 * place.low) = make_uint2(T::pack(v[0], v[1]), T::pack(v[2], v[3]));
+                *reinterpret_cast<uint2*>(out + 2 * place.high) = make_uint2(T::pack(v[4], v[5]), T::pack(v[6], v[7]));
+            }
+        }
+    }
+}
+
+// Key and value heads from 8 y on: the values' behind the keys'.
+template <typename T, int D, bool SINGLE, bool INTERLEAVED>
+__device__ __forceinline__ void append_rows(const AppendArgs& a, int y) {
+    constexpr int kLanes = D / 8, kRows = 32 / kLanes, kHeld = SINGLE ? 1 : ::kHeld;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, n = a.c.block_size, slot = y * 8 + warp;
+    if (slot >= 2 * a.c.kv_heads) return;
     PageRun run;
     if (!find_page<SINGLE>(a.b, n, blockIdx.x, run, a.status)) return;
     const int sub = lane / kLanes, at = lane % kLanes * 8, end = run.first + run.count;
     const int base = run.page * n;                               // position of the page's slot 0
     if (a.rotary_dim && base + end > a.positions && threadIdx.x == 0) atomicOr(a.status, KVSNAP_C8_BAD_POSITION);
     const Place place(lane % kLanes, a.rotary_dim, INTERLEAVED);
-
-    if (queries) {
-        // (one row: a head a warp)
-        const int head = (blockIdx.y - kv_ctas) * 8 + (SINGLE ? warp : 0), heads = min(SINGLE ? 1 : 8, a.q_heads - head);
-        for (int first = run.first + (SINGLE ? 0 : warp * kRows); first < end; first += 8 * kRows) {
-            const int r = first + sub;
-            const int64_t row = run.row + (r - run.first);
-            const char* from = a.query.at + row * a.query.token + head * a.query.head;
-            char* to = a.query_out + (row * a.q_heads + head) * (2 * D);
-            Turn turn;
-            fetch_turn(turn, a, base + r, place, r < end);
-            for (int h = 0; h < heads; h += kTogether) {
-                uint4 raw[kTogether];
-#pragma unroll
-                for (int i = 0; i < kTogether; ++i)
-                    raw[i] = fetch_place(from + (h + i) * a.query.head, place, r < end && h + i < heads);
-#pragma unroll
-                for (int i = 0; i < kTogether; ++i) {
-                    float v[8];
-                    turn8<T, INTERLEAVED>(raw[i], turn, place, v);
-                    if (r < end && h + i < heads) {
-                        char* const out = to + (h + i) * (2 * D);
-                        *reinterpret_cast<uint2*>(out + 2 * place.low) = make_uint2(T::pack(v[0], v[1]), T::pack(v[2], v[3]));
-                        *reinterpret_cast<uint2*>(out + 2 * place.high) = make_uint2(T::pack(v[4], v[5]), T::pack(v[6], v[7]));
-                    }
-                }
-            }
-        }
-        return;
-    }
 
     const int side = slot / a.c.kv_heads, head = slot % a.c.kv_heads;
     const int64_t block = ints(a.b.table)[run.seq * a.b.table_pitch + run.page];
@@ -197,41 +217,57 @@ __global__ void __launch_bounds__(256, 2) append_kernel(const __grid_constant__ 
     const Rows& from = side ? a.value : a.key;
     const char* rows = from.at + head * from.head + (run.row - run.first) * from.token;
     const float held = run.first ? *scale_at : 0.0f;
-    uint4 raw[kHeld];
-    float top = 0.0f, scale = 0.0f, by = 0.0f;
-    const bool turned = side == 0 && a.rotary_dim;
+    float scale = 0.0f, by = 0.0f;
+    const auto sized = [&](float top) { scale = fmaxf(held, needed_scale(top)), by = inverse(scale); };
     // The largest size of all rows, then their codes; rows too many to hold are fetched twice.
+    const int together = kHeld * kRows, passes = run.count > together ? 2 : 1;
+    float top = 0.0f;
+    if (side == 0 && a.rotary_dim) {
 #pragma unroll 1
-    for (int pass = 0; pass < 2; ++pass) {
-        for (int first = run.first; first < end; first += kHeld * kRows) {
-            if (pass == 0 || run.count > kHeld * kRows) {
+        for (int pass = 0; pass < passes; ++pass)
+            for (int first = run.first; first < end; first += together) {
+                float v[kHeld][8];
+                uint4 raw[kHeld];
+                constexpr int kTurns = SINGLE ? 1 : kHeld - 2;      // on their way together: all would be spilled
+                Turn turn[kTurns];
 #pragma unroll
                 for (int i = 0; i < kHeld; ++i) {
                     const int r = first + i * kRows + sub;
-                    if (turned) raw[i] = fetch_place(rows + r * from.token, place, r < end);
-                    else raw[i] = fetch16(rows + r * from.token + 2 * at, r < end);
+                    if (i < kTurns) fetch_turn(turn[i], a, base + r, place, r < end);
+                    raw[i] = fetch_place(rows + r * from.token, place, r < end);
                 }
-            }
-            if (turned) {
+#pragma unroll
+                for (int i = 0; i < kHeld; ++i) {
+                    turn8<T, INTERLEAVED>(raw[i], turn[i % kTurns], place, v[i]);
+                    const int next = i + kTurns, r = first + next * kRows + sub;
+                    if (next < kHeld) fetch_turn(turn[i], a, base + r, place, r < end);
+                }
+                if (pass == 0) top = fmaxf(top, largest(v));
+                if (pass + 1 < passes) continue;
+                sized(top);
 #pragma unroll
                 for (int i = 0; i < kHeld; ++i) {
                     const int r = first + i * kRows + sub;
-                    if (first + i * kRows >= end) break;
-                    Turn turn;
-                    float v[8];
-                    fetch_turn(turn, a, base + r, place, r < end);
-                    turn8<T, INTERLEAVED>(raw[i], turn, place, v);
-                    if (pass == 0) {
-                        top = max8(v, top);
-                    } else if (r < end) {
-                        const uint2 both = codes_of(v, by);
+                    const uint2 both = codes_of(v[i], by);
+                    if (r < end) {
                         *reinterpret_cast<uint32_t*>(codes + r * a.c.token_pitch + place.low) = both.x;
                         *reinterpret_cast<uint32_t*>(codes + r * a.c.token_pitch + place.high) = both.y;
                     }
                 }
-            } else if (pass == 0) {
-                top = fmaxf(top, largest<T>(raw));
-            } else {
+            }
+    } else {
+#pragma unroll 1
+        for (int pass = 0; pass < passes; ++pass)
+            for (int first = run.first; first < end; first += together) {
+                uint4 raw[kHeld];
+#pragma unroll
+                for (int i = 0; i < kHeld; ++i) {
+                    const int r = first + i * kRows + sub;
+                    raw[i] = fetch16(rows + r * from.token + 2 * at, r < end);
+                }
+                if (pass == 0) top = fmaxf(top, largest<T>(raw));
+                if (pass + 1 < passes) continue;
+                sized(top);
 #pragma unroll
                 for (int i = 0; i < kHeld; ++i) {
                     const int r = first + i * kRows + sub;
@@ -240,8 +276,6 @@ __global__ void __launch_bounds__(256, 2) append_kernel(const __grid_constant__ 
                     if (r < end) store_codes(codes + r * a.c.token_pitch + at, v, by);
                 }
             }
-        }
-        if (pass == 0) scale = fmaxf(held, needed_scale(warp_max(top))), by = inverse(scale);
     }
     if (!run.first || scale > held) {
         for (int r = sub; r < run.first; r += kRows) {                 // older tokens, at the grown scale
@@ -252,6 +286,31 @@ __global__ void __launch_bounds__(256, 2) append_kernel(const __grid_constant__ 
         __syncwarp();
         if (lane == 0) *scale_at = scale;
     }
+}
+
+// One row a sequence: a token of each of 64 sequences takes 5.3 us, which is a launch and two fetches, one
+// after the other, with nothing in the caches.
+template <typename T, int D, bool INTERLEAVED>
+__global__ void __launch_bounds__(256, 4) append_one_kernel(const __grid_constant__ AppendArgs a) {
+    const int kv_ctas = (2 * a.c.kv_heads + 7) / 8;
+    if (blockIdx.y < kv_ctas) append_rows<T, D, true, INTERLEAVED>(a, blockIdx.y);
+    else turn_queries<T, D, true, INTERLEAVED>(a, blockIdx.y - kv_ctas);
+}
+
+// The queries too where the grid has CTAs for them; otherwise they are turn_kernel's, whose CTAs start as
+// these end.
+template <typename T, int D, bool INTERLEAVED>
+__global__ void __launch_bounds__(256, 2) append_kernel(const __grid_constant__ AppendArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;");
+    const int kv_ctas = (2 * a.c.kv_heads + 7) / 8;
+    if (blockIdx.y < kv_ctas) append_rows<T, D, false, INTERLEAVED>(a, blockIdx.y);
+    else turn_queries<T, D, false, INTERLEAVED>(a, blockIdx.y - kv_ctas);
+}
+
+template <typename T, int D, bool INTERLEAVED>
+__global__ void __launch_bounds__(256, 4) turn_kernel(const __grid_constant__ AppendArgs a) {
+    turn_queries<T, D, false, INTERLEAVED>(a, blockIdx.y);
+    asm volatile("griddepcontrol.wait;" ::: "memory");       // what follows in the stream needs both kernels' ends
 }
 
 // ---- conversion ----------------------------------------------------------------------
@@ -383,20 +442,25 @@ extern "C" int kvsnap_c8_append(const kvsnap_c8_cache* cache, const kvsnap_c8_ba
                            rotary ? rotary_dim : 0, query ? q_heads : 0, status};
         const bool single = batch->max_query <= 1;
         const int64_t units = single ? batch->seqs : batch->rows / cache->block_size + 2LL * batch->seqs;
-        const dim3 grid(unsigned(units), unsigned((2 * cache->kv_heads + 7) / 8 + (a.q_heads + 7) / 8));
+        const unsigned kv_ctas = unsigned(2 * cache->kv_heads + 7) / 8, q_ctas = unsigned(a.q_heads + 7) / 8;
         by_type(type, cache->head_dim, [&](auto t, auto d) {
             using T = decltype(t);
             constexpr int D = decltype(d)::value;
             const auto s = reinterpret_cast<cudaStream_t>(stream);
+            const auto run = [&](auto kernel, unsigned high, bool beside) {
+                launch(kernel, dim3(unsigned(units), high), 256, 0, s, beside, a);
+            };
             if (single) {
-                if (interleaved) append_kernel<T, D, true, true><<<grid, 256, 0, s>>>(a);
-                else append_kernel<T, D, true, false><<<grid, 256, 0, s>>>(a);
-            } else {
-                if (interleaved) append_kernel<T, D, false, true><<<grid, 256, 0, s>>>(a);
-                else append_kernel<T, D, false, false><<<grid, 256, 0, s>>>(a);
+                run(interleaved ? append_one_kernel<T, D, true> : append_one_kernel<T, D, false>, kv_ctas + q_ctas, false);
+                return;
             }
+            // Queries in a launch of their own are worth it from two full waves of the GPU on (an 8k prompt
+            // 38 us of kernels, together 49); below that the launch costs more (5 sequences of up to 701 tokens,
+            // 350 CTAs, appended and read back in 18.2 us together, 19.8 apart).
+            const bool apart = q_ctas && units * (kv_ctas + q_ctas) > 600;
+            run(interleaved ? append_kernel<T, D, true> : append_kernel<T, D, false>, kv_ctas + (apart ? 0 : q_ctas), false);
+            if (apart) run(interleaved ? turn_kernel<T, D, true> : turn_kernel<T, D, false>, q_ctas, true);
         });
-        check(cudaGetLastError());
     });
 }
 

@@ -15,6 +15,9 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <mutex>
+#include <set>
+#include <utility>
 
 #include "kvsnap_cuda.h"
 #include "kvsnap_internal.h"
@@ -192,6 +195,32 @@ int on_device(int device, C&& checks, F&& body) {
     }
     if (before >= 0 && device != before) cudaSetDevice(before);
     return rc;
+}
+
+// Raise a kernel's shared memory limit on the current device, once per kernel and device.
+void allow_shared(const void* kernel, int bytes) {
+    static std::mutex mu;
+    static std::set<std::pair<const void*, int>> done;
+    int device = 0;
+    check(cudaGetDevice(&device));
+    std::lock_guard<std::mutex> hold(mu);
+    if (done.count({kernel, device})) return;
+    check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done.insert({kernel, device});
+}
+
+// `after`: the kernel may start while the one before it in the stream ends (and waits for it itself).
+template <typename K, typename... A>
+void launch(K kernel, dim3 grid, int threads, size_t shared, cudaStream_t stream, bool after, const A&... args) {
+    if (shared > 48 << 10) allow_shared(reinterpret_cast<const void*>(kernel), int(shared));
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid, config.blockDim = dim3(unsigned(threads));
+    config.dynamicSmemBytes = shared, config.stream = stream;
+    cudaLaunchAttribute attribute{};
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &attribute, config.numAttrs = after ? 1 : 0;
+    check(cudaLaunchKernelEx(&config, kernel, args...));
 }
 
 bool aligned(int64_t v) { return v % 16 == 0; }

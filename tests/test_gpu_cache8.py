@@ -367,6 +367,29 @@ def test_append_rotated(interleaved, dim, rotary_dim, sequences):
                  interleaved=interleaved)
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dim,block_size,rotary_dim", [(128, 48, 128), (64, 80, 64), (128, 32, 48)])
+def test_append_rotated_to_pages_of_more_rows_than_a_warp_holds(interleaved, dim, block_size, rotary_dim):
+    p = Paged([(100, 7), (3, 46), (50, 0), (1, 90)], dim=dim, block_size=block_size, heads=3)
+    check_append(p, torch.float16, group=2, rotary_dim=rotary_dim, interleaved=interleaved)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_append_of_a_long_chunk_turns_its_queries_in_a_launch_of_their_own(interleaved):
+    p = Paged([(1900, 5), (0, 40), (700, 33), (1, 0)], heads=8, pad_rows=5)
+    check_append(p, torch.bfloat16, group=4, rotary_dim=128, interleaved=interleaved)
+    check_append(Paged([(2500, 9)], dim=64, heads=4), torch.float16, group=9, rotary_dim=32, interleaved=interleaved)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_append_rotated_values_not_finite(interleaved):
+    p = Paged([(6, 20), (1, 3), (2, 1)], heads=2, dim=64)
+    values = torch.randn(p.rows, 2, 64, generator=torch.Generator().manual_seed(3))
+    values[1, 0, 5], values[2, 1, 40], values[3, 0, 0], values[6, 1, 63] = math.inf, -math.inf, math.nan, math.inf
+    values = values.to(torch.bfloat16)
+    check_append(p, torch.bfloat16, data=(values, values), rotary_dim=64, interleaved=interleaved)
+
+
 def test_append_far_positions():
     """Angles of far positions come from 64 bits."""
     p = Paged([(1, 131071), (3, 99990)], heads=1, dim=64)
