@@ -658,27 +658,34 @@ __global__ void __launch_bounds__(32 * kWarps, 1) step_kernel(const __grid_const
     }
 }
 
-// Joins the parts of the shared unit that CTA blockIdx.x of the kernel before began, which lie in
-// consecutive CTAs' slots. Where units have few parts (WIDE false) a warp takes a row, else a CTA does,
-// its warps a share of the parts each. Bound by the way to a part and back, 4 parts at once: 6 to 8 us
-// with nothing in the caches, of which the launch is hidden behind the kernel before.
+// Joins the parts of the shared unit that a CTA of the kernels before began, which lie in consecutive CTAs'
+// slots: the first CTAs those of the kernel for few rows, `first_high` of each, the others the chunks'. Where
+// units have few parts (WIDE false) a warp takes a row, else a CTA does, its warps a share of the parts
+// each. Bound by the way to a part and back, 4 parts at once: 6 to 8 us with nothing in the caches, of which
+// the launch is hidden behind the kernel before.
 constexpr int kJoinWarps = 8;
 
 template <typename T, int D, bool WIDE>
 __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_constant__ AttendArgs a,
-                                                               const __grid_constant__ Parts p) {
+                                                               const __grid_constant__ Parts first, unsigned first_ctas,
+                                                               unsigned first_high, const __grid_constant__ Parts second,
+                                                               unsigned second_high) {
     constexpr int kEach = D / 32;
     using Piece = std::conditional_t<kEach == 4, float4, float2>;
     __shared__ float sums[kJoinWarps][D];
     __shared__ float stat[kJoinWarps];
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    const int task = WIDE ? blockIdx.y : blockIdx.y * kJoinWarps + warp;       // a row of one of the heads
+    const bool of_first = blockIdx.x < first_ctas * first_high;
+    const Parts& p = of_first ? first : second;
+    const unsigned high = of_first ? first_high : second_high, place = blockIdx.x - (of_first ? 0 : first_ctas * first_high);
+    const int cta = place / high, in_high = place % high;
+    const int task = WIDE ? in_high : in_high * kJoinWarps + warp;             // a row of one of the heads
     const int h = task / p.used_rows, row = task % p.used_rows;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const SharedUnit u = p.units[blockIdx.x];
+    const SharedUnit u = p.units[cta];
     if (u.parts == 0 || h >= p.heads || row >= u.rows) return;
     const int slot_rows = p.heads * p.head_rows, in = h * p.head_rows + row;
-    const auto at = [&](int f) { return int64_t(2 * (int(blockIdx.x) + f) + (f == 0)) * slot_rows + in; };
+    const auto at = [&](int f) { return int64_t(2 * (cta + f) + (f == 0)) * slot_rows + in; };
     const auto part = [&](int f) { return *reinterpret_cast<const Piece*>(p.sums + at(f) * D + lane * kEach); };
     float o[kEach] = {}, top = kLowest, sum = 0.0f;
     const auto add = [&](const Piece& v, float by) {
@@ -688,8 +695,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
     };
     // The maximum of all parts; then a warp's parts (of WIDE every eighth), 4 on their way at a time.
     for (int i = lane; i < u.parts; i += 32) top = fmaxf(top, p.ml[at(i)].x);
-    const int first = WIDE ? warp : 0, step = WIDE ? kJoinWarps : 1;
-    for (int i = first; i < u.parts; i += 4 * step) {
+    const int begin = WIDE ? warp : 0, step = WIDE ? kJoinWarps : 1;
+    for (int i = begin; i < u.parts; i += 4 * step) {
         Piece v[4];
         float2 ml[4];
 #pragma unroll
@@ -697,7 +704,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
             const int f = min(i + j * step, u.parts - 1);
             v[j] = part(f), ml[j] = p.ml[at(f)];
         }
-        if (i == first) top = warp_max(top);
+        if (i == begin) top = warp_max(top);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const float by = i + j * step < u.parts ? exp2_fast(ml[j].x - top) : 0.0f;
@@ -1589,7 +1596,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
     for (int w = 0; w < kAll; ++w) total += sh.c.scratch[w];
     total *= a.c.kv_heads;
     const Cut cut(uint32_t(total), gridDim.x);
-    if (blockIdx.x >= cut.ctas) return;
+    if (blockIdx.x >= cut.ctas) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        return;
+    }
     const int64_t pos = cut.begin(blockIdx.x), end = cut.begin(blockIdx.x + 1);
     int64_t before = 0;
     for (int base = 0; base < seqs; base += kScanned) {
@@ -1704,6 +1714,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
     if (warp == kIssueWarp)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(sh.c.tensor));
     if (threadIdx.x == 0 && sh.c.stop) atomicOr(a.status, KVSNAP_C8_STALLED);
+    // These CTAs start as those of the kernel for few rows end, and share nothing with them; what follows needs
+    // both kernels' ends.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // ---- host side ----------------------------------------------------------------------------
@@ -1716,7 +1729,7 @@ struct Plan {
     int step_rows;
     int most_rows;            // that a KV head of a sequence can have
     int64_t ctas, step_ctas, step_units;
-    int64_t slots, sum_bytes, bytes;
+    int64_t step_slots, chunk_slots, slots, sum_bytes, bytes;
 };
 
 int sm_count() {
@@ -1761,13 +1774,13 @@ Plan plan_for(const Cache& c, const Batch& b, int q_heads, int sms) {
     const int64_t costs = 4 + (plan.step_units < 96 ? plan.step_units : 96) / 6;
     plan.split = most * (2 * sms * waves - plan.step_units) > costs * 2 * sms;
     plan.step_ctas = plan.split ? plan.ctas : plan.step_units;
-    const int64_t step_slot = plan.stepped && plan.split ? p.hc * kStepRows : 0;
-    const int64_t chunk_slot = plan.chunked ? kUnitRows : 0;
-    // The two kernels and their joins run one after the other: they use the same bytes.
-    plan.slots = 2 * plan.ctas * (step_slot > chunk_slot ? step_slot : chunk_slot);
+    // The two kernels may run at the same time: each has its own part of the workspace.
+    plan.step_slots = plan.stepped && plan.split ? 2 * plan.ctas * p.hc * kStepRows : 0;
+    plan.chunk_slots = plan.chunked ? 2 * plan.ctas * kUnitRows : 0;
+    plan.slots = plan.step_slots + plan.chunk_slots;
     plan.sum_bytes = plan.slots * c.head_dim * int64_t(sizeof(float));
     plan.bytes = plan.slots ? plan.sum_bytes + plan.slots * int64_t(sizeof(float2)) +
-                                  plan.ctas * int64_t(sizeof(SharedUnit))
+                                  2 * plan.ctas * int64_t(sizeof(SharedUnit))
                             : 0;
     return plan;
 }
@@ -1780,28 +1793,36 @@ void launch_step(const Plan& plan, const StepArgs& p, cudaStream_t stream) {
 }
 
 template <typename T, int D>
-void launch_attend(const Plan& plan, const AttendArgs& a, Parts parts, cudaStream_t stream) {
-    // Few units have many parts each, and a CTA joins a row (8 units' 8191 tokens 15.1 us, a warp a row 17.0);
-    // many have few, and a warp does (chunks of 128 tokens in 24 sequences 282 us, a CTA a row 360).
-    const auto join = [&](int64_t units) {
-        const unsigned rows = unsigned(parts.heads * parts.used_rows), ctas = unsigned(plan.ctas);
-        if (units * 8 <= plan.ctas) launch(join_kernel<T, D, true>, dim3(ctas, rows), 32 * kJoinWarps, 0, stream, true, a, parts);
-        else launch(join_kernel<T, D, false>, dim3(ctas, (rows + kJoinWarps - 1) / kJoinWarps), 32 * kJoinWarps, 0, stream, true, a, parts);
-    };
+void launch_attend(const Plan& plan, const AttendArgs& a, char* workspace, cudaStream_t stream) {
+    const unsigned ctas = unsigned(plan.ctas);
+    const Parts of_steps{reinterpret_cast<float*>(workspace), reinterpret_cast<float2*>(workspace + plan.sum_bytes),
+                   reinterpret_cast<SharedUnit*>(workspace + plan.sum_bytes + plan.slots * int64_t(sizeof(float2))),
+                   plan.step.hc, kStepRows, plan.wide ? kStepRows : plan.most_rows};
+    const Parts of_chunks{of_steps.sums + plan.step_slots * D, of_steps.ml + plan.step_slots, of_steps.units + ctas,
+                          1, kUnitRows, plan.most_rows < kUnitRows ? plan.most_rows : kUnitRows};
     if (plan.stepped) {
         StepArgs p = plan.step;
-        parts.heads = p.hc, parts.head_rows = kStepRows, parts.used_rows = plan.wide ? kStepRows : plan.most_rows;
-        p.a = a, p.parts = parts;
+        p.a = a, p.parts = of_steps;
         if (plan.wide) launch_step<T, D, 2>(plan, p, stream);
         else launch_step<T, D, 1>(plan, p, stream);
-        if (plan.split) join(plan.step_units);
     }
-    if (plan.chunked) {
-        parts.heads = 1, parts.head_rows = kUnitRows, parts.used_rows = plan.most_rows < kUnitRows ? plan.most_rows : kUnitRows;
-        launch(chunk_kernel<T, D>, dim3(unsigned(plan.ctas)), kChunkThreads, sizeof(ChunkShared<D>) + 1024, stream, false,
-               ChunkArgs{a, parts});
-        join(plan.ctas);
-    }
+    // Without a wait between the two, and one join for both, batches of steps and chunks gain 4 to 10 % (16
+    // sequences of up to 4000 tokens and 9 new ones 65.8 us, one kernel after the other 72.5).
+    if (plan.chunked)
+        launch(chunk_kernel<T, D>, dim3(ctas), kChunkThreads, sizeof(ChunkShared<D>) + 1024, stream, plan.stepped,
+               ChunkArgs{a, of_chunks});
+    if (!plan.slots) return;
+    // Few units have many parts each, and a CTA joins a row (8 units' 8191 tokens 15.1 us, a warp a row 17.0);
+    // many have few, as chunks do, and a warp does (chunks of 128 tokens in 24 sequences 282 us, a CTA a row 360).
+    const bool wide = !plan.chunked && plan.step_units * 8 <= plan.ctas;
+    const auto high = [&](const Parts& p) {
+        const unsigned rows = unsigned(p.heads * p.used_rows);
+        return wide ? rows : (rows + kJoinWarps - 1) / kJoinWarps;
+    };
+    const unsigned joined = plan.step_slots ? ctas : 0, step_high = high(of_steps), chunk_high = high(of_chunks);
+    const dim3 grid(joined * step_high + (plan.chunked ? ctas * chunk_high : 0));
+    launch(wide ? join_kernel<T, D, true> : join_kernel<T, D, false>, grid, 32 * kJoinWarps, 0, stream, true, a, of_steps,
+           joined, step_high, of_chunks, chunk_high);
 }
 
 void check_attend(const Cache* cache, const Batch* batch, int q_heads) {
@@ -1854,12 +1875,9 @@ extern "C" int kvsnap_c8_attend(const kvsnap_c8_cache* cache, const kvsnap_c8_ba
         const AttendArgs a{*cache, *batch, {static_cast<const char*>(query), query_token, query_head},
                            static_cast<char*>(out), q_heads, q_heads / cache->kv_heads, plan.step_rows,
                            scale * 1.4426950408889634f, status};
-        char* at = static_cast<char*>(workspace);
-        const Parts parts{reinterpret_cast<float*>(at), reinterpret_cast<float2*>(at + plan.sum_bytes),
-                          reinterpret_cast<SharedUnit*>(at + plan.sum_bytes + plan.slots * int64_t(sizeof(float2))),
-                          0, 0, 0};
         by_type(type, cache->head_dim, [&](auto t, auto d) {
-            launch_attend<decltype(t), decltype(d)::value>(plan, a, parts, reinterpret_cast<cudaStream_t>(stream));
+            launch_attend<decltype(t), decltype(d)::value>(plan, a, static_cast<char*>(workspace),
+                                                           reinterpret_cast<cudaStream_t>(stream));
         });
     });
 }
