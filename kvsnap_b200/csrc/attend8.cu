@@ -99,7 +99,7 @@ struct Parts {
 // Bound by the cache's bytes, so nothing but a page's codes is read, once: a step of 64 sessions of 512 to
 // 8192 tokens with 8 heads of 128, 372 MB, takes 79 us, 4.7 TB/s, of which the loop over granules runs at 86 %
 // of the rate of a plain copy, and the rest is the scan for a CTA's chunks (2 us), the first copies'
-// way and the merge of a CTA's slices (2 us a unit). With few sequences those are what bounds it: 27 us for
+// way and the merge of a CTA's slices (2 us a unit). With few sequences those are what bounds it: 22 us for
 // one of 32k tokens, whose 67 MB are 10 us. A warp copies a granule of 16 tokens to its own shared memory
 // asynchronously, kAhead granules ahead, no warp waiting for another; 8 lanes copy
 // one token's line, as 16-byte requests are joined among 8 lanes (with lanes that
@@ -114,6 +114,11 @@ struct Parts {
 
 constexpr int kStepRows = 16;
 constexpr int kWarps = 16;                 // a CTA: HC heads x TS slices of a chunk
+// What a unit costs besides its chunks (its first pages and copies, which wait for the unit before, and its
+// merge), in chunks: work is cut by chunks and this. Without it, with 3, 5, 9 (us): a 32k step of 64 and 8
+// heads 31.0, 27.7, 25.8, 25.4; 16 sequences of up to 32k tokens of one head 29.4, 25.6, 23.8, 23.7; 64
+// sessions of 1k to 8k 94.5, 90.0, 89.3, 91.0; 16 of mixed rows 65.3, 59.5, 60.7, 64.8.
+constexpr int kStepUnitCost = 5;
 constexpr int kSpread = 48;                // units of few sequences that heads are spread for
 constexpr int kAhead = 3;                  // granules a warp holds: one in use, the others on their way
 constexpr float kLowest = -3e38f;          // the running maximum before any token
@@ -193,6 +198,12 @@ struct __align__(16) StepPage {
 __device__ __forceinline__ int chunks_of(const StepArgs& p, int s, Sequence& q) {
     if (!read_sequence(p.a.b, p.a.c.block_size, s, q, p.a.status) || q.rows * p.a.group > p.a.step_rows) return 0;
     return max(1, (q.length + p.ts * kGranule - 1) / (p.ts * kGranule));
+}
+
+// What a head group of a sequence costs: its chunks, and what it costs besides; without chunks nothing.
+__device__ __forceinline__ int cost_of(const StepArgs& p, int s, Sequence& q) {
+    const int chunks = chunks_of(p, s, q);
+    return chunks ? chunks + kStepUnitCost : 0;
 }
 
 // One warp's share of chunks [c0, c1) of one head of one sequence.
@@ -510,15 +521,16 @@ __global__ void __launch_bounds__(32 * kWarps, 1) step_kernel(const __grid_const
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, seqs = p.a.b.seqs;
     asm volatile("griddepcontrol.launch_dependents;");
 
-    uint32_t pos = 0, end = 1, cut_total = 0;
-    int s = 0, hg = 0, c0 = 0;
+    uint32_t pos = 0, end = 1, cut_total = 0;     // this CTA's part [pos, end) of what all units cost
+    uint32_t from = 0;                            // where the unit's chunks begin in that
+    int s = 0, hg = 0;
     Sequence q;
     if (SPLIT) {
         if (threadIdx.x == 0) p.parts.units[blockIdx.x].parts = 0;
-        // All chunks; those of up to 512 sequences are summed and found in one pass, one's need no sum.
+        // What all units cost; that of up to 512 sequences are summed and found in one pass, one's need no sum.
         uint32_t mine = 0;
-        if (seqs == 1) mine = chunks_of(p, 0, q) * p.hg;
-        else for (int i = threadIdx.x; i < seqs; i += blockDim.x) mine += chunks_of(p, i, q) * p.hg;
+        if (seqs == 1) mine = cost_of(p, 0, q) * p.hg;
+        else for (int i = threadIdx.x; i < seqs; i += blockDim.x) mine += cost_of(p, i, q) * p.hg;
         uint32_t sum = mine, low = 0;
         if (seqs == 1) {
             cut_total = mine;
@@ -549,7 +561,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1) step_kernel(const __grid_const
             uint32_t before = 0;
             for (int tile = 0; tile < seqs && before <= pos; tile += blockDim.x) {
                 const int i = tile + threadIdx.x;
-                const uint32_t n = i < seqs ? chunks_of(p, i, q) * p.hg : 0;
+                const uint32_t n = i < seqs ? cost_of(p, i, q) * p.hg : 0;
                 sum = n;
 #pragma unroll
                 for (int k = 1; k < 32; k <<= 1) {
@@ -569,8 +581,9 @@ __global__ void __launch_bounds__(32 * kWarps, 1) step_kernel(const __grid_const
             }
         }
         s = sh.found;
-        const uint32_t n = chunks_of(p, s, q), within = pos - sh.found_first;
-        hg = within / n, c0 = within % n;
+        const uint32_t n = cost_of(p, s, q);
+        hg = (pos - sh.found_first) / n;
+        from = sh.found_first + hg * n + kStepUnitCost;
     } else {
         s = blockIdx.x / p.hg, hg = blockIdx.x % p.hg;
     }
@@ -582,7 +595,8 @@ __global__ void __launch_bounds__(32 * kWarps, 1) step_kernel(const __grid_const
             ++s;
             continue;
         }
-        const int c1 = SPLIT ? min(chunks, c0 + int(end - pos)) : chunks;
+        const int c0 = SPLIT ? max(int(pos - from), 0) : 0, c1 = SPLIT ? min(chunks, int(end - from)) : chunks;
+        if (c1 <= c0) return;                         // its chunks begin with the next CTA
         const int rows = q.rows * p.a.group;
         const int hc = warp % p.hc, slice = warp / p.hc;       // a warp without a slice only waits
         StepWarp<T, D, NT> w;
@@ -647,13 +661,12 @@ __global__ void __launch_bounds__(32 * kWarps, 1) step_kernel(const __grid_const
         }
         if (SPLIT) {
             if (!whole && c0 == 0 && threadIdx.x == 0) {
-                const int last = Cut(cut_total, gridDim.x).of(pos + chunks - 1);       // who ends the unit
+                const int last = Cut(cut_total, gridDim.x).of(from + chunks - 1);      // who ends the unit
                 p.parts.units[blockIdx.x] = SharedUnit{q.row, hg * p.hc, 0, rows, last - int(blockIdx.x) + 1};
             }
             __syncthreads();
         }
-        pos += c1 - c0;
-        c0 = 0;
+        pos = from + c1, from = pos + kStepUnitCost;
         if (++hg == p.hg) hg = 0, ++s;
     }
 }
@@ -1834,7 +1847,7 @@ void check_attend(const Cache* cache, const Batch* batch, int q_heads) {
     // All the work of a call is counted in 32 bits: granules of each head, steps of each 256 rows and head.
     const double granules = double(batch->width) * cache->block_size / kGranule + 1;
     const double units = double(batch->rows) * (q_heads / cache->kv_heads) / kUnitRows + batch->seqs;
-    require(batch->seqs * granules * cache->kv_heads < 2147483648.0 &&
+    require(batch->seqs * (granules + kStepUnitCost) * cache->kv_heads < 2147483648.0 &&
                 units * cache->kv_heads * (granules * kGranule / kStep + kUnitCost + 1) < 2147483648.0,
             "too much work for one attention");
 }
