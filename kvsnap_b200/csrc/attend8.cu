@@ -97,9 +97,9 @@ struct Parts {
 // new tokens): what m16n8k16 products take without idle rows, while the kernel below works on 256 rows
 // whatever there are (16 sequences of 8000 tokens with 8 rows a head: 61 us, there 153; with 16 rows 113).
 // Bound by the cache's bytes, so nothing but a page's codes is read, once: a step of 64 sessions of 512 to
-// 8192 tokens with 8 heads of 128, 372 MB, takes 79 us, 4.7 TB/s, of which the loop over granules runs at 86 %
+// 8192 tokens with 8 heads of 128, 372 MB, takes 70 us, 5.3 TB/s, of which the loop over granules runs at 86 %
 // of the rate of a plain copy, and the rest is the scan for a CTA's chunks (2 us), the first copies'
-// way and the merge of a CTA's slices (2 us a unit). With few sequences those are what bounds it: 22 us for
+// way and the merge of a CTA's slices (2 us a unit). With few sequences those are what bounds it: 21 us for
 // one of 32k tokens, whose 67 MB are 10 us. A warp copies a granule of 16 tokens to its own shared memory
 // asynchronously, kAhead granules ahead, no warp waiting for another; 8 lanes copy
 // one token's line, as 16-byte requests are joined among 8 lanes (with lanes that
@@ -1781,8 +1781,8 @@ Plan plan_for(const Cache& c, const Batch& b, int q_heads, int sms) {
     // Cutting the chunks evenly over the CTAs costs a scan of the lengths, merges of parts and a join: as
     // much as 4 chunks in turn, more with more units, up to 20. It saves at most the longest unit's chunks
     // less an even share, taken at half of what the table could hold. Cut and uncut, in us: 1 sequence of
-    // 1300 tokens 13.7 and 15.0, of 4000 14.3 and 23.3; 64 of 300 24.5 and 19.1, of 1000 41.4 and 41.7; of
-    // mixed lengths up to 1000 29.5 and 39.7; 128 of 700 47.8 and 40.7.
+    // 4000 tokens 15.2 and 23.4; 64 of 300 21.3 and 19.1, of 1000 38.7 and 41.7, of mixed lengths up to 1000
+    // 27.3 and 39.6; 128 of 700 48.7 and 40.1; 200 of 700 65.6 and 69.6.
     const int64_t waves = (plan.step_units + sms - 1) / sms;
     const int64_t costs = 4 + (plan.step_units < 96 ? plan.step_units : 96) / 6;
     plan.split = most * (2 * sms * waves - plan.step_units) > costs * 2 * sms;
