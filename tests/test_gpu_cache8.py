@@ -507,7 +507,7 @@ def step(p, dtype=torch.bfloat16, group=2):
     return run
 
 
-@pytest.mark.parametrize("sequences", [[(1, 700), (1, 20)], [(50, 700), (3, 20)]], ids=str)
+@pytest.mark.parametrize("sequences", [[(1, 700), (1, 20)], [(50, 700), (3, 20)], [(4800, 40), (20, 5)]], ids=str)
 def test_a_captured_step_replays_on_new_contents(sequences):
     p = Paged(sequences)
     run = step(p)
