@@ -4,7 +4,9 @@
 // over the tokens j that row i sees, in one pass with the running maximum m. Codes
 // meet queries and weights as fp16 (e4m3 is exact in it) in matrix instructions
 // with 32-bit sums; a page's key scale multiplies its scores, its value scale its
-// weights, both in 32 bits.
+// weights, both in 32 bits. Weights meet values as fp16, so they are held relative to a
+// second running maximum, of weight times value scale: a page of large values and next to
+// no weight then takes no bits from the pages that make up the result.
 #include <type_traits>
 
 #include "cache8.cuh"
@@ -121,7 +123,7 @@ constexpr int kWarps = 16;                 // a CTA: HC heads x TS slices of a c
 constexpr int kStepUnitCost = 5;
 constexpr int kSpread = 48;                // units of few sequences that heads are spread for
 constexpr int kAhead = 3;                  // granules a warp holds: one in use, the others on their way
-constexpr float kLowest = -3e38f;          // the running maximum before any token
+constexpr float kLowest = -1e38f;          // the running maxima before any token
 constexpr float kSlack = 14.0f;            // log2 by which a weight may exceed 1 before sums are rescaled (fp16: 2^16)
 
 struct StepArgs {
@@ -188,6 +190,18 @@ __device__ __forceinline__ uint4 read_shared(uint32_t at) {
     return v;
 }
 
+// A scale as 2^power * part, part in [1, 2): the weights of its values take the power into their exponent.
+// Of a scale of 0 the part is 0 and the power -infinity, which raises no maximum.
+struct ValueScale {
+    float power, part;
+
+    __device__ __forceinline__ explicit ValueScale(float s) {
+        const int bits = min(max(int(__float_as_uint(s) >> 23), 1), 253);
+        part = s * __uint_as_float(uint32_t(254 - bits) << 23);
+        power = part > 0.0f ? float(bits - 127) : -INFINITY;
+    }
+};
+
 // Where a warp's granule of a chunk lies, and its scales. A page that is not there: off < 0.
 struct __align__(16) StepPage {
     int64_t off;
@@ -211,9 +225,10 @@ template <typename T, int D, int NT>
 struct StepWarp {
     static constexpr int kHalves = D / 64, kTiles = D / 16;
     static constexpr uint32_t kSideBytes = kGranule * D, kGranuleBytes = 2 * kSideBytes;
-    float o[NT][kTiles][4];                // (dim pair, row) sums, relative to m and vref
-    float m[NT][2], l[NT][2];              // of rows 8 nt + 2 t, + 1
-    float vref;                            // largest value scale so far
+    // Of rows 8 nt + 2 t, + 1: l = sum of 2^(s - m), and o 2^e = sum of 2^(s - m) v, a weight in it being
+    // 2^(s - m + power - e). m and e are whole numbers, rounded up, so that exponents add without error.
+    float o[NT][kTiles][4];                // (dim pair, row)
+    float m[NT][2], e[NT][2], l[NT][2];
 
     // `ring`: the warp's kAhead granules of shared memory; `pages`: what it knows of 64 chunks' pages.
     __device__ __forceinline__ void run(const StepArgs& p, const Sequence& q, int s, int head, int slice, int c0,
@@ -221,10 +236,9 @@ struct StepWarp {
         const int lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
         const Cache& c = p.a.c;
         const int rows = q.rows * p.a.group, first_seen = q.length - q.rows + 1;
-        vref = 0.0f;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            m[nt][0] = m[nt][1] = kLowest, l[nt][0] = l[nt][1] = 0.0f;
+            m[nt][0] = m[nt][1] = e[nt][0] = e[nt][1] = kLowest, l[nt][0] = l[nt][1] = 0.0f;
 #pragma unroll
             for (int mt = 0; mt < kTiles; ++mt)
 #pragma unroll
@@ -342,9 +356,6 @@ struct StepWarp {
         }
 
         uint32_t at = ring;
-        float limit[NT][2], v_by = 0.0f;             // m + kSlack; 1 / vref
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) limit[nt][0] = limit[nt][1] = kLowest;
 #pragma unroll 1
         for (int chunk = c0; chunk < c1; ++chunk) {
             copy();
@@ -388,7 +399,8 @@ struct StepWarp {
 
             // Edge: tokens that some row does not see, or a page that is not there.
             const bool dead = page.off < 0, edge = dead || base + kGranule > first_seen;
-            bool grow = page.vs > vref;
+            const ValueScale vs(page.vs);
+            bool grow = false;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -408,12 +420,9 @@ struct StepWarp {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) grow |= fmaxf(sc[nt][i], sc[nt][2 + i]) > limit[nt][i];
+                for (int i = 0; i < 2; ++i)
+                    grow |= fmaxf(sc[nt][i], sc[nt][2 + i]) + fmaxf(vs.power - e[nt][i], 0.0f) > m[nt][i] + kSlack;
             if (__any_sync(~0u, grow)) {
-                // Weights carry the page's value scale relative to the largest so far, so fp16 holds them.
-                const float v_keep = page.vs > vref ? vref / page.vs : 1.0f;
-                vref = fmaxf(vref, page.vs);
-                v_by = vref > 0.0f ? 1.0f / vref : 0.0f;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -422,25 +431,27 @@ struct StepWarp {
                         top = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
                         top = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
                         top = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
-                        top = fmaxf(top, m[nt][i]);
-                        const float keep = exp2_fast(m[nt][i] - top);
-                        m[nt][i] = top, l[nt][i] *= keep;
-                        limit[nt][i] = top + kSlack;
+                        const float up = fmaxf(m[nt][i], ceilf(top));
+                        const float same = e[nt][i] + (m[nt][i] - up);        // leaves m + e, and so o, as it is
+                        l[nt][i] *= exp2_fast(m[nt][i] - up);
+                        m[nt][i] = up, e[nt][i] = fmaxf(same, ceilf(top - up) + vs.power);
+                        const float keep = exp2_fast(same - e[nt][i]);
 #pragma unroll
-                        for (int mt = 0; mt < kTiles; ++mt)
-                            o[nt][mt][i] *= keep * v_keep, o[nt][mt][2 + i] *= keep * v_keep;
+                        for (int mt = 0; mt < kTiles; ++mt) o[nt][mt][i] *= keep, o[nt][mt][2 + i] *= keep;
                     }
             }
-            const float part = page.vs * v_by;
             uint32_t pb[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 float w[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = exp2_fast(sc[nt][i] - m[nt][i % 2]);
-                l[nt][0] += w[0] + w[2], l[nt][1] += w[1] + w[3];
-                pb[nt][0] = transpose8x8(pack_half2(w[0] * part, w[1] * part));
-                pb[nt][1] = transpose8x8(pack_half2(w[2] * part, w[3] * part));
+                for (int i = 0; i < 2; ++i) {
+                    const float a = sc[nt][i] - m[nt][i], b = sc[nt][2 + i] - m[nt][i], by = vs.power - e[nt][i];
+                    l[nt][i] += exp2_fast(a) + exp2_fast(b);
+                    w[i] = exp2_fast(a + by) * vs.part, w[2 + i] = exp2_fast(b + by) * vs.part;
+                }
+                pb[nt][0] = transpose8x8(pack_half2(w[0], w[1]));
+                pb[nt][1] = transpose8x8(pack_half2(w[2], w[3]));
             }
 
             const auto add_values = [&](const uint4 (&v)[4], const uint32_t (&b)[NT][2]) {
@@ -613,11 +624,12 @@ __global__ void __launch_bounds__(32 * kWarps, 1) step_kernel(const __grid_const
                 for (int i = 0; i < 2; ++i) {
                     const int n = nt * 8 + 2 * t + i;
                     if (g == 0) sh.ml[warp][n] = make_float2(w.m[nt][i], w.l[nt][i]);
+                    const float by = exp2_fast(w.e[nt][i]);
 #pragma unroll
                     for (int mt = 0; mt < D / 16; mt += 2)
                         *reinterpret_cast<float4*>(&sh.o[warp][n][(D / 8) * g + 2 * mt]) =
-                            make_float4(w.o[nt][mt][i] * w.vref, w.o[nt][mt][2 + i] * w.vref,
-                                        w.o[nt][mt + 1][i] * w.vref, w.o[nt][mt + 1][2 + i] * w.vref);
+                            make_float4(w.o[nt][mt][i] * by, w.o[nt][mt][2 + i] * by, w.o[nt][mt + 1][i] * by,
+                                        w.o[nt][mt + 1][2 + i] * by);
                 }
             }
         }
@@ -766,9 +778,11 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
 // prompt of 32 heads.
 // The running maximum follows a row's true maximum only when that exceeds it by 2^14 (weights stay
 // within fp16), so sums in tensor memory are rarely touched (followed at every step: an 8k prompt 738 us,
-// so 662). A page's scale goes into the conversion
-// relative to the largest key scale of the tile (which multiplies S) and the largest value scale so
-// far (which divides O at the end): powers of two, exact in fp16.
+// so 662). A page's scale goes into the conversion relative to the largest of its step, where e4m3's
+// 9 fraction bits below 1 leave fp16 room: keys down to 2^-14, values down to 2^-6. The step's key scale
+// multiplies S, its value scale the weights, relative to a running maximum of their products (a row's e:
+// O 2^e are the sums). Steps whose pages lie further apart take their pages' own scales into
+// the scores instead, and sum their weights apart.
 
 constexpr int kTile = 128;                 // rows a tile
 constexpr int kUnitRows = 2 * kTile;
@@ -783,6 +797,9 @@ constexpr int kConvertWarps = 4, kIssueWarp = 12, kLookWarp = 13, kChunkThreads 
 constexpr int kLooked = 16;                // steps looked up ahead
 constexpr int kScales = 8;                 // steps whose scales the softmax may still need
 constexpr int kLookedUnits = 4;            // units
+constexpr float kKeysApart = 1.0f / 16384;  // a step's smallest key scale to its largest, and powers of value
+constexpr float kValuesApart = 6.0f;       // scales, up to which the conversion takes them
+constexpr float kFarBelow = 60.0f;         // powers of two below a row's e from which weights are summed apart
 constexpr uint32_t kSumsAt = 256;          // columns of tensor memory: S and P 0 to 255, O from here
 
 struct ChunkArgs {
@@ -827,12 +844,15 @@ __device__ __forceinline__ int64_t head_cost(const AttendArgs& a, int s) {
 constexpr int kScanned = 256;              // sequences scanned at a time
 constexpr int kNanUnits = 64;              // more units than the roles can be apart
 
+constexpr uint32_t kAllLive = (1u << kGranules) - 1, kApart = 1u << kGranules;
+
 // What a step's conversion needs to know.
 struct Looked {
     int64_t keys[kGranules];               // addresses of the granules' key codes; 0: not there
-    uint32_t k_by[kGranules], v_by[kGranules];   // their scales relative to the two below, as fp16 pairs
-    float k_scale, v_scale;                // largest key scale of the step; largest value scale so far
-    uint32_t live;                         // granules that are there
+    uint32_t k_by[kGranules], v_by[kGranules];   // what their codes are multiplied by, as fp16 pairs
+    float k_scale, v_power;                // largest key scale of the step; power of its largest value scale
+    uint32_t live;                         // granules that are there; kApart: their own scales count
+    float k_own[kGranules], v_own[kGranules];    // with kApart: their key scales, and powers less v_power
     int tokens;                            // of the step that the sequence has
     int edge;                              // some row does not see all of them
     int last;                              // of the CTA
@@ -854,8 +874,9 @@ struct ChunkControl {
     Looked look[kLooked];
     uint64_t unit_looked[kLookedUnits], unit_free[kLookedUnits];
     LookedUnit unit[kLookedUnits];
-    float k_scale[kScales], v_scale[kScales];    // of a step: largest key scale; largest value scale so far
-    uint32_t live[kScales];                // of a step: its 16-token granules that are there
+    float k_scale[kScales], v_power[kScales];    // of a step, as in Looked
+    uint32_t live[kScales];
+    float k_own[kScales][kGranules], v_own[kScales][kGranules];
     int nan_unit[kNanUnits];               // a unit (counted from 1) whose last steps hold a NaN value
     uint32_t tensor;                       // tensor memory's address
     volatile int stop;                     // a wait ran out
@@ -1107,6 +1128,11 @@ __device__ __forceinline__ void tensor_store(uint32_t at, const uint32_t (&v)[16
           "r"(at) : "memory");
 }
 
+__device__ __forceinline__ void tensor_store(uint32_t at, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};"
+        :: "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(at) : "memory");
+}
+
 __device__ __forceinline__ void tensor_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Where 16 bytes (8 fp16) `chunk` of row r lie in a matrix of R rows of fp16.
@@ -1149,7 +1175,6 @@ __device__ __forceinline__ void look_role(const ChunkArgs& p, ChunkControl& c, W
             asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
             if (cache.head_dim > 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + 128));
         }
-        float v_top = 0.0f;
         for (int first = w.begin; first < w.end; first += kParts) {
             const int n = min(kParts, w.end - first), step = first + part;
             const int64_t token = int64_t(step) * kStep + granule * kGranule;
@@ -1166,13 +1191,19 @@ __device__ __forceinline__ void look_role(const ChunkArgs& p, ChunkControl& c, W
                     ks = scales[0], vs = scales[cache.kv_heads];
                 }
             }
-            const uint32_t live = __ballot_sync(~0u, at != 0) >> (kGranules * part) & ((1u << kGranules) - 1);
-            float k_top = ks;
+            const ValueScale v(vs);
+            float k_top = ks, v_top = v.power;
 #pragma unroll
-            for (int i = kGranules / 2; i; i >>= 1) k_top = fmaxf(k_top, __shfl_xor_sync(~0u, k_top, i));
-            v_top = fmaxf(v_top, warp_max(vs));        // of all these steps: it changes once in 8 at most
-            const __half2 k_by = __float2half2_rn(k_top > 0.0f ? ks / k_top : 0.0f);
-            const __half2 v_by = __float2half2_rn(v_top > 0.0f ? vs / v_top : 0.0f);
+            for (int i = kGranules / 2; i; i >>= 1) {
+                k_top = fmaxf(k_top, __shfl_xor_sync(~0u, k_top, i));
+                v_top = fmaxf(v_top, __shfl_xor_sync(~0u, v_top, i));
+            }
+            v_top = fmaxf(v_top, -126.0f);             // of no values but zeros: any finite one
+            const bool far = at && ((ks > 0.0f && ks < k_top * kKeysApart) || v.power < v_top - kValuesApart);
+            const uint32_t live = __ballot_sync(~0u, at != 0) >> (kGranules * part) & kAllLive;
+            const bool apart = __ballot_sync(~0u, far) >> (kGranules * part) & kAllLive;
+            const __half2 k_by = __float2half2_rn(apart ? 1.0f : k_top > 0.0f ? ks / k_top : 0.0f);
+            const __half2 v_by = __float2half2_rn(apart ? v.part : v.part * exp2_fast(v.power - v_top));
             for (int i = 0; i < n; ++i)
                 if (!warp_wait(&c.look_free[(it + i) % kLooked], uint32_t((it + i) / kLooked + 1) % 2, c)) return;
             if (part < n) {
@@ -1180,8 +1211,9 @@ __device__ __forceinline__ void look_role(const ChunkArgs& p, ChunkControl& c, W
                 to.keys[granule] = at;
                 to.k_by[granule] = reinterpret_cast<const uint32_t&>(k_by);
                 to.v_by[granule] = reinterpret_cast<const uint32_t&>(v_by);
+                to.k_own[granule] = ks, to.v_own[granule] = v.power - v_top;
                 if (granule == 0) {
-                    to.k_scale = k_top, to.v_scale = v_top, to.live = live;
+                    to.k_scale = k_top, to.v_power = v_top, to.live = live | (apart ? kApart : 0);
                     to.tokens = int(min(int64_t(kStep), max(int64_t(0), w.u.q.length - token)));
                     to.edge = int64_t(step + 1) * kStep > w.u.first_seen;
                     to.last = !more && step + 1 == w.end;
@@ -1246,8 +1278,11 @@ __device__ __forceinline__ void convert_role(const ChunkArgs& p, ChunkShared<D>&
         const Looked& look = sh.c.look[step % kLooked];
         const bool more = !look.last;
         if (tid == 0) {
-            sh.c.k_scale[step % kScales] = look.k_scale, sh.c.v_scale[step % kScales] = look.v_scale;
+            sh.c.k_scale[step % kScales] = look.k_scale, sh.c.v_power[step % kScales] = look.v_power;
             sh.c.live[step % kScales] = look.live;
+            if (look.live & kApart)
+                for (int i = 0; i < kGranules; ++i)
+                    sh.c.k_own[step % kScales][i] = look.k_own[i], sh.c.v_own[step % kScales][i] = look.v_own[i];
         }
         if (!warp_wait(&sh.c.k_empty[slot], free, sh.c)) return false;
         convert(kr, sh.k[slot], look.k_by);
@@ -1372,6 +1407,93 @@ __device__ __forceinline__ char* staged(char* warp_rows, int row, int chunk) {
     return warp_rows + row * 128 + (chunk ^ row % 8) * 16;
 }
 
+// What a softmax thread knows of its row: l = sum of 2^(s - m); sums in tensor memory, times 2^e, = sum of
+// 2^(s - m) v. Whole numbers m and e, as in StepWarp.
+struct RowState {
+    float m, e, l;
+};
+
+constexpr float kLeast = 1.17549435e-38f;  // the smallest normal number
+
+// Multiplies the sums so far in tensor memory, once the step before is in them.
+template <int D>
+__device__ __forceinline__ bool rescale(uint32_t sums, float keep, uint64_t* summed, uint32_t parity, ChunkControl& c) {
+    if (!warp_wait(summed, parity, c)) return false;
+    fence_after();
+#pragma unroll 1
+    for (int i = 0; i < D / 16; ++i) {
+        float y[16];
+        __syncwarp();                                    // lanes meet before each access to tensor memory
+        tensor_load(sums + 16 * i, y);
+        tensor_loaded(y);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) y[j] *= keep;
+        tensor_store(sums + 16 * i, y);
+    }
+    return true;
+}
+
+// A step whose weights in the sums do not tell those of l: a granule of 16 columns at a time, three times. `k_own`: pages by their own scales. Weights take columns that
+// have been read. Out of line, as the loop over steps is to stay in the instruction cache: an 8k prompt takes
+// 697 us, with this in the loop's way 731, without it at all 689.
+template <int D>
+__device__ __noinline__ bool step_alone(RowState& row, uint32_t at, uint64_t seen, const float* k_own, const float* v_own,
+                                        float factor, float f, float power, uint32_t sums, uint64_t* summed,
+                                        uint32_t parity, ChunkControl& c) {
+    float m = row.m, e = row.e, top = -INFINITY, sum = 0.0f, by = 0.0f;
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+#pragma unroll 1
+        for (int i = 0; i < kGranules; ++i) {
+            float y[kGranule];
+            __syncwarp();
+            tensor_load(at + kGranule * i, y);
+            const float k = k_own ? fmaxf(factor * k_own[i], kLeast) : f, v = k_own ? v_own[i] : 0.0f;
+            const uint32_t see = uint32_t(seen >> (kGranule * i));
+            tensor_loaded(y);
+#pragma unroll
+            for (int j = 0; j < kGranule; ++j) y[j] = see >> j & 1 ? y[j] * k : -INFINITY;
+            if (pass == 0) {
+#pragma unroll
+                for (int j = 0; j < kGranule; ++j) top = fmaxf(top, y[j]);
+            } else if (pass == 1) {
+#pragma unroll
+                for (int j = 0; j < kGranule; ++j) {
+                    y[j] -= m;
+                    sum += exp2_fast(y[j]), top = fmaxf(top, y[j] + v);
+                }
+            } else {
+                uint32_t weights[kGranule / 2];
+#pragma unroll
+                for (int j = 0; j < kGranule; ++j) y[j] = exp2_fast(y[j] - m + (v + by));
+#pragma unroll
+                for (int j = 0; j < kGranule / 2; ++j) weights[j] = pack_half2(y[2 * j], y[2 * j + 1]);
+                __syncwarp();
+                tensor_store(at + kGranule / 2 * i, weights);
+            }
+        }
+        if (pass == 0) {
+            if (top > m) {                               // leaves m + e, and so the sums, as they are
+                const float up = ceilf(top);
+                row.l *= exp2_fast(m - up);
+                e += m - up, m = up;
+            }
+            top = -INFINITY;
+        } else if (pass == 1) {
+            float keep = 1.0f;
+            if (top + power > e + kSlack) {
+                const float up = ceilf(top) + power;
+                keep = exp2_fast(e - up);
+                e = up;
+            }
+            if (summed && __any_sync(~0u, keep != 1.0f) && !rescale<D>(sums, keep, summed, parity, c)) return false;
+            by = power - e;
+        }
+    }
+    row.m = m, row.e = e, row.l += sum;
+    return true;
+}
+
 // The role of warps 0-3 (row tile 0) and 4-7 (row tile 1).
 template <typename T, int D>
 __device__ __forceinline__ void softmax_role(const ChunkArgs& p, ChunkShared<D>& sh) {
@@ -1440,7 +1562,16 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs& p, ChunkShared<D>&
             if (lane == 0) barrier_arrive(&sh.c.q_full[tile]);
         }
 
-        float m = kLowest, l = 0.0f, v_scale = 0.0f;
+        float m = kLowest, e = kLowest, l = 0.0f;        // as in RowState
+        // A step's weights are in tensor memory.
+        const auto weighed = [&] {
+            __syncwarp();
+            tensor_stored();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) barrier_arrive(&sh.c.p_full[tile][turn % 2]);
+            ++turn;
+        };
         for (int step = begin; step < end; ++step, ++it) {
             if (!warp_wait(&sh.c.s_full[tile][turn % 2], turn / 2 % 2, sh.c)) return;
             fence_after();
@@ -1448,16 +1579,25 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs& p, ChunkShared<D>&
             float x[kStep];
             tensor_load(at, x);
             // Never 0, so that a hidden score stays -infinity.
-            const float f = fmaxf(factor * sh.c.k_scale[it % kScales], 1.17549435e-38f);
-            const float now_v = sh.c.v_scale[it % kScales];
+            const float f = fmaxf(factor * sh.c.k_scale[it % kScales], kLeast);
+            const float power = sh.c.v_power[it % kScales];
             const uint32_t live = sh.c.live[it % kScales];
             const int see = min(max(seen - step * kStep, 0), kStep);       // columns up to here are seen
+            // A weight in the sums is 2^(s f + by), and `share` of it is its part of l. That holds for scores up to
+            // `limit`: above it a maximum moves. Where the weights in the sums are too far below l's, no score is below it.
+            const bool odd = power - e < -kFarBelow;
+            const float limit = odd ? 2 * kLowest : m + kSlack + fminf(e - power, 0.0f);
+            float by = power - e - m, share = exp2_fast(fminf(e - power, kFarBelow));
             tensor_loaded(x);
-            if (__any_sync(~0u, see < kStep) || live != (1u << kGranules) - 1) {
+            const auto seen_bits = [&] {
                 uint64_t bits = see == kStep ? ~0ull : (1ull << see) - 1;
 #pragma unroll
                 for (int i = 0; i < kGranules; ++i)
                     if (!(live >> i & 1)) bits &= ~(0xFFFFull << (kGranule * i));
+                return bits;
+            };
+            if (__any_sync(~0u, see < kStep) || (live & kAllLive) != kAllLive) {
+                const uint64_t bits = seen_bits();
 #pragma unroll
                 for (int i = 0; i < kStep; ++i)
                     if (!(bits >> i & 1)) x[i] = -INFINITY;
@@ -1467,39 +1607,44 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs& p, ChunkShared<D>&
             for (int j = 0; j < kStep; j += 8)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) tops[i] = max3(tops[i], x[j + 2 * i], x[j + 2 * i + 1]);
-            const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * f;
-            float keep = 1.0f;
-            if (top > m + kSlack) {
-                keep = exp2_fast(m - top);
-                m = top, l *= keep;
-            }
-            if (now_v != v_scale) {
-                keep *= v_scale / now_v;
-                v_scale = now_v;
-            }
-            if (step > begin && __any_sync(~0u, keep != 1.0f)) {
-                // The sums so far, in tensor memory, once the step before is in them.
-                if (!warp_wait(&sh.c.o_full[tile][(turn - 1) % 2], (turn - 1) / 2 % 2, sh.c)) return;
-                fence_after();
-#pragma unroll 1
-                for (int i = 0; i < D / 16; ++i) {
-                    float y[16];
-                    __syncwarp();                        // lanes meet before each access to tensor memory
-                    tensor_load(sums + 16 * i, y);
-                    tensor_loaded(y);
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) y[j] *= keep;
-                    tensor_store(sums + 16 * i, y);
+            float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * f;
+            if ((live & kApart) || __any_sync(~0u, top > limit)) {
+                uint64_t* const summed = step > begin ? &sh.c.o_full[tile][(turn - 1) % 2] : nullptr;
+                const uint32_t parity = (turn - 1) / 2 % 2;
+                if ((live & kApart) || __any_sync(~0u, odd)) {
+                    const bool apart = live & kApart;
+                    RowState now{m, e, l};
+                    if (!step_alone<D>(now, at, seen_bits(), apart ? sh.c.k_own[it % kScales] : nullptr,
+                                       sh.c.v_own[it % kScales], factor, f, power, sums, summed, parity, sh.c))
+                        return;
+                    m = now.m, e = now.e, l = now.l;
+                    weighed();
+                    continue;
                 }
+                // With a larger maximum of the sums comes one of the scores, so that e is no larger than the powers seen.
+                const bool lift = top - m + power > e + kSlack;
+                if (top > m + (lift ? 0.0f : kSlack)) {      // leaves m + e, and so the sums, as they are
+                    const float up = ceilf(top);
+                    l *= exp2_fast(m - up);
+                    e += m - up, m = up;
+                }
+                float keep = 1.0f;
+                if (lift) {
+                    const float up = ceilf(top - m) + power;
+                    keep = exp2_fast(e - up);
+                    e = up;
+                }
+                if (summed && __any_sync(~0u, keep != 1.0f) && !rescale<D>(sums, keep, summed, parity, sh.c)) return;
+                by = power - e - m, share = exp2_fast(fminf(e - power, kFarBelow));
             }
             float2 some[2] = {};
-            const float2 ff = make_float2(f, f), mm = make_float2(-m, -m);
+            const float2 ff = make_float2(f, f), bb = make_float2(by, by);
 #pragma unroll
             for (int i = 0; i < kStep; i += 32) {
                 uint32_t weights[16];
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
-                    float2 y = fma2(make_float2(x[i + 2 * j], x[i + 2 * j + 1]), ff, mm);
+                    float2 y = fma2(make_float2(x[i + 2 * j], x[i + 2 * j + 1]), ff, bb);
                     y.x = exp2_fast(y.x), y.y = exp2_fast(y.y);
                     some[j % 2] = add2(some[j % 2], y);
                     weights[j] = pack_half2(y.x, y.y);
@@ -1508,13 +1653,8 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs& p, ChunkShared<D>&
                 tensor_store(at + i / 2, weights);
             }
             some[0] = add2(some[0], some[1]);
-            l += some[0].x + some[0].y;
-            __syncwarp();
-            tensor_stored();
-            fence_before();
-            __syncwarp();
-            if (lane == 0) barrier_arrive(&sh.c.p_full[tile][turn % 2]);
-            ++turn;
+            l += (some[0].x + some[0].y) * share;
+            weighed();
         }
 
         if (!warp_wait(&sh.c.o_full[tile][(turn - 1) % 2], (turn - 1) / 2 % 2, sh.c)) return;
@@ -1523,7 +1663,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs& p, ChunkShared<D>&
         const int64_t slot = (2 * int64_t(blockIdx.x) + (begin == 0)) * kUnitRows + tile * kTile + warp_row;
         const bool nans = sh.c.nan_unit[unit % kNanUnits] == int(unit) + 1;
         // A row that sees no token has l = 0, and sums of zero weights that count as zeros.
-        const float by = l == 0.0f ? 0.0f : whole ? v_scale / l : v_scale;
+        const float by = l == 0.0f ? 0.0f : whole ? exp2_fast(e) / l : exp2_fast(e);
         // The queries are done with: their place takes the rows on their way out, 128 bytes of each at a time.
         char* const warp_rows = sh.q[tile] + warp_row * 128;
 #pragma unroll 1
