@@ -406,7 +406,9 @@ struct StepWarp {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const float f = factor[nt][i] * page.ks;
-                    sc[nt][i] = (sc[nt][i] + odd[nt][i]) * f, sc[nt][2 + i] = (sc[nt][2 + i] + odd[nt][2 + i]) * f;
+                    // rounded here: fused with the subtraction of m, a score of 2^26 could exceed its own maximum by 2^4
+                    sc[nt][i] = __fmul_rn(sc[nt][i] + odd[nt][i], f);
+                    sc[nt][2 + i] = __fmul_rn(sc[nt][2 + i] + odd[nt][2 + i], f);
                 }
             if (edge) {
 #pragma unroll
@@ -800,6 +802,7 @@ constexpr int kLookedUnits = 4;            // units
 constexpr float kKeysApart = 1.0f / 16384;  // a step's smallest key scale to its largest, and powers of value
 constexpr float kValuesApart = 6.0f;       // scales, up to which the conversion takes them
 constexpr float kFarBelow = 60.0f;         // powers of two below a row's e from which weights are summed apart
+constexpr float kLargeScore = 1048576.0f;  // size of scores from which they are rounded before m is taken away
 constexpr uint32_t kSumsAt = 256;          // columns of tensor memory: S and P 0 to 255, O from here
 
 struct ChunkArgs {
@@ -1415,6 +1418,8 @@ struct RowState {
 
 constexpr float kLeast = 1.17549435e-38f;  // the smallest normal number
 
+__device__ __forceinline__ bool large_score(float s) { return fabsf(s) > kLargeScore && s > kLowest / 2; }
+
 // Multiplies the sums so far in tensor memory, once the step before is in them.
 template <int D>
 __device__ __forceinline__ bool rescale(uint32_t sums, float keep, uint64_t* summed, uint32_t parity, ChunkControl& c) {
@@ -1433,7 +1438,8 @@ __device__ __forceinline__ bool rescale(uint32_t sums, float keep, uint64_t* sum
     return true;
 }
 
-// A step whose weights in the sums do not tell those of l: a granule of 16 columns at a time, three times. `k_own`: pages by their own scales. Weights take columns that
+// A step whose weights in the sums do not tell those of l: a granule of 16 columns at a time, three times, from
+// scores that are rounded before m is taken away. `k_own`: pages by their own scales. Weights take columns that
 // have been read. Out of line, as the loop over steps is to stay in the instruction cache: an 8k prompt takes
 // 697 us, with this in the loop's way 731, without it at all 689.
 template <int D>
@@ -1452,7 +1458,7 @@ __device__ __noinline__ bool step_alone(RowState& row, uint32_t at, uint64_t see
             const uint32_t see = uint32_t(seen >> (kGranule * i));
             tensor_loaded(y);
 #pragma unroll
-            for (int j = 0; j < kGranule; ++j) y[j] = see >> j & 1 ? y[j] * k : -INFINITY;
+            for (int j = 0; j < kGranule; ++j) y[j] = see >> j & 1 ? __fmul_rn(y[j], k) : -INFINITY;
             if (pass == 0) {
 #pragma unroll
                 for (int j = 0; j < kGranule; ++j) top = fmaxf(top, y[j]);
@@ -1584,8 +1590,9 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs& p, ChunkShared<D>&
             const uint32_t live = sh.c.live[it % kScales];
             const int see = min(max(seen - step * kStep, 0), kStep);       // columns up to here are seen
             // A weight in the sums is 2^(s f + by), and `share` of it is its part of l. That holds for scores up to
-            // `limit`: above it a maximum moves. Where the weights in the sums are too far below l's, no score is below it.
-            const bool odd = power - e < -kFarBelow;
+            // `limit`: above it a maximum moves. Where the weights in the sums are too far below l's, or scores so
+            // large that their rounding is no small part of a weight, no score is below it.
+            const bool odd = power - e < -kFarBelow || large_score(m);
             const float limit = odd ? 2 * kLowest : m + kSlack + fminf(e - power, 0.0f);
             float by = power - e - m, share = exp2_fast(fminf(e - power, kFarBelow));
             tensor_loaded(x);
@@ -1611,7 +1618,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs& p, ChunkShared<D>&
             if ((live & kApart) || __any_sync(~0u, top > limit)) {
                 uint64_t* const summed = step > begin ? &sh.c.o_full[tile][(turn - 1) % 2] : nullptr;
                 const uint32_t parity = (turn - 1) / 2 % 2;
-                if ((live & kApart) || __any_sync(~0u, odd)) {
+                if ((live & kApart) || __any_sync(~0u, odd || large_score(top))) {
                     const bool apart = live & kApart;
                     RowState now{m, e, l};
                     if (!step_alone<D>(now, at, seen_bits(), apart ? sh.c.k_own[it % kScales] : nullptr,

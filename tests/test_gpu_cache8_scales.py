@@ -84,7 +84,8 @@ def test_a_large_page_of_little_weight(shape, sequences, place, above, below):
     check(p, q, q_gpu, scale)
 
 
-@pytest.mark.parametrize("side,above", [(0, 8), (0, 20), (1, 8), (1, 16), (1, 30), (1, 70)])
+@pytest.mark.parametrize("side", [0, 1])
+@pytest.mark.parametrize("above", [8, 16, 30, 70])
 @pytest.mark.parametrize("shape", SHAPES, ids=str)
 @pytest.mark.parametrize("sequences", [[(5, 3), (6, 40)], [(45, 530), (20, 50)], [(400, 0)]], ids=str)
 def test_rows_do_not_depend_on_the_scales_of_later_tokens(side, above, shape, sequences):
@@ -148,3 +149,38 @@ def test_scales_that_are_no_powers_of_two(sequences):
             # a key's rounding moves each score by at most 2^-11 of its products' size, numerator and sum alike
             more = (2.0 ** -11 + 2 * (torch.expm1(2.0 ** -11 * size.amax(dim=1)))[:, None]) * spread
         assert ((got[row] - expected[row]).abs() <= bound[row] + more).all()
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+@pytest.mark.parametrize("sequences", [[(1, 530)], [(3, 200), (1, 40)], [(45, 530)], [(300, 0), (70, 90)]], ids=str)
+@pytest.mark.parametrize("size", [2.0 ** 24, 2.0 ** 27, 2.0 ** 40, 2.0 ** 90])
+def test_scores_so_large_that_one_token_takes_all(shape, sequences, size):
+    """Scores of `size` and its quarters: a row is the value of the one largest that it sees, exactly.
+
+    Scores beyond 2^24 lie further apart than weights reach; what bounds them is 32 bits.
+    """
+    dim, block_size, heads, group = shape
+    p = Paged(sequences, dim=dim, block_size=block_size, heads=heads, seed=12)
+    codes, scales = p.codes(), p.scales()
+    scales[:, 0] = 1.0
+    first = torch.zeros(codes.shape[1], block_size, heads)
+    late = 20                                              # the largest from here on; token 0 before it
+    for row, length in zip(p.table, p.lengths):
+        for i, b in enumerate(row[: -(-length // block_size)]):
+            first[b] = -448.0
+        first[row[0], 0] = 112.0
+        if length > late:
+            first[row[late // block_size], late % block_size] = 448.0
+    codes[0] = 0
+    codes[0][..., 0] = first.to(E4M3).view(torch.uint8)
+    p.codes_gpu.copy_(codes), p.scales_gpu.copy_(scales)
+    q, q_gpu = p.random(heads * group, torch.bfloat16, 7)
+    q[..., 0] = 1.5
+    q_gpu.copy_(q)
+    got = p.cache.attend("l", q_gpu, p.batch, scale=size / 672).cpu()
+    p.cache.check()
+    for s, row, position in rows_of(p.start, p.lengths):
+        at = late if position >= late else 0
+        block = p.table[s][at // block_size]
+        value = codes[1, block, at % block_size].view(E4M3).float() * scales[block, 1][:, None]
+        assert torch.equal(got[row].float(), value.repeat_interleave(group, dim=0))
