@@ -1932,7 +1932,7 @@ Plan plan_for(const Cache& c, const Batch& b, int q_heads, int sms) {
     // 27.3 and 39.6; 128 of 700 48.7 and 40.1; 200 of 700 65.6 and 69.6.
     const int64_t waves = (plan.step_units + sms - 1) / sms;
     const int64_t costs = 4 + (plan.step_units < 96 ? plan.step_units : 96) / 6;
-    plan.split = most * (2 * sms * waves - plan.step_units) > costs * 2 * sms;
+    plan.split = most_rows > 0 && most * (2 * sms * waves - plan.step_units) > costs * 2 * sms;
     plan.step_ctas = plan.split ? plan.ctas : plan.step_units;
     // The two kernels may run at the same time: each has its own part of the workspace.
     plan.step_slots = plan.stepped && plan.split ? 2 * plan.ctas * p.hc * kStepRows : 0;

@@ -1,0 +1,41 @@
+"""Calls of the 8-bit cache at the edges of what it takes, on a B200."""
+import pytest
+import torch
+
+from test_gpu_cache8 import Paged
+
+pytestmark = pytest.mark.gpu
+
+
+def expand_one(cache):
+    """A conversion of one block: any later call of the thread."""
+    codes = cache.codes["l"]
+    wide = torch.zeros((2, 1, *codes.shape[2:]), dtype=torch.bfloat16, device="cuda")
+    cache.converter({"l": wide}).expand([0], [0])
+    torch.cuda.synchronize()
+
+
+def wide_table(p, width):
+    """The batch of `p` over a table of `width` pages a sequence."""
+    from kvsnap_b200.cache8 import PagedBatch
+    held = p.batch.table
+    table = torch.zeros((held.shape[0], width), dtype=torch.int32, device="cuda")
+    table[:, : held.shape[1]] = held
+    return PagedBatch(table, p.batch.start, p.batch.lengths, max_query=p.batch.max_query)
+
+
+@pytest.mark.parametrize("group", [1, 4, 24])
+@pytest.mark.parametrize("width", [5, 96, 4000])
+@pytest.mark.parametrize("seqs", [1, 7])
+def test_a_bound_of_no_rows(seqs, width, group):
+    """A padded step in which no sequence has rows, on both sides of the rule that cuts a step: nothing is written."""
+    p = Paged([(0, 37)] * seqs, heads=8, dim=64, pad_rows=5, max_query=0)
+    p.batch = wide_table(p, width)
+    before = p.codes(), p.scales()
+    out = torch.full((5, 8 * group, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    q, k = p.random(8 * group, torch.bfloat16)[1], p.random(8, torch.bfloat16)[1]
+    p.cache.append("l", k, k, p.batch)
+    p.cache.attend("l", q, p.batch, out=out)
+    expand_one(p.cache)
+    p.cache.check()
+    assert (out == 7).all() and torch.equal(p.codes(), before[0]) and torch.equal(p.scales(), before[1])
