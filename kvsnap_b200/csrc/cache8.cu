@@ -486,10 +486,9 @@ int convert(const kvsnap_c8_pair* pairs, int layers, int block_size, int kv_head
             using T = decltype(t);
             constexpr int D = decltype(d)::value;
             const auto s = reinterpret_cast<cudaStream_t>(stream);
-            if (EXPAND) expand_kernel<T, D><<<grid, 256, 0, s>>>(a);
-            else compress_kernel<T, D><<<grid, 256, 0, s>>>(a);
+            if (EXPAND) launch(expand_kernel<T, D>, grid, 256, 0, s, false, a);
+            else launch(compress_kernel<T, D>, grid, 256, 0, s, false, a);
         });
-        check(cudaGetLastError());
     });
 }
 

@@ -168,8 +168,11 @@ struct Fail {
     const char* what;
 };
 
+// A call's error is its own: it is not left behind as the thread's last one, which later launches would take for theirs.
 void check(cudaError_t rc) {
-    if (rc != cudaSuccess) throw Fail{cudaGetErrorString(rc)};
+    if (rc == cudaSuccess) return;
+    cudaGetLastError();
+    throw Fail{cudaGetErrorString(rc)};
 }
 
 void require(bool ok, const char* what) {

@@ -1,4 +1,6 @@
-"""Calls of the 8-bit cache at the edges of what it takes, on a B200."""
+"""Calls of the 8-bit cache at the edges of what it takes, on a B200: bounds of no rows, launches that cannot be,
+batches and positions that do not fit, and the sizes at which its kernels change their way.
+"""
 import pytest
 import torch
 
@@ -39,3 +41,15 @@ def test_a_bound_of_no_rows(seqs, width, group):
     expand_one(p.cache)
     p.cache.check()
     assert (out == 7).all() and torch.equal(p.codes(), before[0]) and torch.equal(p.scales(), before[1])
+
+
+def test_a_launch_that_cannot_be_leaves_later_calls_alone():
+    """More query heads than a grid holds: the call fails, and the calls after it do not."""
+    from kvsnap_b200.cache8 import rotary_table
+    p = Paged([(1, 3)], heads=2, dim=64)
+    k = p.random(2, torch.bfloat16)[1]
+    q = torch.zeros((1, 8 * 65536, 64), dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(RuntimeError):
+        p.cache.append("l", k, k, p.batch, query=q, rotary=rotary_table(8, 64))
+    expand_one(p.cache)
+    p.cache.check()
