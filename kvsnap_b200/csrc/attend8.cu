@@ -1908,7 +1908,8 @@ Plan plan_for(const Cache& c, const Batch& b, int q_heads, int sms) {
     plan.most_rows = int(most_rows);
     // With one sequence, the kernel for many rows takes it whatever it holds: one launch, not two (a prompt
     // of 300 tokens 29.3 us, else 32.8).
-    plan.stepped = group <= kStepRows && !(plan.chunked && b.seqs == 1);
+    // Where no sequence may have rows, it is there to record those that do.
+    plan.stepped = !plan.chunked || (group <= kStepRows && b.seqs > 1);
     plan.step_rows = plan.stepped ? kStepRows : 0;
     plan.wide = most_rows > 8;
     // Heads a CTA: up to 8, whose lines of a token lie side by side; but few sequences are spread over CTAs by

@@ -53,3 +53,13 @@ def test_a_launch_that_cannot_be_leaves_later_calls_alone():
         p.cache.append("l", k, k, p.batch, query=q, rotary=rotary_table(8, 64))
     expand_one(p.cache)
     p.cache.check()
+
+
+@pytest.mark.parametrize("group", [1, 24])
+def test_rows_beyond_a_bound_of_none_are_reported(group):
+    p = Paged([(0, 37), (2, 20)], heads=2, dim=64, max_query=0)
+    out = torch.full((2, 2 * group, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    p.cache.attend("l", p.random(2 * group, torch.bfloat16)[1], p.batch, out=out)
+    with pytest.raises(ValueError, match="length"):
+        p.cache.check()
+    assert (out == 7).all()
