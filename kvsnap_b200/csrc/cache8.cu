@@ -46,7 +46,7 @@ __device__ __forceinline__ bool find_page(const Batch& b, int n, int64_t u, Page
     }
     const int from = start[s], to = start[s + 1], length = ints(b.lengths)[s];
     if (from >= to || length <= 0) return false;
-    if (from < 0 || to > b.rows || (SINGLE && to - from > 1) || int64_t(length) > int64_t(b.width) * n) {
+    if (from < 0 || to > b.rows || to - from > b.max_query || int64_t(length) > int64_t(b.width) * n) {
         atomicOr(status, KVSNAP_C8_BAD_LENGTH);
         return false;
     }

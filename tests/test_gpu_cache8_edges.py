@@ -63,3 +63,18 @@ def test_rows_beyond_a_bound_of_none_are_reported(group):
     with pytest.raises(ValueError, match="length"):
         p.cache.check()
     assert (out == 7).all()
+
+
+@pytest.mark.parametrize("sequences,bound", [([(5, 20), (9, 3), (1, 16)], 8), ([(1, 20), (0, 3)], 0), ([(2, 4)], 1)], ids=str)
+def test_an_append_keeps_to_its_bound(sequences, bound):
+    """A sequence of more rows than max_query is left out and reported; the others are appended."""
+    p = Paged(sequences, heads=2, dim=64, max_query=bound)
+    held, k = p.codes(), p.random(2, torch.bfloat16, 3)[1]
+    p.cache.append("l", k, k, p.batch)
+    with pytest.raises(ValueError, match="length"):
+        p.cache.check()
+    now = p.codes()
+    for (new, _), row, length in zip(sequences, p.table, p.lengths):
+        pages = row[: -(-length // p.block_size)]
+        same = all(torch.equal(held[:, b], now[:, b]) for b in pages)
+        assert same == (new > bound or new == 0)
