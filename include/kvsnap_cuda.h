@@ -381,7 +381,7 @@ typedef struct kvsnap_c8_batch {
 /* Status bits beside KVSNAP_DP_BAD_BLOCK (a table entry outside the cache). A
    kernel that sets one has skipped what the bit is about, not faulted. */
 #define KVSNAP_C8_BAD_LENGTH 16u     /* lengths, start or max_query do not fit the table or the rows */
-#define KVSNAP_C8_BAD_POSITION 32u   /* a position behind the rotary table's end */
+#define KVSNAP_C8_BAD_POSITION 32u   /* a position behind the rotary table's end: its token is left out */
 #define KVSNAP_C8_STALLED 64u        /* a wait inside a kernel ran out (two seconds): its results are not valid */
 
 /*

@@ -201,7 +201,8 @@ class PagedCache8:
         ``rotary``: a :func:`rotary_table` (any rotary_dim up to head_dim); keys are rotated on the way in 32
         bits, pairs (i, i + rotary_dim / 2) or, ``interleaved``, (2i, 2i + 1). ``query`` ``[rows, q_heads,
         head_dim]`` is rotated the same way, and returned as a new tensor (None without ``query``). Its rows
-        that are no sequence's, or whose position would be negative, are unspecified.
+        that are no sequence's, or whose position would be negative or lies behind the table, are unspecified.
+        Tokens behind the table are not written, and reported by :meth:`check`.
 
         A page's scale only grows while tokens are added to it, older codes being rounded again; a page whose
         first slot is written starts anew. Slots behind a sequence's last token keep their codes. Sequences

@@ -61,6 +61,16 @@ __device__ __forceinline__ bool find_page(const Batch& b, int n, int64_t u, Page
     return true;
 }
 
+// The page's rows that the rotary table has angles for; false where there are none. The others are left out and
+// recorded.
+__device__ __forceinline__ bool within_table(const AppendArgs& a, PageRun& run) {
+    const int64_t left = a.positions - (int64_t(run.page) * a.c.block_size + run.first);
+    if (!a.rotary_dim || left >= run.count) return true;
+    if (threadIdx.x == 0) atomicOr(a.status, KVSNAP_C8_BAD_POSITION);
+    run.count = int(max(left, int64_t(0)));
+    return run.count > 0;
+}
+
 // A lane's 8 elements of a row of rotated heads: 4 from `low` on and 4 from `high` on, 4 whole pairs, so that
 // nothing passes between lanes and a row's angles are read once: of a row of 16 lanes each reads 8 bytes
 // of two lines, and 32 bytes of angles. Elements from rotary_dim on, and interleaved pairs, lie together.
@@ -82,7 +92,7 @@ struct Turn {
 
 __device__ __forceinline__ void fetch_turn(Turn& turn, const AppendArgs& a, int64_t position, const Place& at,
                                            bool there) {
-    const float2* from = a.rotary + min(position, a.positions - 1) * (a.rotary_dim / 2) + at.pair;
+    const float2* from = a.rotary + position * (a.rotary_dim / 2) + at.pair;
 #pragma unroll
     for (int i = 0; i < 2; ++i) turn.x[i] = fetch16(reinterpret_cast<const char*>(from + 2 * i), there && at.turned);
 }
@@ -164,7 +174,7 @@ __device__ __forceinline__ void turn_queries(const AppendArgs& a, int y) {
     constexpr int kLanes = D / 8, kRows = 32 / kLanes, kTogether = SINGLE ? 1 : 8;
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, n = a.c.block_size;
     PageRun run;
-    if (!find_page<SINGLE>(a.b, n, blockIdx.x, run, a.status)) return;
+    if (!find_page<SINGLE>(a.b, n, blockIdx.x, run, a.status) || !within_table(a, run)) return;
     const int sub = lane / kLanes, end = run.first + run.count;
     const int base = run.page * n;                               // position of the page's slot 0
     const Place place(lane % kLanes, a.rotary_dim, INTERLEAVED);
@@ -199,10 +209,9 @@ __device__ __forceinline__ void append_rows(const AppendArgs& a, int y) {
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, n = a.c.block_size, slot = y * 8 + warp;
     if (slot >= 2 * a.c.kv_heads) return;
     PageRun run;
-    if (!find_page<SINGLE>(a.b, n, blockIdx.x, run, a.status)) return;
+    if (!find_page<SINGLE>(a.b, n, blockIdx.x, run, a.status) || !within_table(a, run)) return;
     const int sub = lane / kLanes, at = lane % kLanes * 8, end = run.first + run.count;
     const int base = run.page * n;                               // position of the page's slot 0
-    if (a.rotary_dim && base + end > a.positions && threadIdx.x == 0) atomicOr(a.status, KVSNAP_C8_BAD_POSITION);
     const Place place(lane % kLanes, a.rotary_dim, INTERLEAVED);
 
     const int side = slot / a.c.kv_heads, head = slot % a.c.kv_heads;

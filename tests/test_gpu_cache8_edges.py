@@ -78,3 +78,36 @@ def test_an_append_keeps_to_its_bound(sequences, bound):
         pages = row[: -(-length // p.block_size)]
         same = all(torch.equal(held[:, b], now[:, b]) for b in pages)
         assert same == (new > bound or new == 0)
+
+
+@pytest.mark.parametrize("sequences,positions", [
+    ([(3, 40)], 42), ([(3, 40)], 40), ([(3, 40)], 17), ([(40, 5), (1, 16), (9, 0)], 21), ([(1, 20), (1, 9), (1, 16)], 16),
+    ([(20, 0), (2, 3)], 1)], ids=str)
+def test_positions_behind_the_rotary_table_are_left_out(sequences, positions):
+    """Their tokens are not written and set no scale; all others are as if the call ended before them."""
+    from kvsnap_b200.cache8 import PagedBatch, rotary_table
+    p, same = Paged(sequences, heads=2, dim=64, seed=4), Paged(sequences, heads=2, dim=64, seed=4)
+    k, v = p.random(2, torch.bfloat16, 3)[1].clone(), p.random(2, torch.bfloat16, 5)[1].clone()
+    q = p.random(4, torch.bfloat16, 6)[1]
+    for s, length in enumerate(p.lengths):                 # what is left out is the largest
+        behind = min(max(length - positions, 0), p.start[s + 1] - p.start[s])
+        k[p.start[s + 1] - behind: p.start[s + 1]] *= 100
+        v[p.start[s + 1] - behind: p.start[s + 1]] *= 100
+    table = rotary_table(64, 64)
+    got_q = p.cache.append("l", k, v, p.batch, query=q, rotary=table[:positions].contiguous())
+    with pytest.raises(ValueError, match="rotary"):
+        p.cache.check()
+    # The same rows, sequence by sequence, up to the table's end.
+    for s, length in enumerate(p.lengths):
+        new = p.start[s + 1] - p.start[s]
+        held = length - new
+        kept = min(max(positions - held, 0), new)
+        if not kept:
+            continue
+        rows = slice(p.start[s], p.start[s] + kept)
+        one = PagedBatch(p.batch.table[s: s + 1], torch.tensor([0, kept], dtype=torch.int32).cuda(),
+                         torch.tensor([held + kept], dtype=torch.int32).cuda())
+        want_q = same.cache.append("l", k[rows], v[rows], one, query=q[rows], rotary=table)
+        assert torch.equal(got_q[rows], want_q)
+    same.cache.check()
+    assert torch.equal(p.codes(), same.codes()) and torch.equal(p.scales(), same.scales())
