@@ -92,7 +92,9 @@ struct Turn {
 
 __device__ __forceinline__ void fetch_turn(Turn& turn, const AppendArgs& a, int64_t position, const Place& at,
                                            bool there) {
-    const float2* from = a.rotary + position * (a.rotary_dim / 2) + at.pair;
+    // Lanes past the page's rows have positions too, for which nothing is fetched. They are held within the table:
+    // without that the compiler's code for an 8k prompt takes 53.3 us, so 52.3.
+    const float2* from = a.rotary + min(position, a.positions - 1) * (a.rotary_dim / 2) + at.pair;
 #pragma unroll
     for (int i = 0; i < 2; ++i) turn.x[i] = fetch16(reinterpret_cast<const char*>(from + 2 * i), there && at.turned);
 }
