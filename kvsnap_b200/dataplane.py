@@ -478,6 +478,23 @@ def _block_views(scales):
     return views
 
 
+def _check_scales(caches, scales):
+    """Refuses scales that are not those of the registered codes: blocks would be saved, and read again, without theirs."""
+    import torch
+    missing = [name for name, tensor in caches.items() if tensor.dtype is torch.float8_e4m3fn and name not in scales]
+    if missing:
+        raise ValueError(f"scales of {missing[0]} are missing: with scales, every float8_e4m3fn layer has some")
+    for name, scale in scales.items():
+        if name not in caches:
+            raise ValueError(f"scales of {name}, which is no registered layer")
+        codes = caches[name]
+        shape = tuple(codes.shape)
+        if len(shape) != 5 or shape[0] != 2 or codes.element_size() != 1:
+            raise ValueError(f"scales of {name}, which is no 8-bit [2, blocks, block_size, kv_heads, head_dim] layer")
+        if scale.dtype is not torch.float32 or tuple(scale.shape) != (shape[1], 2, shape[3]):
+            raise ValueError(f"scales of {name} must be float32 [{shape[1]}, 2, {shape[3]}], as its codes are")
+
+
 def _layer_record(name, tensor, block_size, device):
     """The reference's record of one registered layer view, after its checks (reference dataplane.py:230-247).
 
@@ -604,7 +621,10 @@ class TorchBlockDataPlane:
     ``scales`` (layer name -> contiguous float32 ``[blocks, 2, kv_heads]``): the
     scales of caches held in 8 bits (:mod:`kvsnap_b200.cache8`), saved and
     restored with their blocks; the packed block then has a ``name.scale`` span
-    a layer.
+    a layer. With it, every ``float8_e4m3fn`` layer must have scales of its own
+    blocks and heads; layers of 16 bits may be registered beside them. Without
+    it, 8-bit layers are moved as they are (for caches whose scales are not a
+    block's, and are kept elsewhere).
     """
 
     save_mode = "staged"
@@ -621,6 +641,8 @@ class TorchBlockDataPlane:
         views, block_views = _split_paged(caches, block_size), _block_views(scales)
         if views.keys() & block_views.keys():
             raise ValueError("a layer's name collides with another's scales")
+        if scales is not None:
+            _check_scales(caches, scales)
         self.block_views = frozenset(block_views)
         self.caches = dict(sorted({**views, **block_views}.items()))
         self.block_size = block_size
