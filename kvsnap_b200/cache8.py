@@ -17,7 +17,8 @@ the host link in half the time, scales included.
 Every call runs on the caller's current stream of the cache's device, allocates only its outputs and
 workspaces there, never waits for the GPU, and can be captured into a CUDA graph (block ids given as lists
 are copied to the GPU first: both need tensors). Tables and lengths are read on the GPU; what a kernel finds
-wrong with them it skips and records, and ``check()`` raises. For serving: no gradients are taken.
+wrong with them it skips and records, and ``check()`` raises. For serving: no gradients are taken, and rows
+that ask for some are refused (call under ``torch.no_grad()`` or ``torch.inference_mode()``).
 """
 from __future__ import annotations
 
@@ -146,6 +147,7 @@ class PagedCache8:
             self._records[name] = _abi.C8Cache(tensor.data_ptr(), scale.data_ptr(), *pitches[:4], tensor.shape[1],
                                                *shape[2:], self.device.index, 0)
         self._lib, self._current_stream, self._index = _dp(_load()), _raw_stream(), first.device.index
+        self._grad_enabled = torch.is_grad_enabled
         if not hasattr(self._lib, "kvsnap_c8_append"):
             raise RuntimeError("the CUDA library has no 8-bit cache kernels; rebuild with python -m kvsnap_b200.build")
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
@@ -171,6 +173,8 @@ class PagedCache8:
         """(address, token pitch, head pitch) in bytes of ``[rows, heads, head_dim]`` 16-bit rows."""
         if tensor.device != self.device:
             raise ValueError(f"{what} must be on {self.device}")
+        if tensor.requires_grad and self._grad_enabled():
+            raise ValueError(f"{what} requires a gradient, which the 8-bit cache does not take: call under torch.no_grad()")
         shape = tensor.shape
         if len(shape) != 3 or shape[2] != self.head_dim or (heads and shape[1] != heads):
             raise ValueError(f"{what} must be [rows, {heads or 'heads'}, {self.head_dim}]")

@@ -4,7 +4,7 @@ from unittest.mock import patch
 import pytest
 import torch
 
-from test_cache8_host import OnCuda
+from test_cache8_host import OnCuda, batch, make, rows  # noqa: F401 (make is a fixture)
 
 
 class View(OnCuda):
@@ -58,3 +58,21 @@ def test_scales_beside_layers_of_16_bits_and_8_bits_without_scales():
     assert [layer["name"] for layer in plane({"a": codes()}, None).layers] == ["a.k", "a.v"]
     assert [layer["name"] for layer in plane({"a": codes(dtype=torch.uint8)}, {"a": scale()}).layers] == ["a.k", "a.scale", "a.v"]
     assert [layer["name"] for layer in plane({"a": codes(dtype=torch.bfloat16)}, {}).layers] == ["a.k", "a.v"]
+
+
+@pytest.mark.parametrize("which", ["key", "value", "query"])
+def test_rows_that_require_a_gradient_are_refused(make, which):    # noqa: F811
+    """They would be detached without a word."""
+    given = {"key": rows(), "value": rows(), "query": rows(heads=4)}
+    given[which]._tensor.requires_grad_()
+    rotary = OnCuda(torch.zeros((9, 32, 2)))
+    cache = make()
+    with pytest.raises(ValueError, match=f"{which} requires a gradient"):
+        cache.append("l", given["key"], given["value"], batch(), query=given["query"], rotary=rotary)
+    if which == "query":
+        with pytest.raises(ValueError, match="query requires a gradient"):
+            cache.attend("l", given["query"], batch())
+    else:
+        cache._rows(which, given["query"])
+    with torch.no_grad():                                  # as a model that serves calls it
+        assert cache._rows(which, given[which])
