@@ -302,6 +302,7 @@ class PagedCache8:
         found = int(self.status.item())
         if found:
             self.status.zero_()
+            torch.cuda.synchronize(self.device)              # before a call on another stream records anew
             raise ValueError("8-bit cache: " + "; ".join(text for bit, text in _PROBLEMS.items() if found & bit))
 
 

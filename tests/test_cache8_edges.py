@@ -76,3 +76,22 @@ def test_rows_that_require_a_gradient_are_refused(make, which):    # noqa: F811
         cache._rows(which, given["query"])
     with torch.no_grad():                                  # as a model that serves calls it
         assert cache._rows(which, given[which])
+
+
+def test_check_clears_what_it_found_before_it_returns(make):    # noqa: F811
+    """A call on another stream after it must not have its record cleared."""
+    cache, order = make(), []
+
+    class Word:
+        def item(self):
+            order.append("read")
+            return 32
+
+        def zero_(self):
+            order.append("clear")
+
+    cache.status = Word()
+    with patch.object(torch.cuda, "synchronize", lambda device: order.append("wait")):
+        with pytest.raises(ValueError, match="rotary"):
+            cache.check()
+    assert order == ["wait", "read", "clear", "wait"]
