@@ -4,7 +4,8 @@ batches and positions that do not fit, and the sizes at which its kernels change
 import pytest
 import torch
 
-from test_gpu_cache8 import Paged
+from cache8_reference import attend
+from test_gpu_cache8 import Paged, check_append, check_attend
 
 pytestmark = pytest.mark.gpu
 
@@ -111,3 +112,54 @@ def test_positions_behind_the_rotary_table_are_left_out(sequences, positions):
         assert torch.equal(got_q[rows], want_q)
     same.cache.check()
     assert torch.equal(p.codes(), same.codes()) and torch.equal(p.scales(), same.scales())
+
+
+# ---- sizes at which the kernels change their way --------------------------------------------------
+
+
+def test_more_sequences_than_a_step_finds_in_one_pass():
+    """More than 512 sequences whose work is cut: a CTA's share is sought a part of them at a time."""
+    sequences = [(1, 250 + s * 37 % 350) for s in range(600)]
+    check_attend(Paged(sequences, dim=64, heads=8, poison=True), torch.bfloat16, 2)
+
+
+def test_more_sequences_than_a_chunk_call_scans_at_once():
+    """More than 256 sequences of 1 or 20 new tokens: both kernels, and the second scan of the chunks' one."""
+    sequences = [(20 if s % 3 == 0 else 1, s * 29 % 150) for s in range(300)]
+    check_attend(Paged(sequences, dim=64, heads=2, poison=True), torch.float16, 2)
+
+
+@pytest.mark.parametrize("heads,group", [(3, 2), (5, 1), (6, 2), (7, 2), (16, 2), (10, 1), (14, 1), (24, 1)])
+def test_heads_that_do_not_fill_a_cta(heads, group):
+    """Numbers of KV heads that share a CTA's 16 warps with some to spare, and several groups of heads."""
+    sequences = [(1, s * 41 % 230) for s in range(60)]
+    check_attend(Paged(sequences, dim=64, heads=heads, poison=True), torch.bfloat16, group)
+    check_attend(Paged([(1 + s % 2, s * 41 % 1900) for s in range(30)], dim=64, heads=heads), torch.float16, group)
+
+
+@pytest.mark.parametrize("group,rows", [(16, 1), (12, 1), (5, 3), (3, 5), (8, 2), (9, 1)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_steps_of_9_to_16_rows_a_head(dim, group, rows):
+    sequences = [(rows, 300 + s * 53 % 700) for s in range(9)]
+    check_attend(Paged(sequences, dim=dim, heads=2, poison=True), torch.bfloat16, group)
+
+
+@pytest.mark.parametrize("group", [17, 24, 40])
+def test_groups_of_more_than_16_heads(group):
+    check_attend(Paged([(1, 300), (2, 40), (0, 9), (1, 0)], dim=64, heads=2, poison=True), torch.bfloat16, group)
+
+
+@pytest.mark.parametrize("sequences,width", [([(1, 128)], 2560), ([(1, 200 + s) for s in range(64)], 2560),
+                                             ([(1, 300 + s % 400) for s in range(128)], 300)], ids=["one", "64", "128"])
+def test_a_table_wider_than_its_sequences(sequences, width):
+    """An engine's table is as wide as its longest sequence may be: the same results as over a trimmed one."""
+    p = Paged(sequences, dim=64, heads=4)
+    q, q_gpu = p.random(8, torch.bfloat16)
+    got = p.cache.attend("l", q_gpu, wide_table(p, width)).cpu().double()
+    p.cache.check()
+    expected, bound = attend(q, p.codes(), p.scales(), p.table, p.start, p.lengths, p.block_size, p.dim ** -0.5)
+    assert ((got - expected).abs() <= bound).all()
+
+
+def test_an_append_over_many_sequences():
+    check_append(Paged([(1 + s % 3, s * 31 % 90) for s in range(300)], dim=64, heads=2), torch.bfloat16, group=1, rotary_dim=64)
