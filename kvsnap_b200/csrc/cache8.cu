@@ -465,10 +465,11 @@ extern "C" int kvsnap_c8_append(const kvsnap_c8_cache* cache, const kvsnap_c8_ba
                 run(interleaved ? append_one_kernel<T, D, true> : append_one_kernel<T, D, false>, kv_ctas + q_ctas, false);
                 return;
             }
-            // Queries in a launch of their own are worth it from two full waves of the GPU on (an 8k prompt
-            // 38 us of kernels, together 49); below that the launch costs more (5 sequences of up to 701 tokens,
-            // 350 CTAs, appended and read back in 18.2 us together, 19.8 apart).
-            const bool apart = q_ctas && units * (kv_ctas + q_ctas) > 600;
+            // Queries in a launch of their own are worth it from three full waves of the GPU's 148 SMs on; below that
+            // the launch costs more. Of 32 and 8 heads of 128, together and apart, in us (a call; in a graph): 1500
+            // tokens, 576 CTAs, 11.9 and 14.2 (9.2, 10.1); 2600, 984 CTAs, 16.9 and 17.0 (14.1, 14.4); 4000,
+            // 1512 CTAs, 23.0 and 21.0 (20.1, 18.8); 8192, 3084 CTAs, 41.6 and 39.9 (39.5, 37.5).
+            const bool apart = q_ctas && units * (kv_ctas + q_ctas) > 1000;
             run(interleaved ? append_kernel<T, D, true> : append_kernel<T, D, false>, kv_ctas + (apart ? 0 : q_ctas), false);
             if (apart) run(interleaved ? turn_kernel<T, D, true> : turn_kernel<T, D, false>, q_ctas, true);
         });

@@ -163,3 +163,26 @@ def test_a_table_wider_than_its_sequences(sequences, width):
 
 def test_an_append_over_many_sequences():
     check_append(Paged([(1 + s % 3, s * 31 % 90) for s in range(300)], dim=64, heads=2), torch.bfloat16, group=1, rotary_dim=64)
+
+
+@pytest.mark.parametrize("sequences", [[(1, 90), (1, 33)], [(24, 90), (20, 7)]], ids=str)
+def test_nan_queries_and_keys_reach_who_they_concern(sequences):
+    """A NaN in a row's query is that row's and head's; one in a key is the rows' that see it, of its head."""
+    p = Paged(sequences, heads=2, dim=64)
+    q, q_gpu = p.random(8, torch.bfloat16)
+    q[0, 5, 7] = float("nan")                              # KV head 1
+    last = p.lengths[1] - 1                                # the last token of sequence 1
+    p.codes_gpu[0, p.table[1][last // 16], last % 16, 0, 9] = 0x7F
+    q_gpu.copy_(q)
+    got = p.cache.attend("l", q_gpu, p.batch).cpu().double()
+    p.cache.check()
+    final = p.start[2] - 1
+    assert got[0, 5].isnan().all() and got[final, :4].isnan().all()
+    got[0, 5] = 0
+    got[final, :4] = 0
+    q[0, 5, 7] = 0
+    expected, bound = attend(q, p.codes(), p.scales(), p.table, p.start, p.lengths, p.block_size, p.dim ** -0.5)
+    expected[0, 5] = 0
+    expected[final, :4] = 0
+    bound = bound.nan_to_num(1.0)
+    assert ((got - expected).abs() <= bound).all()
