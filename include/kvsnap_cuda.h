@@ -395,7 +395,8 @@ typedef struct kvsnap_c8_batch {
  * A page that already holds tokens of its sequence keeps its scale or grows it
  * to what the new tokens need, and its older codes are then rounded again at
  * the new scale; a page whose first slot is written starts anew. Slots behind
- * the last token keep their codes. Infinities become the largest value the
+ * the last token keep their codes. Tokens behind the rotary table's last
+ * position, and all of a sequence that does not fit, are left out. Infinities become the largest value the
  * block's scale holds, NaN stays NaN. Two sequences that append in one call
  * must not share the page they append to.
  */
@@ -409,8 +410,10 @@ int kvsnap_c8_append(const kvsnap_c8_cache* cache, const kvsnap_c8_batch* batch,
  * Attention of query rows [rows][q_heads][head_dim] over their sequences'
  * cached tokens: out[i][h] = sum_j softmax_j(scale * q.k_j) v_j over positions j
  * up to the row's own. Query heads g * q_heads / kv_heads .. share KV head g.
- * A row that sees no token is zeros; rows that belong to nobody are not
- * written. out is dense and of the query's type. The workspace is device memory,
+ * A row that sees no token is zeros; rows that belong to nobody, or to a
+ * sequence that does not fit, are not written. out may be query if that is
+ * dense. A weight times its page's value scale is rounded to 16 bits once,
+ * relative to the row's largest such product. out is dense and of the query's type. The workspace is device memory,
  * 16-byte aligned, of at least kvsnap_c8_attend_workspace's bytes for the same
  * cache, batch and heads; calls that may overlap need one each. What it holds
  * before does not matter.

@@ -256,7 +256,15 @@ class PagedCache8:
         included. ``scale`` (not negative) multiplies the scores, 1 / sqrt(head_dim) by default. Query heads g * group to
         (g + 1) * group - 1 share KV head g. ``out``: a contiguous tensor like ``query`` to write to. A row
         that sees no token is zeros; rows that are no sequence's are left as they are in ``out`` (unspecified
-        without it). Sums and the softmax's statistics are 32-bit; weights and cached values meet in 16 bits.
+        without it), and so are those of a sequence that does not fit. ``out`` may be ``query``.
+
+        Sums and the softmax's statistics are 32-bit. A weight times its page's value scale is rounded to 16 bits
+        once: by at most 2^-11 of itself or 2^-24 of the row's largest such product, whichever is more (in
+        sequences of many new rows a page's scale counts for the latter as up to 2^6 more, where its neighbours' are).
+        A scale that is no power of two is itself rounded to 16 bits there.
+
+        Sequences of up to 16 rows a KV head (query heads of a group times new tokens) are read at the memory's
+        rate; others, groups of more than 16 heads among them, 256 rows at a time.
         """
         import torch
         cache, dtype, shape = self._layer(layer), query.dtype, query.shape

@@ -97,7 +97,8 @@ struct Parts {
 //
 // Sequences with at most kStepRows rows a KV head (query heads of the group times
 // new tokens): what m16n8k16 products take without idle rows, while the kernel below works on 256 rows
-// whatever there are (16 sequences of 8000 tokens with 8 rows a head: 61 us, there 153; with 16 rows 113).
+// whatever there are (16 sequences of 8000 tokens with 8 rows a head: 58 us, there 153; with 16 rows, whose
+// registers spill at 128 dims, 98; 64 of 512 to 8192 with 4, 8, 16 and 24 rows 107, 110, 185 and, there, 323).
 // Bound by the cache's bytes, so nothing but a page's codes is read, once: a step of 64 sessions of 512 to
 // 8192 tokens with 8 heads of 128, 372 MB, takes 70 us, 5.3 TB/s, of which the loop over granules runs at 86 %
 // of the rate of a plain copy, and the rest is the scan for a CTA's chunks (2 us), the first copies'
@@ -688,8 +689,9 @@ __global__ void __launch_bounds__(32 * kWarps, 1) step_kernel(const __grid_const
 // Joins the parts of the shared unit that a CTA of the kernels before began, which lie in consecutive CTAs'
 // slots: the first CTAs those of the kernel for few rows, `first_high` of each, the others the chunks'. Where
 // units have few parts (WIDE false) a warp takes a row, else a CTA does, its warps a share of the parts
-// each. Bound by the way to a part and back, 4 parts at once: 6 to 8 us with nothing in the caches, of which
-// the launch is hidden behind the kernel before.
+// each. Bound by the way to a part and back, 4 parts at once: with nothing in the caches 5 to 6 us after steps, 14
+// after 3 chunks and 18 after an 8k prompt (5000 CTAs of which most find no part), of which the launch is
+// hidden behind the kernel before.
 constexpr int kJoinWarps = 8;
 
 template <typename T, int D, bool WIDE>
@@ -764,8 +766,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
 // ---- many rows: chunks and prompts --------------------------------------------------------
 //
 // Sequences that the kernel above does not take. 4 D operations a query head and visible token, in two
-// products of fp16 operands with 32-bit sums in tensor memory: 0.66 to 0.70 ms for an 8k prompt of 32 heads
-// of 128, 790 to 830 TFLOP/s, half of what a plain product reaches. What bounds it are the softmax warps: the
+// products of fp16 operands with 32-bit sums in tensor memory: 0.67 to 0.71 ms for an 8k prompt of 32 heads
+// of 128, 770 to 820 TFLOP/s, half of what a plain product reaches. What bounds it are the softmax warps: the
 // weights' exponentials and what surrounds them take about 1900 clocks a step of both row tiles, the
 // tensor cores' part 1300. Chunks that do not fill 256 rows pay for the rows that they lack.
 // A CTA takes 256 rows (two tiles of 128) of one KV head in steps of 64 tokens:
@@ -779,8 +781,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
 // (4 x 64). With one step of 128 tokens instead, scores and softmax took turns: 1.02 ms for an 8k
 // prompt of 32 heads.
 // The running maximum follows a row's true maximum only when that exceeds it by 2^14 (weights stay
-// within fp16), so sums in tensor memory are rarely touched (followed at every step: an 8k prompt 738 us,
-// so 662). A page's scale goes into the conversion relative to the largest of its step, where e4m3's
+// within fp16), so sums in tensor memory are rarely touched (followed at every step: an 8k prompt 780 us,
+// so 669). A page's scale goes into the conversion relative to the largest of its step, where e4m3's
 // 9 fraction bits below 1 leave fp16 room: keys down to 2^-14, values down to 2^-6. The step's key scale
 // multiplies S, its value scale the weights, relative to a running maximum of their products (a row's e:
 // O 2^e are the sums). Steps whose pages lie further apart take their pages' own scales into
@@ -792,8 +794,8 @@ constexpr int kStep = 64;                  // tokens a step
 constexpr int kGranules = kStep / kGranule;
 constexpr int kStages = 4;                 // steps of keys and of values in shared memory
 // What a unit costs besides its steps (queries in, sums out, the pipeline's filling), in steps: work is
-// cut by steps and this (by steps alone an 8k prompt takes 778 us, so 662: a CTA with many short units was
-// 1.6 times as long as others).
+// cut by steps and this (by steps alone an 8k prompt takes 770 us, so 669, and 24 chunks of 128 tokens 270, so
+// 185: a CTA with many short units was 1.6 times as long as others).
 constexpr int kUnitCost = 8;
 constexpr int kConvertWarps = 4, kIssueWarp = 12, kLookWarp = 13, kChunkThreads = 512;
 constexpr int kLooked = 16;                // steps looked up ahead
@@ -1913,9 +1915,9 @@ Plan plan_for(const Cache& c, const Batch& b, int q_heads, int sms) {
     plan.step_rows = plan.stepped ? kStepRows : 0;
     plan.wide = most_rows > 8;
     // Heads a CTA: up to 8, whose lines of a token lie side by side; but few sequences are spread over CTAs by
-    // heads, so that a unit's tokens are cut among fewer CTAs (of 8 heads, 1 sequence of 8191 tokens takes
-    // 15.1 us, with all heads in a CTA 21.0, and 16 sequences 60.5 and 66.5; with a head a CTA 48 sequences
-    // of 4000 take 87.5, and 81.9 by this rule, 64 of 200 29.4 and 17.0).
+    // heads, so that a unit's tokens are cut among fewer CTAs (of 8 heads on 148 SMs, 1 sequence of 8191 tokens
+    // takes 17.1 us, with all heads in a CTA 22.4, and 16 sequences 58.0 and 63.6; with a head a CTA 16 sequences
+    // take 54.0, 48 of 4000 85.4, and 79.4 by this rule, 64 of 200 31.2 and 18.8).
     p.hc = 1;
     for (int heads = 8; heads > 1; --heads)
         if (c.kv_heads % heads == 0 && int64_t(b.seqs) * (c.kv_heads / heads) >= kSpread) {
@@ -1928,9 +1930,10 @@ Plan plan_for(const Cache& c, const Batch& b, int q_heads, int sms) {
     plan.step_units = int64_t(b.seqs) * p.hg;
     // Cutting the chunks evenly over the CTAs costs a scan of the lengths, merges of parts and a join: as
     // much as 4 chunks in turn, more with more units, up to 20. It saves at most the longest unit's chunks
-    // less an even share, taken at half of what the table could hold. Cut and uncut, in us: 1 sequence of
-    // 4000 tokens 15.2 and 23.4; 64 of 300 21.3 and 19.1, of 1000 38.7 and 41.7, of mixed lengths up to 1000
-    // 27.3 and 39.6; 128 of 700 48.7 and 40.1; 200 of 700 65.6 and 69.6.
+    // less an even share, taken at half of what the table could hold: the lengths are on the GPU, so over a table
+    // much wider than its sequences steps are cut that would be quicker whole. Cut and uncut, in us: 1 sequence
+    // of 4000 tokens 16.3 and 25.2; 64 of 300 23.3 and 21.0, of 1000 38.4 and 43.5, of mixed lengths up to 1000
+    // 28.1 and 41.6; 128 of 700 47.9 and 40.3; 200 of 700 65.6 and 70.7.
     const int64_t waves = (plan.step_units + sms - 1) / sms;
     const int64_t costs = 4 + (plan.step_units < 96 ? plan.step_units : 96) / 6;
     plan.split = most_rows > 0 && most * (2 * sms * waves - plan.step_units) > costs * 2 * sms;
@@ -1967,14 +1970,14 @@ void launch_attend(const Plan& plan, const AttendArgs& a, char* workspace, cudaS
         if (plan.wide) launch_step<T, D, 2>(plan, p, stream);
         else launch_step<T, D, 1>(plan, p, stream);
     }
-    // Without a wait between the two, and one join for both, batches of steps and chunks gain 4 to 10 % (16
-    // sequences of up to 4000 tokens and 9 new ones 65.8 us, one kernel after the other 72.5).
+    // Without a wait between the two, batches of steps and chunks gain 6 % (16 sequences of up to 4000 tokens, with
+    // 1 and 9 new ones by turns, 64.5 us; one kernel after the other 68.4).
     if (plan.chunked)
         launch(chunk_kernel<T, D>, dim3(ctas), kChunkThreads, sizeof(ChunkShared<D>) + 1024, stream, plan.stepped,
                ChunkArgs{a, of_chunks});
     if (!plan.slots) return;
-    // Few units have many parts each, and a CTA joins a row (8 units' 8191 tokens 15.1 us, a warp a row 17.0);
-    // many have few, as chunks do, and a warp does (chunks of 128 tokens in 24 sequences 282 us, a CTA a row 360).
+    // Few units have many parts each, and a CTA joins a row (8 units' 8191 tokens 17.1 us, a warp a row 18.9);
+    // many have few, as chunks do, and a warp does (chunks of 128 tokens in 24 sequences 185 us, a CTA a row 269).
     const bool wide = !plan.chunked && plan.step_units * 8 <= plan.ctas;
     const auto high = [&](const Parts& p) {
         const unsigned rows = unsigned(p.heads * p.used_rows);

@@ -25,7 +25,7 @@ struct PageRun {
     int row;                  // token row of slot `first`
 };
 
-// Unit u's page. Sequence s's units start at start[s] / N + 2 s, which leaves each
+// Unit u's page, its positions in 32 bits (a table row holds at most 2^30 tokens). Sequence s's units start at start[s] / N + 2 s, which leaves each
 // sequence room for the pages that its rows can touch ((rows - 2) / N + 2), whatever
 // slot they start in, so a unit finds its sequence by bisection with no scan over
 // the batch. With one row a sequence (SINGLE) unit u is sequence u.

@@ -186,3 +186,13 @@ def test_nan_queries_and_keys_reach_who_they_concern(sequences):
     expected[final, :4] = 0
     bound = bound.nan_to_num(1.0)
     assert ((got - expected).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("sequences", [[(1, 700), (1, 20)], [(1, 40)] * 70, [(300, 200), (2, 90), (40, 0)]], ids=["cut", "whole", "chunks"])
+def test_the_output_may_be_the_query(sequences):
+    p = Paged(sequences, heads=2, dim=64)
+    q = p.random(8, torch.bfloat16)[1].contiguous()
+    expected = p.cache.attend("l", q, p.batch)
+    assert p.cache.attend("l", q, p.batch, out=q) is q
+    p.cache.check()
+    assert torch.equal(q, expected)
