@@ -768,7 +768,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
 // Sequences that the kernel above does not take. 4 D operations a query head and visible token, in two
 // products of fp16 operands with 32-bit sums in tensor memory: 0.67 to 0.71 ms for an 8k prompt of 32 heads
 // of 128, 770 to 820 TFLOP/s, half of what a plain product reaches. What bounds it are the softmax warps: the
-// weights' exponentials and what surrounds them take about 1900 clocks a step of both row tiles, the
+// weights' exponentials and what surrounds them take about 1980 clocks a step of both row tiles, the
 // tensor cores' part 1300. Chunks that do not fill 256 rows pay for the rows that they lack.
 // A CTA takes 256 rows (two tiles of 128) of one KV head in steps of 64 tokens:
 //   warp 13     looks up the pages of coming steps and their scales;
