@@ -63,9 +63,12 @@ SHAPES = [(128, 16, 2, 4), (64, 32, 3, 2)]            # head_dim, block_size, kv
 @pytest.mark.parametrize("sequences", [[(1, 530)], [(1, 900), (1, 85), (2, 300)], [(45, 530)], [(150, 20), (30, 700)]],
                          ids=str)
 @pytest.mark.parametrize("place", ["first", "some"])
-@pytest.mark.parametrize("above,below", [(16, 87), (30, 87), (30, 30), (100, 110), (7, 9)])
+@pytest.mark.parametrize("above,below", [(16, 87), (30, 87), (30, 30), (100, 110), (7, 9), (64, 1), (100, 9)])
 def test_a_large_page_of_little_weight(shape, sequences, place, above, below):
-    """Pages 2^above larger than the others whose tokens weigh about 2^-below of them."""
+    """Pages 2^above larger than the others whose tokens weigh about 2^-below of them.
+
+    Where they make up the result, the others still count in the softmax.
+    """
     dim, block_size, heads, group = shape
     p = Paged(sequences, dim=dim, block_size=block_size, heads=heads, seed=7)
     codes, scales = p.codes(), torch.full_like(p.scales(), 2.0 ** (-60 if above > 60 else -9))
